@@ -229,6 +229,91 @@ int mscclx_plan_run_static(mscclx_plan* plan, void* const* in, void* const* out,
 /* Times `iters` back-to-back launches with HIP events on `stream`; ms_out[i] = duration of launch i. */
 int mscclx_plan_time(mscclx_plan* plan, void* stream, int32_t iters, float* ms_out);
 
+/* ---- operators of a training step that stand beside its collectives ----------------------------------------------- */
+
+/* Softmax cross entropy over a vocabulary that is cut into the ranks' pieces, and its gradients.  No counterpart in
+ * msccl-tools.  Rank r holds rank_rows[r] rows of the output matrix; row v of the whole vocabulary is the v-th row of the
+ * ranks' pieces one under the other.  With z[n][v] = sum over d of x[n][d] w[v][d]:
+ *   lse[n] = log sum over v of exp z[n][v],  loss[n] = lse[n] - z[n][label[n]]
+ *   dx[n] = sum over v of G[n][v] w[v],  dw[v] = sum over n of G[n][v] x[n],  G[n][v] = g[n] (exp(z[n][v] - lse[n]) - [v = label[n]])
+ * The logits are never kept: tokens go through in pieces whose probabilities fit `piece_bytes`.
+ * A token whose label is `ignore_index` has loss 0 and adds nothing to either gradient; one whose label lies outside the
+ * vocabulary otherwise has loss and gradients NaN (and every dw is NaN then).  MEAN divides by the number of tokens that are not
+ * ignored, or by 1 if all are.  A non-finite grad_loss gives non-finite gradients.
+ * Every call only enqueues kernels on `stream`: it can be captured in a HIP graph and replayed.  Calls that share a
+ * workspace must follow each other on one stream (or be ordered by events). */
+#define MSCCLX_VOCAB_LOSS_MAX_RANKS 64
+#define MSCCLX_VOCAB_LOSS_MAX_STRIDE (1 << 22)
+#define MSCCLX_VOCAB_LOSS_PIECE_BYTES (2ull << 30)
+typedef enum { MSCCLX_LOSS_NONE = 0, MSCCLX_LOSS_SUM = 1, MSCCLX_LOSS_MEAN = 2 } mscclx_loss_reduction;
+
+typedef struct {
+  int32_t ranks;
+  int32_t hidden;           /* a multiple of 8                                                                */
+  const int64_t* rank_rows; /* rows of each rank's piece, 0 allowed; read by create only                      */
+  int64_t max_tokens;
+  int32_t dtype;            /* MSCCLX_BF16 or MSCCLX_F16: x, weights and gradients                            */
+  int32_t reduction;        /* mscclx_loss_reduction                                                          */
+  int64_t ignore_index;
+  uint64_t piece_bytes;     /* room for a piece's probabilities in the workspace; 0: MSCCLX_VOCAB_LOSS_PIECE_BYTES. A piece has at least 256 tokens */
+  int32_t gradients;        /* 0: forward only, a smaller workspace                                           */
+  int32_t reserved;
+} mscclx_vocab_loss_desc;
+
+typedef struct {
+  int64_t tokens;              /* at most max_tokens; 0 is allowed                                            */
+  const void* x;               /* [tokens][hidden], rows x_stride elements apart (a multiple of 8, 16-byte aligned) */
+  int64_t x_stride;
+  const void* const* weights;  /* per rank [rank_rows][hidden], rows weight_stride elements apart              */
+  int64_t weight_stride;
+  const void* labels;          /* [tokens], 32- or 64-bit integers                                            */
+  int32_t label_bytes;
+  int32_t reserved;
+  float* loss;                 /* NONE: [tokens], else one number                                             */
+  float* lse;                  /* [tokens]: written by forward and run, read by backward                      */
+  const float* grad_loss;      /* NONE: [tokens], else one number                                             */
+  void* dx;                    /* [tokens][hidden]; must not overlap any other buffer                         */
+  int64_t dx_stride;
+  void* const* dweights;       /* per rank [rank_rows][hidden]                                                */
+  int64_t dweight_stride;
+  void* workspace;             /* 256-byte aligned                                                            */
+  uint64_t workspace_bytes;
+} mscclx_vocab_loss_io;
+
+typedef struct mscclx_vocab_loss mscclx_vocab_loss;
+
+/* Uses no GPU.  *workspace_bytes: what every call needs; *piece_tokens: tokens per piece. */
+int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_loss** out, uint64_t* workspace_bytes, int64_t* piece_tokens);
+int mscclx_vocab_loss_destroy(mscclx_vocab_loss* loss);
+/* loss and lse. */
+int mscclx_vocab_loss_forward(const mscclx_vocab_loss* loss, const mscclx_vocab_loss_io* io, void* stream);
+/* dx and dweights from x, weights, labels, lse and grad_loss; computes the probabilities again. */
+int mscclx_vocab_loss_backward(const mscclx_vocab_loss* loss, const mscclx_vocab_loss_io* io, void* stream);
+/* Both in one call, which computes the probabilities once. */
+int mscclx_vocab_loss_run(const mscclx_vocab_loss* loss, const mscclx_vocab_loss_io* io, void* stream);
+
+/* The global norm of the gradients in many tensors, and clipping by it.  No counterpart in msccl-tools.
+ *   norm = |scale| sqrt(sum g^2) (L2) or |scale| max |g| (MAX), over the elements of all counted tensors
+ *   coefficient = min(1, max_norm / (norm + 1e-6)),  out = g scale coefficient
+ * Sums are held in 64 bits and added in one order: the same bits at every call.  A NaN among the gradients makes norm,
+ * coefficient and every output NaN; an infinity makes the coefficient 0 (and NaN of itself).  Without tensors the norm is 0. */
+typedef enum { MSCCLX_NORM_L2 = 0, MSCCLX_NORM_MAX = 1 } mscclx_norm;
+typedef struct mscclx_grad_clip mscclx_grad_clip;
+
+/* sizes[i] elements (0 allowed) of in_dtypes[i], clipped into out_dtypes[i]: MSCCLX_F32, MSCCLX_F16 or MSCCLX_BF16 each.
+ * counted[i] = 0 (NULL: all count): the tensor is scaled but not part of the norm, as the copies of a gradient that several ranks hold after an
+ * all-reduce are.  Uses no GPU. */
+int mscclx_grad_clip_create(int32_t ntensors, const uint64_t* sizes, const int32_t* in_dtypes, const int32_t* out_dtypes, const uint8_t* counted,
+                            int32_t norm, mscclx_grad_clip** out, uint64_t* workspace_bytes);
+int mscclx_grad_clip_destroy(mscclx_grad_clip* clip);
+/* Uploads the table of tensors into the workspace and waits for it.  Buffers start on a boundary of their element type.
+ * out = NULL: norms only; out[i] = in[i]: in place.  Otherwise no output may overlap another buffer (ALIASED).  Not while a launch of
+ * the previous binding is in flight, and not while `stream` is being captured. */
+int mscclx_grad_clip_bind(mscclx_grad_clip* clip, const void* const* in, void* const* out, void* workspace, uint64_t workspace_bytes, void* stream);
+/* Enqueues two kernels on `stream`; can be captured in a HIP graph.  max_norm < 0: the norm only.  The results are the two floats at
+ * the start of the workspace: norm, coefficient.  Launches of one binding must follow each other on one stream. */
+int mscclx_grad_clip_launch(const mscclx_grad_clip* clip, float scale, float max_norm, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,6 +1,6 @@
 """Builds libmscclx.so (gfx950) in-tree with hipcc.  Run: python build.py [--force] [--flags "-DX ..."] [--out PATH]
 
-The kernels (exec_device.h) are compiled as five translation units of two element types each
+The step kernels (exec_device.h) are compiled as five translation units of two element types each
 (exec_kernels.hip with -DMSCCLX_KERNEL_GROUP=0..4), in parallel with the host sources."""
 import os
 import subprocess
@@ -10,8 +10,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 LIB = os.path.join(HERE, "libmscclx.so")
 KERNEL_GROUPS = 5
-SOURCES = ["plan.cpp", "exec.hip", "exec_kernels.hip"]
-HEADERS = ["plan.h", "exec_device.h", os.path.join(ROOT, "include", "mscclx.h")]
+OPERATORS = ["vocab_loss", "grad_clip"]
+SOURCES = ["plan.cpp", "exec.hip", "exec_kernels.hip"] + [o + ".hip" for o in OPERATORS]
+HEADERS = ["plan.h", "exec_device.h", "tile_product.h", os.path.join(ROOT, "include", "mscclx.h")]
 
 
 def hipcc():
@@ -40,6 +41,7 @@ def build(force=True, verbose=True, extra_flags=(), out=None):
     tag = "" if out is None else "." + os.path.splitext(os.path.basename(out))[0]
     jobs = [("plan.cpp", ["-x", "c++"], "plan" + tag + ".o"), ("exec.hip", device, "exec" + tag + ".o")]
     jobs += [("exec_kernels.hip", device + [f"-DMSCCLX_KERNEL_GROUP={g}"], f"exec_kernels_{g}{tag}.o") for g in range(KERNEL_GROUPS)]
+    jobs += [(o + ".hip", device, o + tag + ".o") for o in OPERATORS]
     objs = []
     procs = []
     for src, flags, obj in jobs:

@@ -10,6 +10,12 @@ def __getattr__(name):
     if name in ("Executor", "collective_buffers", "dtype_name"):
         from . import runner
         return getattr(runner, name)
+    if name == "VocabLoss":
+        from .vocab_loss import VocabLoss
+        return VocabLoss
+    if name == "GradientClip":
+        from .grad_clip import GradientClip
+        return GradientClip
     if name in ("executor_for", "tables_for"):
         from . import cache
         return getattr(cache, name)

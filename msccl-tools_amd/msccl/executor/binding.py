@@ -33,6 +33,8 @@ EXPORTED_SYMBOLS = (
     "mscclx_plan_min_fifo_depth", "mscclx_plan_algorithmic_units", "mscclx_plan_configure", "mscclx_plan_bind",
     "mscclx_plan_launch", "mscclx_plan_wait", "mscclx_plan_poll", "mscclx_plan_abort", "mscclx_plan_time",
     "mscclx_plan_run_static",
+    "mscclx_vocab_loss_create", "mscclx_vocab_loss_destroy", "mscclx_vocab_loss_forward", "mscclx_vocab_loss_backward", "mscclx_vocab_loss_run",
+    "mscclx_grad_clip_create", "mscclx_grad_clip_destroy", "mscclx_grad_clip_bind", "mscclx_grad_clip_launch",
 )
 
 
@@ -79,6 +81,21 @@ class Status(ctypes.Structure):
                 ("pass_", ctypes.c_int64), ("waiting_on", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+class VocabLossDesc(ctypes.Structure):
+    _fields_ = [("ranks", ctypes.c_int32), ("hidden", ctypes.c_int32), ("rank_rows", ctypes.POINTER(ctypes.c_int64)), ("max_tokens", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("reduction", ctypes.c_int32), ("ignore_index", ctypes.c_int64), ("piece_bytes", ctypes.c_uint64),
+                ("gradients", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class VocabLossIO(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+                ("weights", ctypes.POINTER(ctypes.c_void_p)), ("weight_stride", ctypes.c_int64),
+                ("labels", ctypes.c_void_p), ("label_bytes", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("loss", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("grad_loss", ctypes.c_void_p),
+                ("dx", ctypes.c_void_p), ("dx_stride", ctypes.c_int64), ("dweights", ctypes.POINTER(ctypes.c_void_p)), ("dweight_stride", ctypes.c_int64),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
 _lib = None
 
 
@@ -112,9 +129,18 @@ def load_library(path=None):
     lib.mscclx_plan_time.argtypes = [vp, vp, i32, ctypes.POINTER(ctypes.c_float)]
     lib.mscclx_plan_run_static.argtypes = [vp, ctypes.POINTER(vp), ctypes.POINTER(vp), ctypes.POINTER(vp), vp, ctypes.POINTER(Status)]
     lib.mscclx_plan_run_static.restype = ctypes.c_int
+    ptr = ctypes.POINTER
+    lib.mscclx_vocab_loss_create.argtypes = [ptr(VocabLossDesc), ptr(vp), ptr(u64), ptr(ctypes.c_int64)]
+    lib.mscclx_vocab_loss_destroy.argtypes = [vp]
+    for name in ("forward", "backward", "run"):
+        getattr(lib, f"mscclx_vocab_loss_{name}").argtypes = [vp, ptr(VocabLossIO), vp]
+    lib.mscclx_grad_clip_create.argtypes = [i32, ptr(u64), ptr(i32), ptr(i32), ptr(ctypes.c_uint8), i32, ptr(vp), ptr(u64)]
+    lib.mscclx_grad_clip_destroy.argtypes = [vp]
+    lib.mscclx_grad_clip_bind.argtypes = [vp, ptr(vp), ptr(vp), vp, u64, vp]
+    lib.mscclx_grad_clip_launch.argtypes = [vp, ctypes.c_float, ctypes.c_float, vp]
     for name in ("mscclx_plan_create", "mscclx_plan_destroy", "mscclx_plan_simulate", "mscclx_plan_min_fifo_depth",
                  "mscclx_plan_configure", "mscclx_plan_bind", "mscclx_plan_launch", "mscclx_plan_wait", "mscclx_plan_poll",
-                 "mscclx_plan_abort", "mscclx_plan_time"):
+                 "mscclx_plan_abort", "mscclx_plan_time") + tuple(s for s in EXPORTED_SYMBOLS if "vocab_loss" in s or "grad_clip" in s):
         getattr(lib, name).restype = ctypes.c_int
     if path is None:
         _lib = lib
