@@ -160,22 +160,44 @@ struct TileProduct {
       p = sr.step(s, &k_left);
       rl.copy(at + LLanes::kBytes, p, k_left);
     };
-    if (steps > 0) issue(0);
-    for (int s = 0; s < steps; ++s) {
-      // the copies of this step have arrived, and every wave is done with the other buffer
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (s + 1 < steps) issue(s + 1);
+    auto read = [&](int s, int kk, i16x8 (&a)[FL], i16x8 (&b)[FR]) {
       const char* at = smem + (s & 1) * kStage;
+      fragments<RCOL, TR, FR>(at + LLanes::kBytes, r0, kk, lane, b);
+      fragments<LCOL, TL, FL>(at, l0, kk, lane, a);
+    };
+    auto multiply = [&](const i16x8 (&a)[FL], const i16x8 (&b)[FR]) {
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        i16x8 a[FL], b[FR];
-        fragments<LCOL, TL, FL>(at, l0, kk, lane, a);
-        fragments<RCOL, TR, FR>(at + LLanes::kBytes, r0, kk, lane, b);
+      for (int l = 0; l < FL; ++l)
 #pragma unroll
-        for (int l = 0; l < FL; ++l)
+        for (int r = 0; r < FR; ++r) acc[l][r] = Half<T>::mfma(a[l], b[r], acc[l][r]);
+    };
+    // a read from LDS, then a few products, and so on: neither waits for the other
+    auto interleave = [&] {
+      constexpr int kReads = FL * (LCOL ? 2 : 1) + FR * (RCOL ? 2 : 1), kEach = FL * FR / kReads;
 #pragma unroll
-          for (int r = 0; r < FR; ++r) acc[l][r] = Half<T>::mfma(a[l], b[r], acc[l][r]);
+      for (int i = 0; i < kReads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
       }
+      __builtin_amdgcn_sched_group_barrier(0x008, FL * FR - kReads * kEach, 0);
+    };
+    if (steps <= 0) return;
+    i16x8 a0[FL], b0[FR], a1[FL], b1[FR];  // fragments of the step's first and second 32 values of k
+    issue(0);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (steps > 1) issue(1);
+    read(0, 0, a0, b0);
+    for (int s = 0; s < steps; ++s) {
+      read(s, 1, a1, b1);
+      multiply(a0, b0);
+      interleave();
+      // the copies of the next step have arrived, and every wave has read all of this one: its buffer takes the step after next
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      if (s + 2 < steps) issue(s + 2);
+      read(s + 1, 0, a0, b0);  // (behind the last step: what the other buffer holds, for nothing)
+      multiply(a1, b1);
+      interleave();
     }
   }
 };
