@@ -68,6 +68,7 @@ struct Lanes {
   static constexpr int kChunks = kBytes / kChunk;
   static constexpr int kUnitsPerLine = COL ? TILE / 8 : 8;       // 16-byte units of a line of LDS
   static constexpr int kLines = WAVES * 64 / kUnitsPerLine;      // lines per chunk
+  static_assert(kChunks >= 1 && (COL ? TILE >= 128 : kLines % 16 == 0), "a copy covers whole swizzle patterns");
   unsigned offset[kChunks];
   int k[COL ? kChunks : 1];                                      // the lane's k (its first) in the step
 
@@ -117,14 +118,16 @@ struct ColSource {  // k strided
   }
 };
 
-template <class T, int TL, int TR, int WL, int WR, bool LCOL, bool RCOL>
+// TL x TR: the workgroup's tile, cut among WL x WR waves; STAGES: steps held in LDS, a power of two.
+template <class T, int TL, int TR, int WL, int WR, int STAGES, bool LCOL, bool RCOL>
 struct TileProduct {
   static constexpr int kWaves = WL * WR, kThreads = kWaves * 64;
   static constexpr int FL = TL / WL / 16, FR = TR / WR / 16;  // fragments of a wave
   typedef Lanes<LCOL, TL, kWaves> LLanes;
   typedef Lanes<RCOL, TR, kWaves> RLanes;
   static constexpr int kStage = LLanes::kBytes + RLanes::kBytes;
-  static constexpr int kLdsBytes = 2 * kStage;
+  static constexpr int kLdsBytes = STAGES * kStage;
+  static constexpr int kCopies = LLanes::kChunks + RLanes::kChunks;  // of a wave, per step
 
   template <bool COL, int TILE, int F>
   static __device__ __forceinline__ void fragments(const char* lds, int first, int kk, int lane, i16x8 (&out)[F]) {
@@ -154,14 +157,14 @@ struct TileProduct {
     const unsigned lds = (unsigned)(uintptr_t)(lds_char)smem + wave * 1024;
     auto issue = [&](int s) {
       int k_left;
-      const unsigned at = lds + (s & 1) * kStage;
+      const unsigned at = lds + s % STAGES * kStage;
       const char* p = sl.step(s, &k_left);
       ll.copy(at, p, k_left);
       p = sr.step(s, &k_left);
       rl.copy(at + LLanes::kBytes, p, k_left);
     };
     auto read = [&](int s, int kk, i16x8 (&a)[FL], i16x8 (&b)[FR]) {
-      const char* at = smem + (s & 1) * kStage;
+      const char* at = smem + s % STAGES * kStage;
       fragments<RCOL, TR, FR>(at + LLanes::kBytes, r0, kk, lane, b);
       fragments<LCOL, TL, FL>(at, l0, kk, lane, a);
     };
@@ -173,29 +176,35 @@ struct TileProduct {
     };
     // a read from LDS, then a few products, and so on: neither waits for the other
     auto interleave = [&] {
-      constexpr int kReads = FL * (LCOL ? 2 : 1) + FR * (RCOL ? 2 : 1), kEach = FL * FR / kReads;
+      constexpr int kReads = FL * (LCOL ? 2 : 1) + FR * (RCOL ? 2 : 1), kEach = FL * FR / kReads > 0 ? FL * FR / kReads : 1;
 #pragma unroll
       for (int i = 0; i < kReads; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x008, FL * FR - kReads * kEach, 0);
+      if constexpr (FL * FR > kReads * kEach) __builtin_amdgcn_sched_group_barrier(0x008, FL * FR - kReads * kEach, 0);
     };
     if (steps <= 0) return;
     i16x8 a0[FL], b0[FR], a1[FL], b1[FR];  // fragments of the step's first and second 32 values of k
-    issue(0);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    if (steps > 1) issue(1);
+    // Copies arrive in order: with the next STAGES - 2 steps' copies behind them, the awaited step's are there once no more are under way.
+    // Where the last steps are not followed by others, everything is waited for.
+    constexpr int kBehind = (STAGES - 2) * kCopies;
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s)
+      if (s < steps) issue(s);
+    if (steps >= STAGES) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kBehind + kCopies) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     read(0, 0, a0, b0);
     for (int s = 0; s < steps; ++s) {
       read(s, 1, a1, b1);
       multiply(a0, b0);
       interleave();
-      // the copies of the next step have arrived, and every wave has read all of this one: its buffer takes the step after next
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      // the copies of the next step have arrived, and every wave has read all of this one: its buffer takes the step STAGES further
+      if (STAGES > 2 && s + STAGES <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kBehind) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
-      if (s + 2 < steps) issue(s + 2);
-      read(s + 1, 0, a0, b0);  // (behind the last step: what the other buffer holds, for nothing)
+      if (s + STAGES < steps) issue(s + STAGES);
+      read(s + 1, 0, a0, b0);  // (behind the last step: what that buffer holds, for nothing)
       multiply(a1, b1);
       interleave();
     }

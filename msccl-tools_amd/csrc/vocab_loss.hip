@@ -5,11 +5,11 @@
 //   G[n][v]  = g[n] (exp(z[n][v] - lse[n]) - [v = label[n]]),   dx = G w,   dw = transposed(G) x
 //
 // Tokens go through in pieces of at most `piece` rows; per piece, three products on the matrix cores (tile_product.h):
-//   logits   z of a tile of vocabulary x tokens stays in registers; what leaves are, for each token and each half tile of the
+//   logits   z of a tile of vocabulary x tokens stays in registers; what leaves are, for each token and each wave's part of the
 //            vocabulary, the maximum m and the sum of exp(z - m), and with gradients E = exp(z - m) in 16 bits;
-//   join     the pieces' (m, sum) become the token's lse;
-//   scale    E becomes G in place: G = (E exp(m - lse) - [label]) g / max|g|;
-//   dx, dw   the two products, on G.
+//   tokens   a token's (m, sum) become its lse and loss, and its E becomes G in place: G = (E exp(m - lse) - [label]) g / max|g|;
+//   dx, dw   the two products, on G.  dx sums over the whole vocabulary: where its tiles do not fill the chip, that
+//            axis is cut and the parts are added by a kernel of their own.
 // The 16-bit E and G are what the matrix cores take.  Both are rounded relative to their own size (bf16 2^-9 on average, as the outputs
 // are), with 2^15 as unit in fp16, so that probabilities down to 2^-29 are normal numbers; |g| is divided by its largest value for
 // the same reason and multiplied back in 32 bits behind the products.
@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 #include <new>
 #include <string>
@@ -30,7 +31,7 @@ namespace mscclx {
 namespace {
 
 constexpr int kMaxRanks = MSCCLX_VOCAB_LOSS_MAX_RANKS;
-constexpr int kTile = 256;              // vocabulary, tokens and hidden of a workgroup's tile
+constexpr int kTile = 256;              // rows of the vocabulary: a rank's piece is padded to whole tiles of G
 constexpr float kLog2e = 1.4426950408889634f;
 
 // The ranks' pieces of the vocabulary, passed to the kernels by value.  Tiles of kTile rows; none spans two ranks.
@@ -62,8 +63,29 @@ struct Labels {
   }
 };
 
+// A token's g / max |g|: kept in `factor` where every token has its own, else the sign of the one number.
+struct Upstream {
+  const float* at;
+  const float* factor;  // null: one number for all
+  __device__ __forceinline__ float get(int64_t n, int label) const {
+    if (factor) return factor[n];
+    const float g = *at;
+    return label == -1 ? 0.f : label < 0 ? NAN : g == 0.f ? 0.f : g / fabsf(g);
+  }
+};
+
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 template <class T> constexpr float kUnit = std::is_same_v<T, _Float16> ? 32768.0f : 1.0f;
+
+// How a workgroup's tile is cut.  Large: one workgroup of eight waves per compute unit.  Middle: two of four waves, for products whose large tiles
+// would not fill the chip.  Few: at most 32 tokens, with four steps of copies under way, because then memory is all that counts.
+template <int L, int R, int WL, int WR, int STAGES> struct Shape {
+  static constexpr int kL = L, kR = R, kWavesL = WL, kWavesR = WR, kThreads = WL * WR * 64;
+  template <class T, bool LCOL, bool RCOL> using Product = TileProduct<T, L, R, WL, WR, STAGES, LCOL, RCOL>;
+};
+typedef Shape<256, 256, 2, 4, 2> Large;
+typedef Shape<128, 128, 2, 2, 2> Middle;
+typedef Shape<128, 32, 4, 1, 4> Few;
 
 enum { kStats = 0, kKeep = 1, kGradient = 2 };
 
@@ -72,14 +94,13 @@ struct LogitsArgs {
   int64_t x_stride;  // bytes
   int64_t w_stride;
   int hidden, tokens, token_tiles;
-  int64_t token0;    // of the labels, lse and factor
+  int64_t token0;    // of the labels, lse and factors
   Labels labels;
-  float2* stats;     // [2 * tiles][ld_stats]
-  int64_t ld_stats;
+  Upstream upstream;
+  float2* stats;     // [tokens][waves' parts of the vocabulary]
   float* z_label;
   void* e;           // [tokens][tiles * kTile]
   const float* lse;
-  const float* factor;
 };
 
 // Tiles in an order that keeps the workgroups of one XCD (every eighth of the grid) on neighbouring tiles: columns of
@@ -92,16 +113,18 @@ __device__ __forceinline__ void tile_of(int id, int rows, int cols, int* row, in
   *col = in / high;
 }
 
-template <class T, int MODE>
-__global__ void __launch_bounds__(512, 2) logits_kernel(const Pieces pieces, const LogitsArgs a) {
-  typedef TileProduct<T, kTile, kTile, 2, 4, false, false> Product;
+template <class T, int MODE, class Shape>
+__global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces pieces, const LogitsArgs a) {
+  typedef typename Shape::template Product<T, false, false> Product;
+  constexpr int TL = Shape::kL, TR = Shape::kR, kPart = TL / Shape::kWavesL;  // vocabulary of a wave
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
-  int tt, vt;
-  tile_of(blockIdx.x, a.token_tiles, pieces.tiles, &tt, &vt);
-  const int rank = pieces.rank_of(vt), row0 = (vt - pieces.tile0[rank]) * kTile, rows = min(kTile, pieces.rows[rank] - row0);
-  const int n0 = tt * kTile, tokens = min(kTile, a.tokens - n0);
+  int tt, at;
+  tile_of(blockIdx.x, a.token_tiles, pieces.tiles * (kTile / TL), &tt, &at);
+  const int vt = at / (kTile / TL), rank = pieces.rank_of(vt), row0 = at * TL - pieces.tile0[rank] * kTile;
+  const int rows = min(TL, pieces.rows[rank] - row0);  // none or less: the tile is padding
+  const int n0 = tt * TR, tokens = min(TR, a.tokens - n0);
   f32x4 acc[Product::FL][Product::FR] = {};
-  {
+  if (rows > 0) {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
     ll.place(threadIdx.x, a.w_stride, rows);
@@ -109,7 +132,7 @@ __global__ void __launch_bounds__(512, 2) logits_kernel(const Pieces pieces, con
     Product::run(smem, (a.hidden + kStepK - 1) / kStepK, ll, RowSource{pieces.w[rank] + row0 * a.w_stride, a.hidden}, rl,
                  RowSource{a.x + n0 * a.x_stride, a.hidden}, acc);
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l0 = wave % 2 * 128, r0 = wave / 2 * 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l0 = wave % Shape::kWavesL * kPart, r0 = wave / Shape::kWavesL * (TR / Shape::kWavesR);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
   const int v0 = l0 + (lane >> 4) * 4;  // + 16 * l + i
 #pragma unroll
@@ -118,9 +141,9 @@ __global__ void __launch_bounds__(512, 2) logits_kernel(const Pieces pieces, con
     const bool live = n < tokens;
     const int label = live ? a.labels.get(a.token0 + n0 + n) : -1;
     const int want = label >= 0 ? label - pieces.first[rank] - row0 : -1;
-    typename Half<T>::x4* out = (typename Half<T>::x4*)((T*)a.e + (n0 + n) * ld + (int64_t)vt * kTile + v0);
+    typename Half<T>::x4* out = (typename Half<T>::x4*)((T*)a.e + (n0 + n) * ld + (int64_t)at * TL + v0);
     if constexpr (MODE == kGradient) {
-      const float lse = live ? a.lse[a.token0 + n0 + n] : 0.f, g = live ? a.factor[a.token0 + n0 + n] * kUnit<T> : 0.f;
+      const float lse = live ? a.lse[a.token0 + n0 + n] : 0.f, g = live ? a.upstream.get(a.token0 + n0 + n, label) * kUnit<T> : 0.f;
 #pragma unroll
       for (int l = 0; l < Product::FL; ++l) {
         typename Half<T>::x4 o;
@@ -146,7 +169,7 @@ __global__ void __launch_bounds__(512, 2) logits_kernel(const Pieces pieces, con
         }
       m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
-      const float base = m == -INFINITY ? 0.f : m;  // a half tile of nothing but -inf has sum 0
+      const float base = m == -INFINITY ? 0.f : m;  // a part of nothing but -inf has sum 0
       float sum = 0.f;
 #pragma unroll
       for (int l = 0; l < Product::FL; ++l) {
@@ -162,42 +185,10 @@ __global__ void __launch_bounds__(512, 2) logits_kernel(const Pieces pieces, con
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
       if (live) {
-        if (lane < 16) a.stats[(int64_t)(2 * vt + wave % 2) * a.ld_stats + n0 + n] = make_float2(m, sum);
+        if (lane < 16) a.stats[(n0 + n) * (ld / kPart) + (at * TL + l0) / kPart] = make_float2(m, sum);
         if (found) a.z_label[a.token0 + n0 + n] = z_label;
       }
     }
-  }
-}
-
-// (m, sum) of all half tiles -> lse and loss of 32 tokens; eight threads per token
-__global__ void __launch_bounds__(256) join_kernel(const float2* stats, int64_t ld_stats, int halves, int tokens, int64_t token0, Labels labels,
-                                                   const float* z_label, float* lse, float* loss) {
-  __shared__ float2 part[8][32];
-  const int n = blockIdx.x * 32 + threadIdx.x % 32, g = threadIdx.x / 32;
-  float m = -INFINITY, sum = 0.f;
-  if (n < tokens)
-    for (int h = g; h < halves; h += 8) {
-      const float2 s = stats[(int64_t)h * ld_stats + n];
-      const float top = fmaxf(m, s.x);
-      if (top == -INFINITY) sum += s.y;  // nothing yet: s.y is 0 or NaN
-      else sum = sum * exp_of(m - top) + s.y * exp_of(s.x - top);
-      m = top;
-    }
-  part[g][threadIdx.x % 32] = make_float2(m, sum);
-  __syncthreads();
-  if (g == 0 && n < tokens) {
-    for (int i = 1; i < 8; ++i) {
-      const float2 s = part[i][threadIdx.x];
-      const float top = fmaxf(m, s.x);
-      if (top == -INFINITY) sum += s.y;
-      else sum = sum * exp_of(m - top) + s.y * exp_of(s.x - top);
-      m = top;
-    }
-    const int64_t at = token0 + n;
-    const float v = m + logf(sum);
-    lse[at] = v;
-    const int label = labels.get(at);
-    loss[at] = label == -1 ? 0.f : label < 0 ? NAN : v - z_label[at];
   }
 }
 
@@ -212,74 +203,101 @@ template <class V, class F> __device__ __forceinline__ V block_reduce(V v, F f, 
   return v;
 }
 
-// the tokens' losses to one number, in 64 bits and in one order
-__global__ void __launch_bounds__(1024) total_kernel(const float* rows, int64_t tokens, Labels labels, int mean, float* loss) {
-  __shared__ double shared[16];
-  double sum = 0, count = 0;
-  for (int64_t n = threadIdx.x; n < tokens; n += 1024) {
-    sum += rows[n];
-    count += labels.get(n) != -1;
+struct TokenArgs {
+  const float2* stats;
+  int part;          // vocabulary of one entry
+  int64_t token0;
+  Labels labels;
+  Upstream upstream;
+  const float* z_label;
+  float *lse, *loss;
+  void* e;
+};
+
+// A workgroup per token: its parts' (m, sum) -> lse and loss; KEEP: its E -> G in place
+template <class T, bool KEEP>
+__global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const TokenArgs a) {
+  __shared__ float shared[4];
+  const int64_t ld = (int64_t)pieces.tiles * kTile, at = a.token0 + blockIdx.x;
+  const int parts = (int)(ld / a.part);
+  const float2* stats = a.stats + (int64_t)blockIdx.x * parts;
+  float m = -INFINITY, sum = 0.f;
+  for (int h = threadIdx.x; h < parts; h += 256) m = fmaxf(m, stats[h].x);
+  m = block_reduce(m, [](float a, float b) { return fmaxf(a, b); }, shared);
+  const float base = m == -INFINITY ? 0.f : m;
+  for (int h = threadIdx.x; h < parts; h += 256) {
+    const float2 s = stats[h];
+    sum += s.y * exp_of(s.x - base);
   }
-  auto add = [](double a, double b) { return a + b; };
-  sum = block_reduce(sum, add, shared);
-  count = block_reduce(count, add, shared);
-  if (threadIdx.x == 0) *loss = (float)(mean ? sum / fmax(count, 1.0) : sum);
+  sum = block_reduce(sum, [](float a, float b) { return a + b; }, shared);
+  const float lse = base + logf(sum);
+  const int label = a.labels.get(at);
+  if (threadIdx.x == 0) {
+    a.lse[at] = lse;
+    a.loss[at] = label == -1 ? 0.f : label < 0 ? NAN : lse - a.z_label[at];
+  }
+  if constexpr (KEEP) {
+    const float g = a.upstream.get(at, label);
+    int64_t want = -1;
+    if (label >= 0) {
+      int r = 0;
+      while (r + 1 < pieces.ranks && label >= pieces.first[r + 1]) ++r;
+      want = (int64_t)pieces.tile0[r] * kTile + label - pieces.first[r];
+    }
+    typedef typename Half<T>::x8 x8;
+    T* e = (T*)a.e + blockIdx.x * ld;
+    for (int64_t v = threadIdx.x * 8; v < ld; v += 256 * 8) {
+      const float top = stats[v / a.part].x;
+      const float f = top == -INFINITY ? 0.f : exp_of(top - lse) * g;
+      x8 o = *(x8*)(e + v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = (T)(g == 0.f ? 0.f : (float)o[i] * f - (v + i == want ? kUnit<T> * g : 0.f));
+      *(x8*)(e + v) = o;
+    }
+  }
 }
 
-// factor[n] = g[n] / max |g| and behind the factors, in back[0], what the products are multiplied by
-__global__ void __launch_bounds__(1024) factor_kernel(const float* upstream, int per_token, int64_t tokens, Labels labels, int mean, float unit,
-                                                      float* factor, float* back) {
-  __shared__ double wide[16];
-  __shared__ float narrow[16];
-  double count = 0;
+// One workgroup over all tokens: the loss as one number (rows given), in 64 bits and in one order; with gradients what the
+// products are multiplied by, max |g| (over the mean's count) over the unit, and with a number per token factor[n] = g[n] / max |g|.
+__global__ void __launch_bounds__(1024) sums_kernel(int64_t tokens, Labels labels, int mean, const float* rows, float* loss, const float* upstream, float* factor,
+                                                    float unit, float* back) {
+  __shared__ double shared[16];
+  double sum = 0, count = 0;
   float top = 0.f;
   for (int64_t n = threadIdx.x; n < tokens; n += 1024) {
     const int label = labels.get(n);
     count += label != -1;
-    if (label >= 0) top = fmaxf(top, fabsf(upstream[per_token ? n : 0]));
+    if (rows) sum += rows[n];
+    if (factor && label >= 0) top = fmaxf(top, fabsf(upstream[n]));
   }
-  count = block_reduce(count, [](double a, double b) { return a + b; }, wide);
-  top = block_reduce(top, [](float a, float b) { return fmaxf(a, b); }, narrow);
-  for (int64_t n = threadIdx.x; n < tokens; n += 1024) {
-    const int label = labels.get(n);
-    const float g = upstream[per_token ? n : 0];
-    factor[n] = label == -1 ? 0.f : label < 0 ? NAN : g == 0.f ? 0.f : g / top;
+  auto add = [](double a, double b) { return a + b; };
+  if (mean) count = fmax(block_reduce(count, add, shared), 1.0);
+  else count = 1.0;
+  if (rows) {
+    sum = block_reduce(sum, add, shared);
+    if (threadIdx.x == 0) *loss = (float)(sum / count);
   }
-  if (threadIdx.x == 0) *back = (float)((double)top / (mean ? fmax(count, 1.0) : 1.0) / unit);
-}
-
-// E -> G in place; a workgroup per token
-template <class T>
-__global__ void __launch_bounds__(256) scale_kernel(const Pieces pieces, T* e, const float2* stats, int64_t ld_stats, int64_t token0, Labels labels,
-                                                    const float* lse, const float* factor) {
-  const int n = blockIdx.x;
-  const int64_t ld = (int64_t)pieces.tiles * kTile, at = token0 + n;
-  const float log_sum = lse[at], g = factor[at];
-  const int label = labels.get(at);
-  int64_t want = -1;
-  if (label >= 0) {
-    int r = 0;
-    while (r + 1 < pieces.ranks && label >= pieces.first[r + 1]) ++r;
-    want = (int64_t)pieces.tile0[r] * kTile + label - pieces.first[r];
+  if (!upstream) return;
+  if (factor) {
+    top = (float)block_reduce((double)top, [](double a, double b) { return fmax(a, b); }, shared);
+    for (int64_t n = threadIdx.x; n < tokens; n += 1024) {
+      const int label = labels.get(n);
+      const float g = upstream[n];
+      factor[n] = label == -1 ? 0.f : label < 0 ? NAN : g == 0.f ? 0.f : g / top;
+    }
+  } else {
+    top = fabsf(*upstream);
   }
-  typedef typename Half<T>::x8 x8;
-  for (int64_t v = threadIdx.x * 8; v < ld; v += 256 * 8) {
-    const float m = stats[(v >> 7) * ld_stats + n].x;
-    const float f = m == -INFINITY ? 0.f : exp_of(m - log_sum) * g;
-    x8 o = *(x8*)(e + n * ld + v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (T)(g == 0.f ? 0.f : (float)o[i] * f - (v + i == want ? kUnit<T> * g : 0.f));
-    *(x8*)(e + n * ld + v) = o;
-  }
+  if (threadIdx.x == 0) *back = (float)((double)top / count / unit);
 }
 
 // The rows of all ranks' pieces as k of a product, in steps of kStepK; what pads a rank's last tile counts as outside.
 struct PieceSource {
   const Pieces* p;
   int64_t stride;
-  int col_bytes, r = 0, row = 0;
+  int col_bytes, row, r = 0;
   __device__ __forceinline__ const char* step(int, int* k_left) {
-    while (r + 1 < p->ranks && row >= (p->tile0[r + 1] - p->tile0[r]) * kTile) ++r, row = 0;
+    while (r + 1 < p->ranks && row >= (p->tile0[r + 1] - p->tile0[r]) * kTile) row -= (p->tile0[r + 1] - p->tile0[r]) * kTile, ++r;
     *k_left = min(kStepK, p->rows[r] - row);
     const char* at = *k_left > 0 ? p->w[r] + row * stride + col_bytes : p->w[r];
     row += kStepK;
@@ -292,6 +310,8 @@ struct GradArgs {
   const char* x;
   int64_t x_stride, w_stride;
   int hidden, tokens, token_tiles, hidden_tiles;
+  int split_steps;   // dx: steps of kStepK for each part of the vocabulary
+  float* parts;      // dx: [parts][tokens][hidden]; null: one part
   char* dx;
   int64_t dx_stride, dw_stride;
   const float* back;
@@ -299,23 +319,34 @@ struct GradArgs {
   int first, last;
 };
 
-template <class T>
-__global__ void __launch_bounds__(512, 2) dx_kernel(const Pieces pieces, const GradArgs a) {
-  typedef TileProduct<T, kTile, kTile, 2, 4, true, false> Product;
+template <class T> __device__ __forceinline__ typename Half<T>::x4 narrow(f32x4 v, float by) {
+  typename Half<T>::x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = (T)(v[i] * by);
+  return o;
+}
+
+template <class T, class Shape>
+__global__ void __launch_bounds__(Shape::kThreads, 2) dx_kernel(const Pieces pieces, const GradArgs a) {
+  typedef typename Shape::template Product<T, true, false> Product;
+  constexpr int TL = Shape::kL, TR = Shape::kR;
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
   int tt, ht;
   tile_of(blockIdx.x, a.token_tiles, a.hidden_tiles, &tt, &ht);
-  const int n0 = tt * kTile, d0 = ht * kTile, tokens = min(kTile, a.tokens - n0), width = min(kTile, a.hidden - d0);
+  const int n0 = tt * TR, d0 = ht * TL, tokens = min(TR, a.tokens - n0), width = min(TL, a.hidden - d0);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
+  const int step0 = blockIdx.y * a.split_steps, steps = min(a.split_steps, pieces.tiles * (kTile / kStepK) - step0);
   f32x4 acc[Product::FL][Product::FR] = {};
   {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
     ll.place(threadIdx.x, a.w_stride, width);
     rl.place(threadIdx.x, ld * 2, tokens);
-    Product::run(smem, pieces.tiles * (kTile / kStepK), ll, PieceSource{&pieces, a.w_stride, d0 * 2}, rl, RowSource{(const char*)a.g + n0 * ld * 2, ld}, acc);
+    Product::run(smem, steps, ll, PieceSource{&pieces, a.w_stride, d0 * 2, step0 * kStepK}, rl,
+                 RowSource{(const char*)a.g + (n0 * ld + (int64_t)step0 * kStepK) * 2, ld}, acc);
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l0 = wave % 2 * 128 + (lane >> 4) * 4, r0 = wave / 2 * 64 + (lane & 15);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l0 = wave % Shape::kWavesL * (TL / Shape::kWavesL) + (lane >> 4) * 4, r0 = wave / Shape::kWavesL * (TR / Shape::kWavesR) + (lane & 15);
   const float back = *a.back;
 #pragma unroll
   for (int r = 0; r < Product::FR; ++r)
@@ -323,32 +354,44 @@ __global__ void __launch_bounds__(512, 2) dx_kernel(const Pieces pieces, const G
     for (int l = 0; l < Product::FL; ++l) {
       const int n = r0 + r * 16, d = l0 + l * 16;
       if (n >= tokens || d >= width) continue;
-      typename Half<T>::x4 o;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = (T)(acc[l][r][i] * back);
-      *(typename Half<T>::x4*)(a.dx + (n0 + n) * a.dx_stride + (d0 + d) * 2) = o;
+      if (a.parts) *(f32x4*)(a.parts + ((int64_t)blockIdx.y * a.tokens + n0 + n) * a.hidden + d0 + d) = acc[l][r];
+      else *(typename Half<T>::x4*)(a.dx + (n0 + n) * a.dx_stride + (d0 + d) * 2) = narrow<T>(acc[l][r], back);
     }
 }
 
+// dx from the parts of the vocabulary: four values per thread
 template <class T>
-__global__ void __launch_bounds__(512, 2) dw_kernel(const Pieces pieces, const Grads grads, const GradArgs a) {
-  typedef TileProduct<T, kTile, kTile, 2, 4, true, true> Product;
+__global__ void __launch_bounds__(256) add_parts_kernel(const float* parts, int count, int tokens, int hidden, char* dx, int64_t dx_stride, const float* back) {
+  const int64_t size = (int64_t)tokens * hidden, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= size) return;
+  f32x4 sum = {};
+#pragma unroll 8
+  for (int p = 0; p < count; ++p) sum += *(const f32x4*)(parts + p * size + i);
+  *(typename Half<T>::x4*)(dx + i / hidden * dx_stride + i % hidden * 2) = narrow<T>(sum, *back);
+}
+
+template <class T, class Shape>
+__global__ void __launch_bounds__(Shape::kThreads, 2) dw_kernel(const Pieces pieces, const Grads grads, const GradArgs a) {
+  typedef typename Shape::template Product<T, true, true> Product;
+  constexpr int TL = Shape::kL, TR = Shape::kR;
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
-  int vt, ht;
-  tile_of(blockIdx.x, pieces.tiles, a.hidden_tiles, &vt, &ht);
-  const int rank = pieces.rank_of(vt), row0 = (vt - pieces.tile0[rank]) * kTile, rows = min(kTile, pieces.rows[rank] - row0);
-  const int d0 = ht * kTile, width = min(kTile, a.hidden - d0);
+  int at, ht;
+  tile_of(blockIdx.x, pieces.tiles * (kTile / TR), a.hidden_tiles, &at, &ht);
+  const int rank = pieces.rank_of(at / (kTile / TR)), row0 = at * TR - pieces.tile0[rank] * kTile, rows = min(TR, pieces.rows[rank] - row0);
+  if (rows <= 0) return;  // padding
+  const int d0 = ht * TL, width = min(TL, a.hidden - d0);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
   f32x4 acc[Product::FL][Product::FR] = {};
   {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
     ll.place(threadIdx.x, a.x_stride, width);
-    rl.place(threadIdx.x, ld * 2, kTile);
+    rl.place(threadIdx.x, ld * 2, TR);
     Product::run(smem, (a.tokens + kStepK - 1) / kStepK, ll, ColSource{a.x + d0 * 2, a.tokens, a.x_stride}, rl,
-                 ColSource{(const char*)a.g + (int64_t)vt * kTile * 2, a.tokens, ld * 2}, acc);
+                 ColSource{(const char*)a.g + (int64_t)at * TR * 2, a.tokens, ld * 2}, acc);
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l0 = wave % 2 * 128 + (lane >> 4) * 4, r0 = wave / 2 * 64 + (lane & 15);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l0 = wave % Shape::kWavesL * (TL / Shape::kWavesL) + (lane >> 4) * 4, r0 = wave / Shape::kWavesL * (TR / Shape::kWavesR) + (lane & 15);
   const float back = *a.back;
 #pragma unroll
   for (int r = 0; r < Product::FR; ++r)
@@ -358,17 +401,14 @@ __global__ void __launch_bounds__(512, 2) dw_kernel(const Pieces pieces, const G
       if (v >= rows || d >= width) continue;
       f32x4 sum = acc[l][r];
       if (a.sums) {
-        f32x4* kept = (f32x4*)(a.sums + ((int64_t)vt * kTile + v) * a.hidden + d0 + d);
+        f32x4* kept = (f32x4*)(a.sums + ((int64_t)at * TR + v) * a.hidden + d0 + d);
         if (!a.first) sum += *kept;
         if (!a.last) {
           *kept = sum;
           continue;
         }
       }
-      typename Half<T>::x4 o;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = (T)(sum[i] * back);
-      *(typename Half<T>::x4*)(grads.dw[rank] + (row0 + v) * a.dw_stride + (d0 + d) * 2) = o;
+      *(typename Half<T>::x4*)(grads.dw[rank] + (row0 + v) * a.dw_stride + (d0 + d) * 2) = narrow<T>(sum, back);
     }
 }
 
@@ -387,7 +427,7 @@ struct mscclx_vocab_loss {
   Pieces pieces;          // without pointers
   int64_t vocab = 0;
   int64_t piece = 0;      // tokens per piece
-  uint64_t off_z = 0, off_loss = 0, off_factor = 0, off_back = 0, off_stats = 0, off_e = 0, off_sums = 0, bytes = 0;
+  uint64_t off_z = 0, off_loss = 0, off_factor = 0, off_back = 0, off_stats = 0, off_e = 0, off_sums = 0, off_parts = 0, bytes = 0;
 };
 
 namespace {
@@ -415,7 +455,7 @@ struct Call {
   Pieces pieces;
   Grads grads;
   Labels labels;
-  float *z_label, *row_loss, *factor, *back, *sums;
+  float *z_label, *row_loss, *factor, *back, *sums, *parts;
   float2* stats;
   void* e;
 };
@@ -459,85 +499,158 @@ int check_call(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool 
   c->back = (float*)(ws + h->off_back);
   c->stats = (float2*)(ws + h->off_stats);
   c->e = ws + h->off_e;
+  c->parts = (float*)(ws + h->off_parts);
   c->sums = h->off_sums ? (float*)(ws + h->off_sums) : nullptr;
   return MSCCLX_OK;
 }
 
-int tiles(int64_t n) { return (int)((n + kTile - 1) / kTile); }
+int tiles(int64_t n, int of = kTile) { return (int)((n + of - 1) / of); }
+
+enum { kLarge, kMiddle, kFew };
+int pick_shape(const char* name, int automatic) {
+#ifdef MSCCLX_SWEEP
+  if (const char* v = getenv(name)) return atoi(v);
+#endif
+  return automatic;
+}
+
+constexpr int kUnits = 256;  // compute units
+
+// Which shape a product of `rows` x `cols` takes.
+int shape_of(const char* name, int64_t rows, int64_t cols, int64_t tokens, bool few) {
+  const int automatic = few && tokens <= Few::kR ? kFew : (int64_t)tiles(rows, 256) * tiles(cols, 256) >= kUnits ? kLarge : kMiddle;
+  return pick_shape(name, automatic);
+}
+
+// Into how many parts dx cuts the vocabulary of `steps` steps, so that `count` tiles fill `slots` workgroups.
+int parts_of(int64_t count, int steps, int slots) {
+  const int parts = pick_shape("DX_PARTS", (int)std::min<int64_t>(steps / 4, slots / std::max<int64_t>(1, count)));
+  return std::max(1, std::min(parts, steps));
+}
+
+struct DxPlan {
+  int shape, token_tiles, hidden_tiles, parts, split_steps;
+};
+DxPlan dx_plan(const Pieces& p, int64_t tokens, int hidden) {
+  DxPlan d;
+  const int steps = p.tiles * (kTile / kStepK);
+  d.shape = pick_shape("DX_SHAPE", tokens <= Few::kR ? kFew : tokens <= Middle::kR ? kMiddle : kLarge);
+  const int l = d.shape == kLarge ? Large::kL : d.shape == kMiddle ? Middle::kL : Few::kL, r = d.shape == kLarge ? Large::kR : d.shape == kMiddle ? Middle::kR : Few::kR;
+  d.token_tiles = tiles(tokens, r);
+  d.hidden_tiles = tiles(hidden, l);
+  const int parts = parts_of((int64_t)d.token_tiles * d.hidden_tiles, steps, d.shape == kLarge ? kUnits : 2 * kUnits);
+  d.split_steps = (steps + parts - 1) / parts;
+  d.parts = (steps + d.split_steps - 1) / d.split_steps;
+  return d;
+}
+
+template <class T, int MODE>
+int launch_logits(int shape, const Pieces& p, LogitsArgs& a, hipStream_t stream) {
+  auto go = [&](auto s) {
+    typedef decltype(s) S;
+    a.token_tiles = tiles(a.tokens, S::kR);
+    hipLaunchKernelGGL((logits_kernel<T, MODE, S>), dim3((unsigned)(a.token_tiles * p.tiles * (kTile / S::kL))), dim3(S::kThreads), 0, stream, p, a);
+    return launched("logits_kernel");
+  };
+  return shape == kLarge ? go(Large()) : shape == kMiddle ? go(Middle()) : go(Few());
+}
 
 template <class T>
 int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool forward, bool backward, const Call& c, hipStream_t stream) {
   const mscclx_vocab_loss_desc& d = h->desc;
+  const Pieces& p = c.pieces;
   const int64_t n = io->tokens;
   const int mean = d.reduction == MSCCLX_LOSS_MEAN, per_token = d.reduction == MSCCLX_LOSS_NONE;
+  const Upstream upstream = {io->grad_loss, per_token ? c.factor : nullptr};
   int rc;
-  if (backward) {
-    hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(1024), 0, stream, io->grad_loss, per_token, n, c.labels, mean, kUnit<T>, c.factor, c.back);
-    if ((rc = launched("factor_kernel"))) return rc;
-  }
-  const int hidden_tiles = tiles(d.hidden);
+  // one number: with the losses, behind the last piece's tokens and in front of its gradients; else first of all
+  auto sums = [&](bool losses) {
+    hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, stream, n, c.labels, mean, losses ? c.row_loss : nullptr, io->loss, backward ? io->grad_loss : nullptr,
+                       per_token ? c.factor : nullptr, kUnit<T>, c.back);
+    return launched("sums_kernel");
+  };
+  const bool early = backward && (per_token || !forward || n > h->piece);
+  if (early && (rc = sums(false))) return rc;
   const int64_t all = std::max<int64_t>(n, backward ? 1 : 0);  // no tokens: dw is still written, with zeros
   for (int64_t at = 0; at < all; at += h->piece) {
     const int now = (int)std::min(h->piece, n - at);
+    const bool last = at + now >= n;
     LogitsArgs a = {};
     a.x = (const char*)io->x + at * io->x_stride * 2;
     a.x_stride = io->x_stride * 2;
     a.w_stride = io->weight_stride * 2;
     a.hidden = d.hidden;
     a.tokens = now;
-    a.token_tiles = tiles(now);
     a.token0 = at;
     a.labels = c.labels;
+    a.upstream = upstream;
     a.stats = c.stats;
-    a.ld_stats = h->piece;
     a.z_label = c.z_label;
     a.e = c.e;
     a.lse = io->lse;
-    a.factor = c.factor;
-    const dim3 grid((unsigned)(a.token_tiles * c.pieces.tiles));
     if (now > 0) {
-      if (!forward) hipLaunchKernelGGL((logits_kernel<T, kGradient>), grid, dim3(512), 0, stream, c.pieces, a);
-      else if (backward) hipLaunchKernelGGL((logits_kernel<T, kKeep>), grid, dim3(512), 0, stream, c.pieces, a);
-      else hipLaunchKernelGGL((logits_kernel<T, kStats>), grid, dim3(512), 0, stream, c.pieces, a);
-      if ((rc = launched("logits_kernel"))) return rc;
+      const int shape = shape_of("LOGITS_SHAPE", now, (int64_t)p.tiles * kTile, now, true);
+      if ((rc = !forward ? launch_logits<T, kGradient>(shape, p, a, stream) : backward ? launch_logits<T, kKeep>(shape, p, a, stream) : launch_logits<T, kStats>(shape, p, a, stream)))
+        return rc;
       if (forward) {
-        hipLaunchKernelGGL(join_kernel, dim3((now + 31) / 32), dim3(256), 0, stream, c.stats, a.ld_stats, 2 * c.pieces.tiles, now, at, c.labels, c.z_label, io->lse, c.row_loss);
-        if ((rc = launched("join_kernel"))) return rc;
-      }
-      if (forward && backward) {
-        hipLaunchKernelGGL((scale_kernel<T>), dim3(now), dim3(256), 0, stream, c.pieces, (T*)c.e, c.stats, a.ld_stats, at, c.labels, io->lse, c.factor);
-        if ((rc = launched("scale_kernel"))) return rc;
+        TokenArgs t = {};
+        t.stats = c.stats;
+        t.part = shape == kLarge ? Large::kL / Large::kWavesL : shape == kMiddle ? Middle::kL / Middle::kWavesL : Few::kL / Few::kWavesL;
+        t.token0 = at;
+        t.labels = c.labels;
+        t.upstream = upstream;
+        t.z_label = c.z_label;
+        t.lse = io->lse;
+        t.loss = c.row_loss;
+        t.e = c.e;
+        if (backward) hipLaunchKernelGGL((token_kernel<T, true>), dim3(now), dim3(256), 0, stream, p, t);
+        else hipLaunchKernelGGL((token_kernel<T, false>), dim3(now), dim3(256), 0, stream, p, t);
+        if ((rc = launched("token_kernel"))) return rc;
       }
     }
-    if (backward) {
-      GradArgs g = {};
-      g.g = c.e;
-      g.x = a.x;
-      g.x_stride = a.x_stride;
-      g.w_stride = a.w_stride;
-      g.hidden = d.hidden;
-      g.tokens = now;
-      g.token_tiles = a.token_tiles;
-      g.hidden_tiles = hidden_tiles;
-      g.dx = (char*)io->dx + at * io->dx_stride * 2;
-      g.dx_stride = io->dx_stride * 2;
-      g.dw_stride = io->dweight_stride * 2;
-      g.back = c.back;
-      g.sums = n > h->piece ? c.sums : nullptr;
-      g.first = at == 0;
-      g.last = at + now >= n;
-      if (now > 0) {
-        hipLaunchKernelGGL((dx_kernel<T>), dim3((unsigned)(g.token_tiles * hidden_tiles)), dim3(512), 0, stream, c.pieces, g);
-        if ((rc = launched("dx_kernel"))) return rc;
+    if (last && forward && !per_token && (rc = sums(true))) return rc;
+    if (!backward) continue;
+    GradArgs g = {};
+    g.g = c.e;
+    g.x = a.x;
+    g.x_stride = a.x_stride;
+    g.w_stride = a.w_stride;
+    g.hidden = d.hidden;
+    g.tokens = now;
+    g.dx = (char*)io->dx + at * io->dx_stride * 2;
+    g.dx_stride = io->dx_stride * 2;
+    g.dw_stride = io->dweight_stride * 2;
+    g.back = c.back;
+    g.sums = n > h->piece ? c.sums : nullptr;
+    g.first = at == 0;
+    g.last = last;
+    if (now > 0) {
+      const DxPlan plan = dx_plan(p, now, d.hidden);
+      g.token_tiles = plan.token_tiles;
+      g.hidden_tiles = plan.hidden_tiles;
+      g.split_steps = plan.split_steps;
+      g.parts = plan.parts > 1 ? c.parts : nullptr;
+      auto go = [&](auto s) {
+        typedef decltype(s) S;
+        hipLaunchKernelGGL((dx_kernel<T, S>), dim3((unsigned)(g.token_tiles * g.hidden_tiles), plan.parts), dim3(S::kThreads), 0, stream, p, g);
+        return launched("dx_kernel");
+      };
+      if ((rc = plan.shape == kLarge ? go(Large()) : plan.shape == kMiddle ? go(Middle()) : go(Few()))) return rc;
+      if (g.parts) {
+        hipLaunchKernelGGL((add_parts_kernel<T>), dim3((unsigned)(((int64_t)now * d.hidden + 1023) / 1024)), dim3(256), 0, stream, c.parts, plan.parts, now, d.hidden, g.dx,
+                           g.dx_stride, c.back);
+        if ((rc = launched("add_parts_kernel"))) return rc;
       }
-      hipLaunchKernelGGL((dw_kernel<T>), dim3((unsigned)(c.pieces.tiles * hidden_tiles)), dim3(512), 0, stream, c.pieces, c.grads, g);
-      if ((rc = launched("dw_kernel"))) return rc;
     }
+    auto go = [&](auto s) {
+      typedef decltype(s) S;
+      g.hidden_tiles = tiles(d.hidden, S::kL);
+      hipLaunchKernelGGL((dw_kernel<T, S>), dim3((unsigned)(p.tiles * (kTile / S::kR) * g.hidden_tiles)), dim3(S::kThreads), 0, stream, p, c.grads, g);
+      return launched("dw_kernel");
+    };
+    if ((rc = shape_of("DW_SHAPE", (int64_t)p.tiles * kTile, d.hidden, now, false) == kLarge ? go(Large()) : go(Middle()))) return rc;
   }
-  if (forward && d.reduction != MSCCLX_LOSS_NONE) {
-    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, stream, c.row_loss, n, c.labels, mean, io->loss);
-    if ((rc = launched("total_kernel"))) return rc;
-  }
+  if (n == 0 && forward && !per_token && !backward) return sums(true);
   return MSCCLX_OK;
 }
 
@@ -602,9 +715,16 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
     h->off_z = take(n * 4);
     h->off_loss = take(n * 4);
     h->off_factor = take(n * 4);
-    h->off_stats = take((uint64_t)h->piece * p.tiles * 2 * sizeof(float2));
+    const uint64_t wide = (uint64_t)p.tiles * kTile;
+    h->off_stats = take(std::max(std::min<uint64_t>(h->piece, Few::kR) * (wide / (Few::kL / Few::kWavesL)), (uint64_t)h->piece * (wide / (Middle::kL / Middle::kWavesL))) * sizeof(float2));
     h->off_e = d.gradients ? take((uint64_t)h->piece * row) : 0;
     h->off_sums = d.gradients && d.max_tokens > h->piece ? take((uint64_t)p.tiles * kTile * d.hidden * 4) : 0;
+    uint64_t parts = 0;  // dx's parts at the token count that needs most of them; its plan is the same for (32 k, 32 k + 32] tokens
+    for (int64_t t = 0; d.gradients && t < h->piece; t += Few::kR) {
+      const DxPlan plan = dx_plan(p, t + 1, d.hidden);
+      if (plan.parts > 1) parts = std::max(parts, (uint64_t)plan.parts * std::min<int64_t>(h->piece, t + Few::kR) * d.hidden * 4);
+    }
+    h->off_parts = take(parts);
     h->bytes = at;
     if (workspace_bytes) *workspace_bytes = at;
     if (piece_tokens) *piece_tokens = h->piece;
