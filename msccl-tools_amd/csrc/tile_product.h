@@ -1,7 +1,7 @@
 // A tile of a 16-bit matrix product on the matrix cores: out[r][l] = sum over k of L[l][k] R[r][k], sums in 32 bits.
 //
-// L runs along the output's rows (its contiguous dimension), R across them, so that the four registers of a
-// 16 x 16 x 32 instruction's result are four neighbours of one output row.  Either operand may be stored with k
+// L runs along the output's rows (its contiguous dimension), R across them, so that four registers of a
+// matrix instruction's result are four neighbours of one output row.  Either operand may be stored with k
 // contiguous ("row": one row of memory per l or r) or with k strided ("col": one row of memory per k).
 //
 // Data path: a workgroup copies the next 64 values of k of both operands from memory into LDS without passing through
@@ -9,8 +9,8 @@
 // the bank swizzle is applied to the addresses they read from:
 //   row operand: 128 bytes per row, the 16-byte unit u of row i sits at u ^ (i / 2 % 8): the sixteen rows that a
 //                fragment read touches at one unit then cover all 64 banks;
-//   col operand: one line of 2 * TILE bytes per k, 32-byte pair p of line k sits at p ^ (k % 4 + 4 * (k / 8 % 2)):
-//                the transposing read takes 8 lines x 32 bytes per half wave, again all banks once.
+//   col operand: one line of 2 * TILE bytes per k, 32-byte pair p of line k sits at p ^ swizzle_of(k): the transposing
+//                read takes 8 lines x 1 pair (16 x 16 instructions) or 4 lines x 2 pairs (32 x 32) per half wave, again all banks once.
 // What lies outside an operand (rows behind the last, k behind the last) is asked for at an offset beyond the
 // buffer resource's range: the hardware writes zeros for it and touches no memory.
 #ifndef MSCCLX_TILE_PRODUCT_H
@@ -19,10 +19,12 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace mscclx {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
@@ -42,12 +44,18 @@ template <> struct Half<__bf16> {
   static __device__ __forceinline__ f32x4 mfma(i16x8 a, i16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f32x16 mfma(i16x8 a, i16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
 };
 template <> struct Half<_Float16> {
   typedef f16x4 x4;
   typedef f16x8 x8;
   static __device__ __forceinline__ f32x4 mfma(i16x8 a, i16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mfma(i16x8 a, i16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
 
@@ -60,8 +68,10 @@ __device__ __forceinline__ i32x4 resource_at(const char* p) {
   return i32x4{(int)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), (int)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)), kResourceBytes, 0x00020000};
 }
 
+template <int SIDE> __device__ __forceinline__ int swizzle_of(int k) { return SIDE == 16 ? (k & 3) | ((k >> 3 & 1) << 2) : (k & 3) << 1; }
+
 // The lanes' places in one operand's tile.  COL: k strided.  WAVES: waves of the workgroup.  CHUNKS copies make a step.
-template <bool COL, int TILE, int WAVES>
+template <bool COL, int TILE, int WAVES, int SIDE>
 struct Lanes {
   static constexpr int kBytes = TILE * kStepK * 2;
   static constexpr int kChunk = WAVES * 1024;
@@ -78,7 +88,7 @@ struct Lanes {
     for (int i = 0; i < kChunks; ++i) {
       const int line = i * kLines + thread / kUnitsPerLine, unit = thread % kUnitsPerLine;
       if constexpr (COL) {
-        const int from = (((unit >> 1) ^ ((line & 3) | ((line >> 3 & 1) << 2))) << 1) | (unit & 1);
+        const int from = (((unit >> 1) ^ swizzle_of<SIDE>(line)) << 1) | (unit & 1);
         offset[i] = from * 8 < valid ? (unsigned)(line * stride) + from * 16 : kOutside;
         k[i] = line;
       } else {
@@ -88,15 +98,9 @@ struct Lanes {
       }
     }
   }
-  __device__ __forceinline__ void copy(unsigned lds, const char* from, int k_left) const {
-    const i32x4 r = resource_at(from);
-    if (k_left >= kStepK) {
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i) copy_to_lds(lds + i * kChunk, offset[i], r);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i) copy_to_lds(lds + i * kChunk, k[COL ? i : 0] < k_left ? offset[i] : kOutside, r);
-    }
+  // copy `i` of a step that has `k_left` values of k
+  __device__ __forceinline__ void copy(int i, unsigned lds, i32x4 from, int k_left) const {
+    copy_to_lds(lds + i * kChunk, k[COL ? i : 0] < k_left ? offset[i] : kOutside, from);
   }
 };
 
@@ -118,96 +122,122 @@ struct ColSource {  // k strided
   }
 };
 
-// TL x TR: the workgroup's tile, cut among WL x WR waves; STAGES: steps held in LDS, a power of two.
-template <class T, int TL, int TR, int WL, int WR, int STAGES, bool LCOL, bool RCOL>
+// TL x TR: the workgroup's tile, cut among WL x WR waves; SIDE: of the matrix instruction, 16 or 32; STAGES: steps held in LDS, a power of two.
+template <class T, int TL, int TR, int WL, int WR, int SIDE, int STAGES, bool LCOL, bool RCOL>
 struct TileProduct {
   static constexpr int kWaves = WL * WR, kThreads = kWaves * 64;
-  static constexpr int FL = TL / WL / 16, FR = TR / WR / 16;  // fragments of a wave
-  typedef Lanes<LCOL, TL, kWaves> LLanes;
-  typedef Lanes<RCOL, TR, kWaves> RLanes;
+  static constexpr int FL = TL / WL / SIDE, FR = TR / WR / SIDE;  // fragments of a wave
+  static constexpr int kSlices = SIDE / 16;                        // instructions for 32 values of k
+  static constexpr int kQuads = SIDE == 16 ? 1 : 4;                // groups of four neighbours that a lane holds of a fragment's result
+  typedef std::conditional_t<SIDE == 16, f32x4, f32x16> Acc;
+  typedef Lanes<LCOL, TL, kWaves, SIDE> LLanes;
+  typedef Lanes<RCOL, TR, kWaves, SIDE> RLanes;
   static constexpr int kStage = LLanes::kBytes + RLanes::kBytes;
   static constexpr int kLdsBytes = STAGES * kStage;
   static constexpr int kCopies = LLanes::kChunks + RLanes::kChunks;  // of a wave, per step
 
-  template <bool COL, int TILE, int F>
-  static __device__ __forceinline__ void fragments(const char* lds, int first, int kk, int lane, i16x8 (&out)[F]) {
+  // where in the tile the lane's quads lie: l of fragment f's quad q (its first), r of fragment f
+  static __device__ __forceinline__ int l_of(int thread, int f, int q) {
+    const int lane = thread & 63;
+    return (thread >> 6) % WL * (TL / WL) + f * SIDE + (SIDE == 16 ? lane >> 4 : 2 * q + (lane >> 5)) * 4;
+  }
+  static __device__ __forceinline__ int r_of(int thread, int f) { return (thread >> 6) / WL * (TR / WR) + f * SIDE + (thread & (SIDE - 1)); }
+  static __device__ __forceinline__ f32x4 quad(const Acc& a, int q) {
+    if constexpr (SIDE == 16) return a;
+    else return f32x4{a[q * 4], a[q * 4 + 1], a[q * 4 + 2], a[q * 4 + 3]};
+  }
+
+  // fragment f of slice s in a step's half
+  template <bool COL, int TILE>
+  static __device__ __forceinline__ i16x8 fragment(const char* lds, int first, int half, int lane, int s, int f) {
+    const int group = SIDE == 16 ? lane >> 4 : lane >> 5;  // of eight values of k
     if constexpr (COL) {
-      const int k = kk * 32 + (lane >> 4) * 8 + (lane >> 2 & 3), swizzle = (lane >> 2 & 3) | ((lane >> 4 & 1) << 2);
-#pragma unroll
-      for (int f = 0; f < F; ++f) {
-        const char* p = lds + k * (TILE * 2) + ((((first >> 4) + f) ^ swizzle) << 5) + (lane & 3) * 8;
-        typedef __attribute__((address_space(3))) i16x4* lds_ptr;
-        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * TILE * 2));
-        out[f] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      }
+      typedef __attribute__((address_space(3))) i16x4* lds_ptr;
+      const int within = group * 8 + (lane >> 2 & 3), pair = (first >> 4) + (SIDE == 32 ? lane >> 4 & 1 : 0) + f * (SIDE / 16);
+      const int k = half * 32 + s * 16 + within;  // (a slice or a half further the swizzle is the same)
+      const char* p = lds + k * (TILE * 2) + ((pair ^ swizzle_of<SIDE>(within)) << 5) + (lane & 3) * 8;
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * TILE * 2));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      const int unit = (kk * 4 + (lane >> 4)) ^ (lane >> 1 & 7);
-#pragma unroll
-      for (int f = 0; f < F; ++f) out[f] = *(const i16x8*)(lds + (first + f * 16 + (lane & 15)) * 128 + unit * 16);
+      const int unit = (half * 4 + s * 2 + group) ^ (lane >> 1 & 7);
+      return *(const i16x8*)(lds + (first + f * SIDE + (lane & (SIDE - 1))) * 128 + unit * 16);
     }
   }
 
   // acc[l][r] += the product over all steps.  Every wave of the workgroup calls this with the same sources.
   template <class SL, class SR>
-  static __device__ __forceinline__ void run(char* smem, int steps, const LLanes& ll, SL sl, const RLanes& rl, SR sr, f32x4 (&acc)[FL][FR]) {
+  static __device__ __forceinline__ void run(char* smem, int steps, const LLanes& ll, SL sl, const RLanes& rl, SR sr, Acc (&acc)[FL][FR]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l0 = wave % WL * (TL / WL), r0 = wave / WL * (TR / WR);
     typedef __attribute__((address_space(3))) char* lds_char;
     const unsigned lds = (unsigned)(uintptr_t)(lds_char)smem + wave * 1024;
-    auto issue = [&](int s) {
-      int k_left;
-      const unsigned at = lds + s % STAGES * kStage;
-      const char* p = sl.step(s, &k_left);
-      ll.copy(at, p, k_left);
-      p = sr.step(s, &k_left);
-      rl.copy(at + LLanes::kBytes, p, k_left);
+    struct Step {  // what the copies of a step read
+      unsigned lds;
+      i32x4 l, r;
+      int l_left, r_left;
     };
-    auto read = [&](int s, int kk, i16x8 (&a)[FL], i16x8 (&b)[FR]) {
+    auto step = [&](int s) {  // in order; behind the last step nothing is left and the copies write zeros
+      Step t;
+      t.lds = lds + s % STAGES * kStage;
+      t.l = resource_at(sl.step(s, &t.l_left));
+      t.r = resource_at(sr.step(s, &t.r_left));
+      return t;
+    };
+    auto copy = [&](const Step& t, int i) {
+      if (i < LLanes::kChunks) ll.copy(i, t.lds, t.l, t.l_left);
+      else rl.copy(i - LLanes::kChunks, t.lds + LLanes::kBytes, t.r, t.r_left);
+    };
+    struct Fragments {  // of half a step
+      i16x8 a[kSlices][FL], b[kSlices][FR];
+    };
+    constexpr int kUnits = (FL + FR) * kSlices;
+    auto read = [&](Fragments& f, int s, int half, int u) {  // unit u: all of r, then of l, as the products want them
       const char* at = smem + s % STAGES * kStage;
-      fragments<RCOL, TR, FR>(at + LLanes::kBytes, r0, kk, lane, b);
-      fragments<LCOL, TL, FL>(at, l0, kk, lane, a);
+      if (u < FR * kSlices) f.b[u % kSlices][u / kSlices] = fragment<RCOL, TR>(at + LLanes::kBytes, r0, half, lane, u % kSlices, u / kSlices);
+      else u -= FR * kSlices, f.a[u % kSlices][u / kSlices] = fragment<LCOL, TL>(at, l0, half, lane, u % kSlices, u / kSlices);
     };
-    auto multiply = [&](const i16x8 (&a)[FL], const i16x8 (&b)[FR]) {
+    // One fragment row of products after another; between them the next half's reads and, in the second half, the copies, so
+    // that neither LDS nor the path to it gets all of a step's requests at once.
+    auto multiply = [&](const Fragments& f, int l) {
 #pragma unroll
-      for (int l = 0; l < FL; ++l)
+      for (int s = 0; s < kSlices; ++s)
 #pragma unroll
-        for (int r = 0; r < FR; ++r) acc[l][r] = Half<T>::mfma(a[l], b[r], acc[l][r]);
+        for (int r = 0; r < FR; ++r) acc[l][r] = Half<T>::mfma(f.a[s][l], f.b[s][r], acc[l][r]);
     };
-    // a read from LDS, then a few products, and so on: neither waits for the other
-    auto interleave = [&] {
-      constexpr int kReads = FL * (LCOL ? 2 : 1) + FR * (RCOL ? 2 : 1), kEach = FL * FR / kReads > 0 ? FL * FR / kReads : 1;
+    Fragments now, next;
 #pragma unroll
-      for (int i = 0; i < kReads; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
-      }
-      if constexpr (FL * FR > kReads * kEach) __builtin_amdgcn_sched_group_barrier(0x008, FL * FR - kReads * kEach, 0);
-    };
-    if (steps <= 0) return;
-    i16x8 a0[FL], b0[FR], a1[FL], b1[FR];  // fragments of the step's first and second 32 values of k
-    // Copies arrive in order: with the next STAGES - 2 steps' copies behind them, the awaited step's are there once no more are under way.
-    // Where the last steps are not followed by others, everything is waited for.
-    constexpr int kBehind = (STAGES - 2) * kCopies;
+    for (int s = 0; s < STAGES; ++s) {
+      const Step t = step(s);
 #pragma unroll
-    for (int s = 0; s < STAGES; ++s)
-      if (s < steps) issue(s);
-    if (steps >= STAGES) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kBehind + kCopies) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    read(0, 0, a0, b0);
-    for (int s = 0; s < steps; ++s) {
-      read(s, 1, a1, b1);
-      multiply(a0, b0);
-      interleave();
-      // the copies of the next step have arrived, and every wave has read all of this one: its buffer takes the step STAGES further
-      if (STAGES > 2 && s + STAGES <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kBehind) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-      if (s + STAGES < steps) issue(s + STAGES);
-      read(s + 1, 0, a0, b0);  // (behind the last step: what that buffer holds, for nothing)
-      multiply(a1, b1);
-      interleave();
+      for (int i = 0; i < kCopies; ++i) copy(t, i);
     }
+    // copies arrive in order: the awaited step's are there once only those of the steps behind it are under way
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * kCopies) : "memory");
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) read(now, 0, 0, u);
+    for (int s = 0; s < steps; ++s) {
+#pragma unroll
+      for (int l = 0; l < FL; ++l) {
+#pragma unroll
+        for (int u = l * kUnits / FL; u < (l + 1) * kUnits / FL; ++u) read(next, s, 1, u);
+        multiply(now, l);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // the copies of the next step have arrived, and every wave has read all of this one: its buffer takes the step STAGES further
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * kCopies) : "memory");
+      const Step t = step(s + STAGES);
+#pragma unroll
+      for (int l = 0; l < FL; ++l) {
+#pragma unroll
+        for (int i = l * kCopies / FL; i < (l + 1) * kCopies / FL; ++i) copy(t, i);
+#pragma unroll
+        for (int u = l * kUnits / FL; u < (l + 1) * kUnits / FL; ++u) read(now, s + 1, 0, u);  // (behind the last step: for nothing)
+        multiply(next, l);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup
   }
 };
 

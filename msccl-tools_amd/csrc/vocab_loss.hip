@@ -6,7 +6,7 @@
 //
 // Tokens go through in pieces of at most `piece` rows; per piece, three products on the matrix cores (tile_product.h):
 //   logits   z of a tile of vocabulary x tokens stays in registers; what leaves are, for each token and each wave's part of the
-//            vocabulary, the maximum m and the sum of exp(z - m), and with gradients E = exp(z - m) in 16 bits;
+//            vocabulary, the maximum m (in units of log 2) and the sum of exp(z - m), and with gradients E = exp(z - m) in 16 bits;
 //   tokens   a token's (m, sum) become its lse and loss, and its E becomes G in place: G = (E exp(m - lse) - [label]) g / max|g|;
 //   dx, dw   the two products, on G.  dx sums over the whole vocabulary: where its tiles do not fill the chip, that
 //            axis is cut and the parts are added by a kernel of their own.
@@ -17,7 +17,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <cstring>
 #include <new>
 #include <string>
@@ -32,7 +31,7 @@ namespace {
 
 constexpr int kMaxRanks = MSCCLX_VOCAB_LOSS_MAX_RANKS;
 constexpr int kTile = 256;              // rows of the vocabulary: a rank's piece is padded to whole tiles of G
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // The ranks' pieces of the vocabulary, passed to the kernels by value.  Tiles of kTile rows; none spans two ranks.
 struct Pieces {
@@ -74,18 +73,19 @@ struct Upstream {
   }
 };
 
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+// Exponents are kept in units of log 2: exp(z - m) = exp2(z log2(e) - M) with M = m log2(e), one multiply-add and one instruction.
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 template <class T> constexpr float kUnit = std::is_same_v<T, _Float16> ? 32768.0f : 1.0f;
 
 // How a workgroup's tile is cut.  Large: one workgroup of eight waves per compute unit.  Middle: two of four waves, for products whose large tiles
 // would not fill the chip.  Few: at most 32 tokens, with four steps of copies under way, because then memory is all that counts.
-template <int L, int R, int WL, int WR, int STAGES> struct Shape {
-  static constexpr int kL = L, kR = R, kWavesL = WL, kWavesR = WR, kThreads = WL * WR * 64;
-  template <class T, bool LCOL, bool RCOL> using Product = TileProduct<T, L, R, WL, WR, STAGES, LCOL, RCOL>;
+template <int L, int R, int WL, int WR, int SIDE, int STAGES> struct Shape {
+  static constexpr int kL = L, kR = R, kWavesL = WL, kWavesR = WR, kThreads = WL * WR * 64, kSide = SIDE;
+  template <class T, bool LCOL, bool RCOL> using Product = TileProduct<T, L, R, WL, WR, SIDE, STAGES, LCOL, RCOL>;
 };
-typedef Shape<256, 256, 2, 4, 2> Large;
-typedef Shape<128, 128, 2, 2, 2> Middle;
-typedef Shape<128, 32, 4, 1, 4> Few;
+typedef Shape<256, 256, 2, 4, 16, 2> Large;
+typedef Shape<128, 128, 2, 2, 16, 2> Middle;
+typedef Shape<128, 32, 4, 1, 16, 4> Few;
 
 enum { kStats = 0, kKeep = 1, kGradient = 2 };
 
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces
   const int vt = at / (kTile / TL), rank = pieces.rank_of(vt), row0 = at * TL - pieces.tile0[rank] * kTile;
   const int rows = min(TL, pieces.rows[rank] - row0);  // none or less: the tile is padding
   const int n0 = tt * TR, tokens = min(TR, a.tokens - n0);
-  f32x4 acc[Product::FL][Product::FR] = {};
+  typename Product::Acc acc[Product::FL][Product::FR] = {};
   if (rows > 0) {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
@@ -132,64 +132,78 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces
     Product::run(smem, (a.hidden + kStepK - 1) / kStepK, ll, RowSource{pieces.w[rank] + row0 * a.w_stride, a.hidden}, rl,
                  RowSource{a.x + n0 * a.x_stride, a.hidden}, acc);
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l0 = wave % Shape::kWavesL * kPart, r0 = wave / Shape::kWavesL * (TR / Shape::kWavesR);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
-  const int v0 = l0 + (lane >> 4) * 4;  // + 16 * l + i
+  const int lane = threadIdx.x & 63, part = (threadIdx.x >> 6) % Shape::kWavesL;
+  auto finish = [&](auto whole) {  // whole: no row of the tile is padding
+    constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-  for (int r = 0; r < Product::FR; ++r) {
-    const int n = r0 + r * 16 + (lane & 15);
-    const bool live = n < tokens;
-    const int label = live ? a.labels.get(a.token0 + n0 + n) : -1;
-    const int want = label >= 0 ? label - pieces.first[rank] - row0 : -1;
-    typename Half<T>::x4* out = (typename Half<T>::x4*)((T*)a.e + (n0 + n) * ld + (int64_t)at * TL + v0);
-    if constexpr (MODE == kGradient) {
-      const float lse = live ? a.lse[a.token0 + n0 + n] : 0.f, g = live ? a.upstream.get(a.token0 + n0 + n, label) * kUnit<T> : 0.f;
+    for (int r = 0; r < Product::FR; ++r) {
+      const int n = Product::r_of(threadIdx.x, r);
+      const bool live = n < tokens;
+      const int label = live ? a.labels.get(a.token0 + n0 + n) : -1;
+      const int want = label >= 0 ? label - pieces.first[rank] - row0 : -1;  // the label's row in the tile
+      const bool here = want >= part * kPart && want < min(rows, (part + 1) * kPart);
+      const bool any = __any(here);                                           // one wave in hundreds holds a label of its tokens
+      T* out = (T*)a.e + (n0 + n) * ld + (int64_t)at * TL;
+      // the wave's logits of the token, in fours
+      auto each = [&](auto f) {
 #pragma unroll
-      for (int l = 0; l < Product::FL; ++l) {
-        typename Half<T>::x4 o;
+        for (int l = 0; l < Product::FL; ++l)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int v = v0 + l * 16 + i;
-          const float p = exp_of(acc[l][r][i] - lse) - (v == want ? 1.f : 0.f);
-          o[i] = (T)(v < rows && g != 0.f ? p * g : 0.f);
+          for (int q = 0; q < Product::kQuads; ++q) f(Product::l_of(threadIdx.x, l, q), Product::quad(acc[l][r], q));
+      };
+      if constexpr (MODE == kGradient) {
+        const float lse = live ? a.lse[a.token0 + n0 + n] * kLog2e : 0.f, g = live ? a.upstream.get(a.token0 + n0 + n, label) * kUnit<T> : 0.f;
+        each([&](int v, f32x4 z) {
+          typename Half<T>::x4 o;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float p = exp2_of(__builtin_fmaf(z[i], kLog2e, -lse));
+            if (any) p -= v + i == want ? 1.f : 0.f;
+            o[i] = (T)((WHOLE || v + i < rows) && g != 0.f ? p * g : 0.f);
+          }
+          if (live) *(typename Half<T>::x4*)(out + v) = o;
+        });
+      } else {
+        float m = -INFINITY;
+        each([&](int v, f32x4 z) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (WHOLE || v + i < rows) m = fmaxf(m, z[i]);
+        });
+        if (any) {
+          float z_label = 0.f;
+          bool found = false;
+          each([&](int v, f32x4 z) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (v + i == want && v + i < rows) z_label = z[i], found = true;
+          });
+          if (found) a.z_label[a.token0 + n0 + n] = z_label;
         }
-        if (live) out[l * 4] = o;
-      }
-    } else {
-      float m = -INFINITY, z_label = 0.f;
-      bool found = false;
 #pragma unroll
-      for (int l = 0; l < Product::FL; ++l)
+        for (int d = Shape::kSide; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+        m *= kLog2e;
+        const float base = m == -INFINITY ? 0.f : m;  // a part of nothing but -inf has sum 0
+        float sum = 0.f;
+        each([&](int v, f32x4 z) {
+          typename Half<T>::x4 o;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int v = v0 + l * 16 + i;
-          if (v == want && v < rows) z_label = acc[l][r][i], found = true;
-          if (v >= rows) acc[l][r][i] = -INFINITY;
-          m = fmaxf(m, acc[l][r][i]);
-        }
-      m = fmaxf(m, __shfl_xor(m, 16));
-      m = fmaxf(m, __shfl_xor(m, 32));
-      const float base = m == -INFINITY ? 0.f : m;  // a part of nothing but -inf has sum 0
-      float sum = 0.f;
+          for (int i = 0; i < 4; ++i) {
+            const float e = WHOLE || v + i < rows ? exp2_of(__builtin_fmaf(z[i], kLog2e, -base)) : 0.f;
+            sum += e;
+            o[i] = (T)(e * kUnit<T>);
+          }
+          if (MODE == kKeep && live) *(typename Half<T>::x4*)(out + v) = o;
+        });
 #pragma unroll
-      for (int l = 0; l < Product::FL; ++l) {
-        typename Half<T>::x4 o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = exp_of(acc[l][r][i] - base);
-          sum += e;
-          o[i] = (T)(e * kUnit<T>);
-        }
-        if (MODE == kKeep && live) out[l * 4] = o;
-      }
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      if (live) {
-        if (lane < 16) a.stats[(n0 + n) * (ld / kPart) + (at * TL + l0) / kPart] = make_float2(m, sum);
-        if (found) a.z_label[a.token0 + n0 + n] = z_label;
+        for (int d = Shape::kSide; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+        if (live && lane < Shape::kSide) a.stats[(n0 + n) * (ld / kPart) + at * TL / kPart + part] = make_float2(m, sum);
       }
     }
-  }
+  };
+  if (rows >= TL) finish(std::true_type());
+  else finish(std::false_type());
 }
 
 template <class V, class F> __device__ __forceinline__ V block_reduce(V v, F f, V* shared) {
@@ -227,10 +241,10 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
   const float base = m == -INFINITY ? 0.f : m;
   for (int h = threadIdx.x; h < parts; h += 256) {
     const float2 s = stats[h];
-    sum += s.y * exp_of(s.x - base);
+    sum += s.y * exp2_of(s.x - base);
   }
   sum = block_reduce(sum, [](float a, float b) { return a + b; }, shared);
-  const float lse = base + logf(sum);
+  const float lse2 = base + log2f(sum), lse = lse2 * kLn2;
   const int label = a.labels.get(at);
   if (threadIdx.x == 0) {
     a.lse[at] = lse;
@@ -248,7 +262,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
     T* e = (T*)a.e + blockIdx.x * ld;
     for (int64_t v = threadIdx.x * 8; v < ld; v += 256 * 8) {
       const float top = stats[v / a.part].x;
-      const float f = top == -INFINITY ? 0.f : exp_of(top - lse) * g;
+      const float f = top == -INFINITY ? 0.f : exp2_of(top - lse2) * g;
       x8 o = *(x8*)(e + v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = (T)(g == 0.f ? 0.f : (float)o[i] * f - (v + i == want ? kUnit<T> * g : 0.f));
@@ -295,13 +309,32 @@ __global__ void __launch_bounds__(1024) sums_kernel(int64_t tokens, Labels label
 struct PieceSource {
   const Pieces* p;
   int64_t stride;
-  int col_bytes, row, r = 0;
+  int col_bytes;
+  int rank = -1, left = 0, padded = 0;  // of the rank: rows behind this step's first, padding included or not
+  const char* at = nullptr;
+  __device__ __forceinline__ PieceSource(const Pieces* pieces, int64_t stride, int col_bytes, int row) : p(pieces), stride(stride), col_bytes(col_bytes) {
+    padded = -row;
+    next();
+    const int skip = (p->tile0[rank + 1] - p->tile0[rank]) * kTile - padded;
+    at += skip * stride;
+    left -= skip;
+  }
+  __device__ __forceinline__ void next() {  // the rank that holds the row `-padded` rows behind this one's end
+    while (padded <= 0 && rank + 1 < p->ranks) {
+      ++rank;
+      padded += (p->tile0[rank + 1] - p->tile0[rank]) * kTile;
+    }
+    left = p->rows[rank];
+    at = p->w[rank] + col_bytes;
+  }
   __device__ __forceinline__ const char* step(int, int* k_left) {
-    while (r + 1 < p->ranks && row >= (p->tile0[r + 1] - p->tile0[r]) * kTile) row -= (p->tile0[r + 1] - p->tile0[r]) * kTile, ++r;
-    *k_left = min(kStepK, p->rows[r] - row);
-    const char* at = *k_left > 0 ? p->w[r] + row * stride + col_bytes : p->w[r];
-    row += kStepK;
-    return at;
+    if (padded <= 0) next();
+    const char* here = at;
+    *k_left = left;
+    at += kStepK * stride;
+    left -= kStepK;
+    padded -= kStepK;
+    return here;
   }
 };
 
@@ -336,27 +369,28 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dx_kernel(const Pieces pie
   const int n0 = tt * TR, d0 = ht * TL, tokens = min(TR, a.tokens - n0), width = min(TL, a.hidden - d0);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
   const int step0 = blockIdx.y * a.split_steps, steps = min(a.split_steps, pieces.tiles * (kTile / kStepK) - step0);
-  f32x4 acc[Product::FL][Product::FR] = {};
+  typename Product::Acc acc[Product::FL][Product::FR] = {};
   {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
     ll.place(threadIdx.x, a.w_stride, width);
     rl.place(threadIdx.x, ld * 2, tokens);
-    Product::run(smem, steps, ll, PieceSource{&pieces, a.w_stride, d0 * 2, step0 * kStepK}, rl,
+    Product::run(smem, steps, ll, PieceSource(&pieces, a.w_stride, d0 * 2, step0 * kStepK), rl,
                  RowSource{(const char*)a.g + (n0 * ld + (int64_t)step0 * kStepK) * 2, ld}, acc);
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int l0 = wave % Shape::kWavesL * (TL / Shape::kWavesL) + (lane >> 4) * 4, r0 = wave / Shape::kWavesL * (TR / Shape::kWavesR) + (lane & 15);
   const float back = *a.back;
 #pragma unroll
   for (int r = 0; r < Product::FR; ++r)
 #pragma unroll
-    for (int l = 0; l < Product::FL; ++l) {
-      const int n = r0 + r * 16, d = l0 + l * 16;
-      if (n >= tokens || d >= width) continue;
-      if (a.parts) *(f32x4*)(a.parts + ((int64_t)blockIdx.y * a.tokens + n0 + n) * a.hidden + d0 + d) = acc[l][r];
-      else *(typename Half<T>::x4*)(a.dx + (n0 + n) * a.dx_stride + (d0 + d) * 2) = narrow<T>(acc[l][r], back);
-    }
+    for (int l = 0; l < Product::FL; ++l)
+#pragma unroll
+      for (int q = 0; q < Product::kQuads; ++q) {
+        const int n = Product::r_of(threadIdx.x, r), d = Product::l_of(threadIdx.x, l, q);
+        if (n >= tokens || d >= width) continue;
+        const f32x4 sum = Product::quad(acc[l][r], q);
+        if (a.parts) *(f32x4*)(a.parts + ((int64_t)blockIdx.y * a.tokens + n0 + n) * a.hidden + d0 + d) = sum;
+        else *(typename Half<T>::x4*)(a.dx + (n0 + n) * a.dx_stride + (d0 + d) * 2) = narrow<T>(sum, back);
+      }
 }
 
 // dx from the parts of the vocabulary: four values per thread
@@ -381,7 +415,7 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dw_kernel(const Pieces pie
   if (rows <= 0) return;  // padding
   const int d0 = ht * TL, width = min(TL, a.hidden - d0);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
-  f32x4 acc[Product::FL][Product::FR] = {};
+  typename Product::Acc acc[Product::FL][Product::FR] = {};
   {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
@@ -390,26 +424,26 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dw_kernel(const Pieces pie
     Product::run(smem, (a.tokens + kStepK - 1) / kStepK, ll, ColSource{a.x + d0 * 2, a.tokens, a.x_stride}, rl,
                  ColSource{(const char*)a.g + (int64_t)at * TR * 2, a.tokens, ld * 2}, acc);
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int l0 = wave % Shape::kWavesL * (TL / Shape::kWavesL) + (lane >> 4) * 4, r0 = wave / Shape::kWavesL * (TR / Shape::kWavesR) + (lane & 15);
   const float back = *a.back;
 #pragma unroll
   for (int r = 0; r < Product::FR; ++r)
 #pragma unroll
-    for (int l = 0; l < Product::FL; ++l) {
-      const int v = r0 + r * 16, d = l0 + l * 16;
-      if (v >= rows || d >= width) continue;
-      f32x4 sum = acc[l][r];
-      if (a.sums) {
-        f32x4* kept = (f32x4*)(a.sums + ((int64_t)at * TR + v) * a.hidden + d0 + d);
-        if (!a.first) sum += *kept;
-        if (!a.last) {
-          *kept = sum;
-          continue;
+    for (int l = 0; l < Product::FL; ++l)
+#pragma unroll
+      for (int q = 0; q < Product::kQuads; ++q) {
+        const int v = Product::r_of(threadIdx.x, r), d = Product::l_of(threadIdx.x, l, q);
+        if (v >= rows || d >= width) continue;
+        f32x4 sum = Product::quad(acc[l][r], q);
+        if (a.sums) {
+          f32x4* kept = (f32x4*)(a.sums + ((int64_t)at * TR + v) * a.hidden + d0 + d);
+          if (!a.first) sum += *kept;
+          if (!a.last) {
+            *kept = sum;
+            continue;
+          }
         }
+        *(typename Half<T>::x4*)(grads.dw[rank] + (row0 + v) * a.dw_stride + (d0 + d) * 2) = narrow<T>(sum, back);
       }
-      *(typename Half<T>::x4*)(grads.dw[rank] + (row0 + v) * a.dw_stride + (d0 + d) * 2) = narrow<T>(sum, back);
-    }
 }
 
 int launched(const char* what) {
@@ -507,38 +541,35 @@ int check_call(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool 
 int tiles(int64_t n, int of = kTile) { return (int)((n + of - 1) / of); }
 
 enum { kLarge, kMiddle, kFew };
-int pick_shape(const char* name, int automatic) {
-#ifdef MSCCLX_SWEEP
-  if (const char* v = getenv(name)) return atoi(v);
-#endif
-  return automatic;
-}
-
 constexpr int kUnits = 256;  // compute units
 
-// Which shape a product of `rows` x `cols` takes.
-int shape_of(const char* name, int64_t rows, int64_t cols, int64_t tokens, bool few) {
-  const int automatic = few && tokens <= Few::kR ? kFew : (int64_t)tiles(rows, 256) * tiles(cols, 256) >= kUnits ? kLarge : kMiddle;
-  return pick_shape(name, automatic);
+// Which shape a product takes, by tokens x vocabulary x hidden (bf16, us with the shape / with the next best).
+// Logits: Few up to four rounds of its workgroups (128 x 8192 x 1024: 14.8 / 19.0 Middle; 40 x 65536 x 4096: 123 / 133) but not where W would be read
+// again from memory for every 32 tokens (128 x 65536 x 4096: 208 / 142 Middle); Large once its tiles fill the chip (384 x 32768 x 2048: 58 / 67
+// Middle) and are not half empty, else Middle (256 x 32768 x 2048: 44 / 52 Large).
+int logits_shape(const Pieces& p, int64_t tokens) {
+  if (tokens <= 256 && (int64_t)tiles(tokens, Few::kR) * p.tiles * (kTile / Few::kL) <= 4 * kUnits) return kFew;
+  return tokens <= 128 || (int64_t)tiles(tokens) * p.tiles < kUnits ? kMiddle : kLarge;
 }
+// dw writes more than it reads where tokens are few: two workgroups per unit then hide each other's stores (dw's part of 128 x 65536 x 4096 is 75 us shorter
+// with Middle); 1021 x 32003 x 1288: Large 15 us shorter.
+int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 256 || (int64_t)p.tiles * tiles(hidden) < kUnits ? kMiddle : kLarge; }
 
-// Into how many parts dx cuts the vocabulary of `steps` steps, so that `count` tiles fill `slots` workgroups.
-int parts_of(int64_t count, int steps, int slots) {
-  const int parts = pick_shape("DX_PARTS", (int)std::min<int64_t>(steps / 4, slots / std::max<int64_t>(1, count)));
-  return std::max(1, std::min(parts, steps));
-}
-
+// dx: into how many parts the vocabulary is cut so that the tiles fill the chip, of at least eight steps each (with four, 1024 x 4096 x 512 takes 5 us
+// longer).  Few as long as reading W again for every 32 tokens costs little (128 x 8192 x 1024: 3 us shorter than Middle; 40 x 65536 x 4096: 26 us longer).
 struct DxPlan {
   int shape, token_tiles, hidden_tiles, parts, split_steps;
 };
 DxPlan dx_plan(const Pieces& p, int64_t tokens, int hidden) {
   DxPlan d;
   const int steps = p.tiles * (kTile / kStepK);
-  d.shape = pick_shape("DX_SHAPE", tokens <= Few::kR ? kFew : tokens <= Middle::kR ? kMiddle : kLarge);
+  const int64_t again = (int64_t)(tiles(tokens, Few::kR) - 1) * p.tiles * kTile * hidden * 2;
+  d.shape = again <= 64 << 20 && tokens <= 256 ? kFew : tiles(tokens) * tiles(hidden) < 24 ? kMiddle : kLarge;
   const int l = d.shape == kLarge ? Large::kL : d.shape == kMiddle ? Middle::kL : Few::kL, r = d.shape == kLarge ? Large::kR : d.shape == kMiddle ? Middle::kR : Few::kR;
   d.token_tiles = tiles(tokens, r);
   d.hidden_tiles = tiles(hidden, l);
-  const int parts = parts_of((int64_t)d.token_tiles * d.hidden_tiles, steps, d.shape == kLarge ? kUnits : 2 * kUnits);
+  const int64_t slots = d.shape == kMiddle ? 2 * kUnits : kUnits;
+  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, slots / ((int64_t)d.token_tiles * d.hidden_tiles)));
   d.split_steps = (steps + parts - 1) / parts;
   d.parts = (steps + d.split_steps - 1) / d.split_steps;
   return d;
@@ -589,7 +620,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
     a.e = c.e;
     a.lse = io->lse;
     if (now > 0) {
-      const int shape = shape_of("LOGITS_SHAPE", now, (int64_t)p.tiles * kTile, now, true);
+      const int shape = logits_shape(p, now);
       if ((rc = !forward ? launch_logits<T, kGradient>(shape, p, a, stream) : backward ? launch_logits<T, kKeep>(shape, p, a, stream) : launch_logits<T, kStats>(shape, p, a, stream)))
         return rc;
       if (forward) {
@@ -648,7 +679,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
       hipLaunchKernelGGL((dw_kernel<T, S>), dim3((unsigned)(p.tiles * (kTile / S::kR) * g.hidden_tiles)), dim3(S::kThreads), 0, stream, p, c.grads, g);
       return launched("dw_kernel");
     };
-    if ((rc = shape_of("DW_SHAPE", (int64_t)p.tiles * kTile, d.hidden, now, false) == kLarge ? go(Large()) : go(Middle()))) return rc;
+    if ((rc = dw_shape(p, now, d.hidden) == kLarge ? go(Large()) : go(Middle()))) return rc;
   }
   if (n == 0 && forward && !per_token && !backward) return sums(true);
   return MSCCLX_OK;
@@ -716,7 +747,7 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
     h->off_loss = take(n * 4);
     h->off_factor = take(n * 4);
     const uint64_t wide = (uint64_t)p.tiles * kTile;
-    h->off_stats = take(std::max(std::min<uint64_t>(h->piece, Few::kR) * (wide / (Few::kL / Few::kWavesL)), (uint64_t)h->piece * (wide / (Middle::kL / Middle::kWavesL))) * sizeof(float2));
+    h->off_stats = take(std::max(std::min<uint64_t>(h->piece, 256) * (wide / (Few::kL / Few::kWavesL)), (uint64_t)h->piece * (wide / (Middle::kL / Middle::kWavesL))) * sizeof(float2));
     h->off_e = d.gradients ? take((uint64_t)h->piece * row) : 0;
     h->off_sums = d.gradients && d.max_tokens > h->piece ? take((uint64_t)p.tiles * kTile * d.hidden * 4) : 0;
     uint64_t parts = 0;  // dx's parts at the token count that needs most of them; its plan is the same for (32 k, 32 k + 32] tokens
