@@ -310,7 +310,7 @@ int mscclx_grad_clip_destroy(mscclx_grad_clip* clip);
  * out = NULL: norms only; out[i] = in[i]: in place.  Otherwise no output may overlap another buffer (ALIASED).  Not while a launch of
  * the previous binding is in flight, and not while `stream` is being captured. */
 int mscclx_grad_clip_bind(mscclx_grad_clip* clip, const void* const* in, void* const* out, void* workspace, uint64_t workspace_bytes, void* stream);
-/* Enqueues two kernels on `stream`; can be captured in a HIP graph.  max_norm < 0: the norm only.  The results are the two floats at
+/* Enqueues one kernel (the norm only: max_norm < 0) or two on `stream`; can be captured in a HIP graph.  The results are the two floats at
  * the start of the workspace: norm, coefficient.  Launches of one binding must follow each other on one stream. */
 int mscclx_grad_clip_launch(const mscclx_grad_clip* clip, float scale, float max_norm, void* stream);
 

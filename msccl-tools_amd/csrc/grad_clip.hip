@@ -3,12 +3,14 @@
 //   norm = |scale| sqrt(sum g^2)  or  |scale| max |g|      over all tensors that count
 //   c    = min(1, max_norm / (norm + 1e-6)),   out = g scale c
 //
-// Two launches.  The first reads every counted tensor once: squares are added in 64 bits (exact for the squares themselves, so no large
-// gradient overflows and no small one is lost; two conversions' and one multiply-add's time per element, a fifth of what memory takes), magnitudes are compared as
-// unsigned integers, in which NaN is above infinity.  Each workgroup leaves one partial result.  The second adds the partial
-// results in one order in every workgroup (no atomics: the same bits at every call) and scales.  Tensors are cut
-// into chunks of kChunk elements; workgroup b takes chunks b, b + grid, ...  The second launch walks them backwards: what the first read last
-// is still in the memory-side cache.
+// Tensors are cut into chunks; a table in the workspace holds each chunk's addresses, so that a workgroup is two dependent loads from its
+// data.  Workgroup b takes chunks b, b + grid, ...
+//
+// The first kernel reads every counted chunk once: squares are added in 64 bits (they are exact there, so no large
+// gradient overflows and no small one is lost; two conversions and a multiply-add per element, a fifth of what memory takes), magnitudes are
+// compared as unsigned integers, in which NaN is above infinity.  Each workgroup leaves one partial result.
+// The norm alone: the last workgroup to arrive adds the partial results, in one order.  Clipping: a second kernel, in which
+// every workgroup adds them, in the same order, and scales its chunks.  No sum goes through an atomic: the same bits at every call.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -24,23 +26,23 @@
 namespace mscclx {
 namespace {
 
-constexpr int kChunk = 16384;    // elements
-constexpr int kMaxGrid = 2048;   // workgroups, and partial results
+constexpr int kMinChunk = 2048, kMaxChunk = 16384;  // elements
+constexpr int kMaxGrid = 2048;                         // workgroups, and partial results
 constexpr int kThreads = 256;
+constexpr int kArrivals = 64;                          // counters of finished workgroups: one for all is a queue of 2048
 
-struct Tensor {
+struct Chunk {
   const void* in;
   void* out;
-  uint64_t n;
-  int32_t in_type, out_type;
-  int32_t counted, reserved;
+  uint32_t n;
+  uint8_t in_type, out_type, counted, reserved[9];
 };
-struct Chunk {
-  uint32_t tensor, index;
-};
+static_assert(sizeof(Chunk) == 32, "two 16-byte loads");
 
 struct alignas(256) Header {
   float norm, coefficient;
+  unsigned done;                  // counters whose last workgroup has arrived
+  unsigned arrived[kArrivals][16];  // each alone in 64 bytes; the last to arrive leaves zeros
 };
 
 __device__ __forceinline__ float widen(float x) { return x; }
@@ -86,21 +88,36 @@ template <> struct Norm<true> {
   static __device__ __forceinline__ double result(unsigned a) { return (double)__uint_as_float(a); }
 };
 
+// The result from the partial results' sum; `threadIdx.x == 0` writes it.  Returns the factor.
 template <bool MAX>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const Tensor* tensors, const Chunk* chunks, int nchunks, typename Norm<MAX>::value* partial) {
+__device__ __forceinline__ float finish(typename Norm<MAX>::value sum, float scale, float max_norm, Header* header, bool writes) {
+  const double norm = Norm<MAX>::result(sum) * fabs((double)scale);
+  double c = 1.0;
+  if (max_norm >= 0.f) {
+    c = (double)max_norm / (norm + 1e-6);
+    if (c >= 1.0) c = 1.0;  // (a NaN stays)
+  }
+  if (writes && threadIdx.x == 0) {
+    header->norm = (float)norm;
+    header->coefficient = (float)c;
+  }
+  return (float)(c * scale);
+}
+
+template <bool MAX>
+__global__ void __launch_bounds__(kThreads) norm_kernel(const Chunk* chunks, int nchunks, typename Norm<MAX>::value* partial, int alone, float scale, Header* header) {
   typedef Norm<MAX> N;
-  __shared__ typename N::value shared[kThreads / 64];
-  typename N::value sum = 0;
+  typedef typename N::value V;
+  __shared__ V shared[kThreads / 64];
+  V sum = 0;
   for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
-    const Chunk chunk = chunks[c];
-    const Tensor t = tensors[chunk.tensor];
+    const Chunk t = chunks[c];
     if (!t.counted) continue;
-    const uint64_t from = (uint64_t)chunk.index * kChunk;
-    const int n = (int)min((uint64_t)kChunk, t.n - from);
     by_type(t.in_type, [&](auto* type) {
       typedef std::remove_pointer_t<decltype(type)> T;
       constexpr int W = 16 / sizeof(T);
-      const T* p = (const T*)t.in + from;
+      const T* p = (const T*)t.in;
+      const int n = (int)t.n;
       int i = threadIdx.x * W;
 #pragma unroll 4
       for (; i + W <= n; i += kThreads * W) {
@@ -112,53 +129,58 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const Tensor* tensors, c
       for (; i < n && i + W > n; ++i) sum = N::of(sum, widen(p[i]));  // the one thread at the end
     });
   }
-  sum = over_workgroup(sum, [](auto a, auto b) { return N::join(a, b); }, shared);
-  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+  auto join = [](V a, V b) { return N::join(a, b); };
+  sum = over_workgroup(sum, join, shared);
+  if (!alone) {
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+    return;
+  }
+  // Who arrives last adds: of the workgroups of a counter, then of the counters.  Release and acquire would write back and drop this XCD's cache for every
+  // workgroup (norm over 256 MiB: 101 us instead of 42).  They are not needed: the partial result is exchanged, not stored, so its old value
+  // comes back only when the new one is where all XCDs see it, and each next atomic waits for the value of the one before; the loads
+  // below go to the same place.
+  __shared__ int last;
+  if (threadIdx.x == 0) {
+    typedef std::conditional_t<sizeof(V) == 8, unsigned long long, unsigned> Bits;
+    const Bits before = __hip_atomic_exchange((Bits*)&partial[blockIdx.x], __builtin_bit_cast(Bits, sum), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::"v"(before) : "memory");
+    const unsigned grid = gridDim.x, mine = blockIdx.x % kArrivals, of_mine = (grid - mine + kArrivals - 1) / kArrivals;
+    last = 0;
+    if (__hip_atomic_fetch_add(&header->arrived[mine][0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == of_mine) {
+      __hip_atomic_store(&header->arrived[mine][0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (__hip_atomic_fetch_add(&header->done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == min(grid, (unsigned)kArrivals)) {
+        __hip_atomic_store(&header->done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = 1;
+      }
+    }
+  }
+  __syncthreads();
+  if (!last) return;
+  sum = 0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kThreads) sum = N::join(sum, __hip_atomic_load(&partial[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  finish<MAX>(over_workgroup(sum, join, shared), scale, -1.f, header, true);
 }
 
-// the partial results' sum in every workgroup, in the same order
 template <bool MAX>
-__device__ __forceinline__ float factor_of(const typename Norm<MAX>::value* partial, int count, float scale, float max_norm, Header* header) {
+__global__ void __launch_bounds__(kThreads) scale_kernel(const Chunk* chunks, int nchunks, const typename Norm<MAX>::value* partial, float scale, float max_norm,
+                                                         Header* header) {
   typedef Norm<MAX> N;
-  __shared__ typename N::value shared[kThreads / 64];
-  typename N::value sum = 0;
-  for (int i = threadIdx.x; i < count; i += kThreads) sum = N::join(sum, partial[i]);
-  sum = over_workgroup(sum, [](auto a, auto b) { return N::join(a, b); }, shared);
-  const double norm = N::result(sum) * fabs((double)scale);
-  double c = 1.0;
-  if (max_norm >= 0.f) {
-    c = (double)max_norm / (norm + 1e-6);
-    if (c >= 1.0) c = 1.0;  // (a NaN stays)
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    header->norm = (float)norm;
-    header->coefficient = (float)c;
-  }
-  return (float)(c * scale);
-}
-
-template <bool MAX>
-__global__ void __launch_bounds__(kThreads) finish_kernel(const typename Norm<MAX>::value* partial, int count, float scale, Header* header) {
-  factor_of<MAX>(partial, count, scale, -1.f, header);
-}
-
-template <bool MAX>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const Tensor* tensors, const Chunk* chunks, int nchunks, const typename Norm<MAX>::value* partial,
-                                                         int count, float scale, float max_norm, Header* header) {
-  const float factor = factor_of<MAX>(partial, count, scale, max_norm, header);
+  typedef typename N::value V;
+  __shared__ V shared[kThreads / 64];
+  V sum = 0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kThreads) sum = N::join(sum, partial[i]);
+  const float factor = finish<MAX>(over_workgroup(sum, [](V a, V b) { return N::join(a, b); }, shared), scale, max_norm, header, blockIdx.x == 0);
   for (int b = blockIdx.x; b < nchunks; b += gridDim.x) {
-    const Chunk chunk = chunks[nchunks - 1 - b];
-    const Tensor t = tensors[chunk.tensor];
+    const Chunk t = chunks[b];
     if (factor == 1.f && t.in == t.out) continue;  // nothing changes (in place, types are the same)
-    const uint64_t from = (uint64_t)chunk.index * kChunk;
-    const int n = (int)min((uint64_t)kChunk, t.n - from);
     by_type(t.in_type, [&](auto* in_type) {
       by_type(t.out_type, [&](auto* out_type) {
         typedef std::remove_pointer_t<decltype(in_type)> T;
         typedef std::remove_pointer_t<decltype(out_type)> U;
-        constexpr int W = 16 / sizeof(T);
-        const T* p = (const T*)t.in + from;
-        U* q = (U*)t.out + from;
+        constexpr int W = 16 / std::max(sizeof(T), sizeof(U));
+        const T* p = (const T*)t.in;
+        U* q = (U*)t.out;
+        const int n = (int)t.n;
         int i = threadIdx.x * W;
 #pragma unroll 4
         for (; i + W <= n; i += kThreads * W) {
@@ -196,10 +218,16 @@ template <class F> int guarded(F f) {
 using namespace mscclx;
 
 struct mscclx_grad_clip {
+  struct Tensor {
+    uint64_t n;
+    int32_t in_type, out_type;
+    bool counted;
+  };
   std::vector<Tensor> tensors;
-  std::vector<Chunk> chunks;
   int norm = 0;
-  uint64_t off_partial = 0, off_tensors = 0, off_chunks = 0, bytes = 0;
+  uint64_t chunk = kMinChunk;  // elements
+  uint64_t chunks = 0;
+  uint64_t off_partial = 0, off_chunks = 0, bytes = 0;
   char* workspace = nullptr;  // of the last bind
   bool outputs = false;
 };
@@ -215,29 +243,26 @@ int mscclx_grad_clip_create(int32_t ntensors, const uint64_t* sizes, const int32
     auto type_ok = [](int32_t t) { return t == MSCCLX_F32 || t == MSCCLX_F16 || t == MSCCLX_BF16; };
     std::unique_ptr<mscclx_grad_clip> h(new mscclx_grad_clip());
     h->norm = norm;
-    uint64_t chunks = 0;
+    uint64_t total = 0;
     for (int i = 0; i < ntensors; ++i) {
       if (!type_ok(in_dtypes[i]) || !type_ok(out_dtypes[i]))
         return fail(MSCCLX_ERR_UNSUPPORTED, "tensor " + std::to_string(i) + ": gradients are float32, float16 or bfloat16");
       if (sizes[i] > (1ull << 40)) return fail(MSCCLX_ERR_INVALID_ARG, "tensor " + std::to_string(i) + ": more than 2^40 elements");
-      chunks += (sizes[i] + kChunk - 1) / kChunk;
-      if (chunks > (1ull << 30)) return fail(MSCCLX_ERR_CAPACITY, "more than 2^30 chunks of gradients");
+      total += sizes[i];
+      if (total > (1ull << 44)) return fail(MSCCLX_ERR_CAPACITY, "more than 2^44 gradients");
+      h->tensors.push_back({sizes[i], in_dtypes[i], out_dtypes[i], !counted || counted[i]});
     }
-    h->tensors.reserve(ntensors);
-    h->chunks.reserve(chunks);
-    for (int i = 0; i < ntensors; ++i) {
-      h->tensors.push_back(Tensor{nullptr, nullptr, sizes[i], in_dtypes[i], out_dtypes[i], counted ? counted[i] != 0 : 1, 0});
-      for (uint64_t c = 0; c < (sizes[i] + kChunk - 1) / kChunk; ++c) h->chunks.push_back(Chunk{(uint32_t)i, (uint32_t)c});
-    }
-    uint64_t at = sizeof(Header);
+    // eight chunks for each workgroup of a full grid, so that the last ones are short against the whole; of at least one pass of its threads
+    while (h->chunk < kMaxChunk && h->chunk * kMaxGrid * 8 < total) h->chunk *= 2;
+    for (const auto& t : h->tensors) h->chunks += (t.n + h->chunk - 1) / h->chunk;
+    uint64_t at = (sizeof(Header) + 255) / 256 * 256;
     auto take = [&](uint64_t bytes) {
       const uint64_t here = at;
       at += (bytes + 255) / 256 * 256;
       return here;
     };
     h->off_partial = take(kMaxGrid * sizeof(double));
-    h->off_tensors = take(h->tensors.size() * sizeof(Tensor));
-    h->off_chunks = take(h->chunks.size() * sizeof(Chunk));
+    h->off_chunks = take(h->chunks * sizeof(Chunk));
     h->bytes = at;
     if (workspace_bytes) *workspace_bytes = at;
     *out = h.release();
@@ -262,21 +287,23 @@ int mscclx_grad_clip_bind(mscclx_grad_clip* h, const void* const* in, void* cons
       bool written;
     };
     std::vector<Span> spans;
-    std::vector<Tensor> tensors = h->tensors;
-    for (size_t i = 0; i < tensors.size(); ++i) {
-      Tensor& t = tensors[i];
-      t.in = t.n && in ? in[i] : nullptr;
-      t.out = t.n && out ? out[i] : nullptr;
+    std::vector<Chunk> chunks;
+    chunks.reserve(h->chunks);
+    for (size_t i = 0; i < h->tensors.size(); ++i) {
+      const mscclx_grad_clip::Tensor& t = h->tensors[i];
       if (!t.n) continue;
       const std::string name = "tensor " + std::to_string(i);
-      if (!t.in || (out && !t.out)) return fail(MSCCLX_ERR_INVALID_ARG, name + ": NULL");
-      const uintptr_t in_size = dtype_size(t.in_type), out_size = dtype_size(t.out_type);
-      if ((uintptr_t)t.in % in_size || (uintptr_t)t.out % out_size) return fail(MSCCLX_ERR_INVALID_ARG, name + ": not aligned to its element type");
-      if (out && t.in == t.out && t.in_type != t.out_type) return fail(MSCCLX_ERR_ALIASED, name + ": in place, but its types differ");
-      const uintptr_t a = (uintptr_t)t.in, b = (uintptr_t)t.out;
+      const uintptr_t a = in ? (uintptr_t)in[i] : 0, b = out ? (uintptr_t)out[i] : 0;
+      if (!a || (out && !b)) return fail(MSCCLX_ERR_INVALID_ARG, name + ": NULL");
+      const uint64_t in_size = dtype_size(t.in_type), out_size = dtype_size(t.out_type);
+      if (a % in_size || b % out_size) return fail(MSCCLX_ERR_INVALID_ARG, name + ": not aligned to its element type");
       const bool in_place = out && a == b;
+      if (in_place && t.in_type != t.out_type) return fail(MSCCLX_ERR_ALIASED, name + ": in place, but its types differ");
       spans.push_back({a, a + t.n * in_size, (int)i, in_place});
       if (out && !in_place) spans.push_back({b, b + t.n * out_size, (int)i, true});
+      for (uint64_t from = 0; from < t.n; from += h->chunk)
+        chunks.push_back({(const void*)(a + from * in_size), out ? (void*)(b + from * out_size) : nullptr, (uint32_t)std::min(h->chunk, t.n - from), (uint8_t)t.in_type,
+                          (uint8_t)t.out_type, (uint8_t)t.counted, {}});
     }
     // what one tensor writes no other may read or write (two inputs may share memory)
     std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
@@ -287,13 +314,13 @@ int mscclx_grad_clip_bind(mscclx_grad_clip* h, const void* const* in, void* cons
     }
     char* ws = (char*)workspace;
     hipStream_t s = (hipStream_t)stream;
-    hipError_t e = hipSuccess;
-    if (!tensors.empty()) e = hipMemcpyAsync(ws + h->off_tensors, tensors.data(), tensors.size() * sizeof(Tensor), hipMemcpyHostToDevice, s);
-    if (e == hipSuccess && !h->chunks.empty()) e = hipMemcpyAsync(ws + h->off_chunks, h->chunks.data(), h->chunks.size() * sizeof(Chunk), hipMemcpyHostToDevice, s);
+    const Header zeros = {};
+    hipError_t e = hipMemcpyAsync(ws, &zeros, sizeof(Header), hipMemcpyHostToDevice, s);
+    if (e == hipSuccess && !chunks.empty()) e = hipMemcpyAsync(ws + h->off_chunks, chunks.data(), chunks.size() * sizeof(Chunk), hipMemcpyHostToDevice, s);
     if (e == hipSuccess) e = hipStreamSynchronize(s);
     if (e != hipSuccess) {
       h->workspace = nullptr;
-      return fail(MSCCLX_ERR_HIP, std::string("uploading the table of tensors: ") + hipGetErrorString(e));
+      return fail(MSCCLX_ERR_HIP, std::string("uploading the table of gradients: ") + hipGetErrorString(e));
     }
     h->workspace = ws;
     h->outputs = out != nullptr;
@@ -309,18 +336,18 @@ int mscclx_grad_clip_launch(const mscclx_grad_clip* h, float scale, float max_no
     const bool clip = max_norm >= 0.f;
     if (clip && !h->outputs) return fail(MSCCLX_ERR_STATE, "the tensors were bound without outputs");
     char* ws = h->workspace;
-    const int nchunks = (int)h->chunks.size(), grid = std::max(1, std::min(nchunks, kMaxGrid));
-    const Tensor* tensors = (const Tensor*)(ws + h->off_tensors);
+    const int nchunks = (int)h->chunks, grid = std::max(1, std::min(nchunks, kMaxGrid));
     const Chunk* chunks = (const Chunk*)(ws + h->off_chunks);
+    Header* header = (Header*)ws;
     hipStream_t s = (hipStream_t)stream;
     auto both = [&](auto max) -> int {
       constexpr bool MAX = decltype(max)::value;
       auto* partial = (typename Norm<MAX>::value*)(ws + h->off_partial);
-      hipLaunchKernelGGL((norm_kernel<MAX>), dim3(grid), dim3(kThreads), 0, s, tensors, chunks, nchunks, partial);
+      hipLaunchKernelGGL((norm_kernel<MAX>), dim3(grid), dim3(kThreads), 0, s, chunks, nchunks, partial, (int)!clip, scale, header);
       if (int rc = launched("norm_kernel")) return rc;
-      if (!clip) hipLaunchKernelGGL((finish_kernel<MAX>), dim3(1), dim3(kThreads), 0, s, partial, grid, scale, (Header*)ws);
-      else hipLaunchKernelGGL((scale_kernel<MAX>), dim3(grid), dim3(kThreads), 0, s, tensors, chunks, nchunks, partial, grid, scale, max_norm, (Header*)ws);
-      return launched(clip ? "scale_kernel" : "finish_kernel");
+      if (!clip) return MSCCLX_OK;
+      hipLaunchKernelGGL((scale_kernel<MAX>), dim3(grid), dim3(kThreads), 0, s, chunks, nchunks, partial, scale, max_norm, header);
+      return launched("scale_kernel");
     };
     return h->norm == MSCCLX_NORM_MAX ? both(std::true_type()) : both(std::false_type());
   });

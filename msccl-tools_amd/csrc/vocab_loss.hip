@@ -9,7 +9,7 @@
 //            vocabulary, the maximum m (in units of log 2) and the sum of exp(z - m), and with gradients E = exp(z - m) in 16 bits;
 //   tokens   a token's (m, sum) become its lse and loss, and its E becomes G in place: G = (E exp(m - lse) - [label]) g / max|g|;
 //   dx, dw   the two products, on G.  dx sums over the whole vocabulary: where its tiles do not fill the chip, that
-//            axis is cut and the parts are added by a kernel of their own.
+//            axis is cut and the parts are added by workgroups that dw's launch has more.
 // The 16-bit E and G are what the matrix cores take.  Both are rounded relative to their own size (bf16 2^-9 on average, as the outputs
 // are), with 2^15 as unit in fp16, so that probabilities down to 2^-29 are normal numbers; |g| is divided by its largest value for
 // the same reason and multiplied back in 32 bits behind the products.
@@ -228,7 +228,8 @@ struct TokenArgs {
   void* e;
 };
 
-// A workgroup per token: its parts' (m, sum) -> lse and loss; KEEP: its E -> G in place
+// A workgroup per token: its parts' (m, sum) -> lse and loss; KEEP: its E -> G in place.  Where tokens are few, several workgroups share one: each
+// works out the lse for itself (a thirtieth of what it then moves) and takes gridDim.y'ths of E.
 template <class T, bool KEEP>
 __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const TokenArgs a) {
   __shared__ float shared[4];
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
   sum = block_reduce(sum, [](float a, float b) { return a + b; }, shared);
   const float lse2 = base + log2f(sum), lse = lse2 * kLn2;
   const int label = a.labels.get(at);
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && blockIdx.y == 0) {
     a.lse[at] = lse;
     a.loss[at] = label == -1 ? 0.f : label < 0 ? NAN : lse - a.z_label[at];
   }
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
     }
     typedef typename Half<T>::x8 x8;
     T* e = (T*)a.e + blockIdx.x * ld;
-    for (int64_t v = threadIdx.x * 8; v < ld; v += 256 * 8) {
+    for (int64_t v = (blockIdx.y * 256 + threadIdx.x) * 8; v < ld; v += gridDim.y * 256 * 8) {
       const float top = stats[v / a.part].x;
       const float f = top == -INFINITY ? 0.f : exp2_of(top - lse2) * g;
       x8 o = *(x8*)(e + v);
@@ -271,38 +272,52 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
   }
 }
 
-// One workgroup over all tokens: the loss as one number (rows given), in 64 bits and in one order; with gradients what the
-// products are multiplied by, max |g| (over the mean's count) over the unit, and with a number per token factor[n] = g[n] / max |g|.
-__global__ void __launch_bounds__(1024) sums_kernel(int64_t tokens, Labels labels, int mean, const float* rows, float* loss, const float* upstream, float* factor,
-                                                    float unit, float* back) {
-  __shared__ double shared[16];
+struct SumsArgs {
+  int64_t tokens;
+  Labels labels;
+  int mean;
+  const float* rows;      // null: no loss
+  float* loss;
+  const float* upstream;  // null: no gradients
+  float* factor;          // null: one number for all tokens
+  float unit;
+  float* back;
+};
+
+// One workgroup over all tokens: the loss as one number, in 64 bits and in one order; with gradients what the products are
+// multiplied by, max |g| (over the mean's count) over the unit, and with a number per token factor[n] = g[n] / max |g|.
+__device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shared) {
   double sum = 0, count = 0;
   float top = 0.f;
-  for (int64_t n = threadIdx.x; n < tokens; n += 1024) {
-    const int label = labels.get(n);
+  for (int64_t n = threadIdx.x; n < a.tokens; n += blockDim.x) {
+    const int label = a.labels.get(n);
     count += label != -1;
-    if (rows) sum += rows[n];
-    if (factor && label >= 0) top = fmaxf(top, fabsf(upstream[n]));
+    if (a.rows) sum += a.rows[n];
+    if (a.factor && label >= 0) top = fmaxf(top, fabsf(a.upstream[n]));
   }
   auto add = [](double a, double b) { return a + b; };
-  if (mean) count = fmax(block_reduce(count, add, shared), 1.0);
+  if (a.mean) count = fmax(block_reduce(count, add, shared), 1.0);
   else count = 1.0;
-  if (rows) {
+  if (a.rows) {
     sum = block_reduce(sum, add, shared);
-    if (threadIdx.x == 0) *loss = (float)(sum / count);
+    if (threadIdx.x == 0) *a.loss = (float)(sum / count);
   }
-  if (!upstream) return;
-  if (factor) {
+  if (!a.upstream) return;
+  if (a.factor) {
     top = (float)block_reduce((double)top, [](double a, double b) { return fmax(a, b); }, shared);
-    for (int64_t n = threadIdx.x; n < tokens; n += 1024) {
-      const int label = labels.get(n);
-      const float g = upstream[n];
-      factor[n] = label == -1 ? 0.f : label < 0 ? NAN : g == 0.f ? 0.f : g / top;
+    for (int64_t n = threadIdx.x; n < a.tokens; n += blockDim.x) {
+      const int label = a.labels.get(n);
+      const float g = a.upstream[n];
+      a.factor[n] = label == -1 ? 0.f : label < 0 ? NAN : g == 0.f ? 0.f : g / top;
     }
   } else {
-    top = fabsf(*upstream);
+    top = fabsf(*a.upstream);
   }
-  if (threadIdx.x == 0) *back = (float)((double)top / count / unit);
+  if (threadIdx.x == 0) *a.back = (float)((double)top / count / a.unit);
+}
+__global__ void __launch_bounds__(1024) sums_kernel(const SumsArgs a) {
+  __shared__ double shared[16];
+  sums_over_tokens(a, shared);
 }
 
 // The rows of all ranks' pieces as k of a product, in steps of kStepK; what pads a rank's last tile counts as outside.
@@ -345,6 +360,9 @@ struct GradArgs {
   int hidden, tokens, token_tiles, hidden_tiles;
   int split_steps;   // dx: steps of kStepK for each part of the vocabulary
   float* parts;      // dx: [parts][tokens][hidden]; null: one part
+  int count;         // of parts
+  int with_sums;     // dx: one workgroup more, for the sums over tokens
+  int adders;        // dw: so many workgroups more, in front, that add dx's parts
   char* dx;
   int64_t dx_stride, dw_stride;
   const float* back;
@@ -360,10 +378,14 @@ template <class T> __device__ __forceinline__ typename Half<T>::x4 narrow(f32x4 
 }
 
 template <class T, class Shape>
-__global__ void __launch_bounds__(Shape::kThreads, 2) dx_kernel(const Pieces pieces, const GradArgs a) {
+__global__ void __launch_bounds__(Shape::kThreads, 2) dx_kernel(const Pieces pieces, const GradArgs a, const SumsArgs sums) {
   typedef typename Shape::template Product<T, true, false> Product;
   constexpr int TL = Shape::kL, TR = Shape::kR;
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
+  if (blockIdx.x == a.token_tiles * a.hidden_tiles) {
+    if (blockIdx.y == 0) sums_over_tokens(sums, (double*)smem);
+    return;
+  }
   int tt, ht;
   tile_of(blockIdx.x, a.token_tiles, a.hidden_tiles, &tt, &ht);
   const int n0 = tt * TR, d0 = ht * TL, tokens = min(TR, a.tokens - n0), width = min(TL, a.hidden - d0);
@@ -378,7 +400,7 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dx_kernel(const Pieces pie
     Product::run(smem, steps, ll, PieceSource(&pieces, a.w_stride, d0 * 2, step0 * kStepK), rl,
                  RowSource{(const char*)a.g + (n0 * ld + (int64_t)step0 * kStepK) * 2, ld}, acc);
   }
-  const float back = *a.back;
+  const float back = a.parts ? 0.f : *a.back;  // (with parts the sums may still be under way)
 #pragma unroll
   for (int r = 0; r < Product::FR; ++r)
 #pragma unroll
@@ -393,15 +415,16 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dx_kernel(const Pieces pie
       }
 }
 
-// dx from the parts of the vocabulary: four values per thread
-template <class T>
-__global__ void __launch_bounds__(256) add_parts_kernel(const float* parts, int count, int tokens, int hidden, char* dx, int64_t dx_stride, const float* back) {
-  const int64_t size = (int64_t)tokens * hidden, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= size) return;
-  f32x4 sum = {};
+// dx from the parts of the vocabulary: four values per thread and turn
+template <class T> __device__ __forceinline__ void add_parts(const GradArgs& a) {
+  const int64_t size = (int64_t)a.tokens * a.hidden;
+  const float back = *a.back;
+  for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4; i < size; i += (int64_t)a.adders * blockDim.x * 4) {
+    f32x4 sum = {};
 #pragma unroll 8
-  for (int p = 0; p < count; ++p) sum += *(const f32x4*)(parts + p * size + i);
-  *(typename Half<T>::x4*)(dx + i / hidden * dx_stride + i % hidden * 2) = narrow<T>(sum, *back);
+    for (int p = 0; p < a.count; ++p) sum += *(const f32x4*)(a.parts + p * size + i);
+    *(typename Half<T>::x4*)(a.dx + i / a.hidden * a.dx_stride + i % a.hidden * 2) = narrow<T>(sum, back);
+  }
 }
 
 template <class T, class Shape>
@@ -409,8 +432,9 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dw_kernel(const Pieces pie
   typedef typename Shape::template Product<T, true, true> Product;
   constexpr int TL = Shape::kL, TR = Shape::kR;
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
+  if ((int)blockIdx.x < a.adders) return add_parts<T>(a);
   int at, ht;
-  tile_of(blockIdx.x, pieces.tiles * (kTile / TR), a.hidden_tiles, &at, &ht);
+  tile_of(blockIdx.x - a.adders, pieces.tiles * (kTile / TR), a.hidden_tiles, &at, &ht);
   const int rank = pieces.rank_of(at / (kTile / TR)), row0 = at * TR - pieces.tile0[rank] * kTile, rows = min(TR, pieces.rows[rank] - row0);
   if (rows <= 0) return;  // padding
   const int d0 = ht * TL, width = min(TL, a.hidden - d0);
@@ -594,10 +618,14 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
   const int mean = d.reduction == MSCCLX_LOSS_MEAN, per_token = d.reduction == MSCCLX_LOSS_NONE;
   const Upstream upstream = {io->grad_loss, per_token ? c.factor : nullptr};
   int rc;
-  // one number: with the losses, behind the last piece's tokens and in front of its gradients; else first of all
+  // The sums over tokens.  One number: with the losses, behind the last piece's tokens and in front of its gradients (or beside them: dx's
+  // parts do without); else first of all.
+  SumsArgs totals = {n, c.labels, mean, forward && !per_token ? c.row_loss : nullptr, io->loss, backward ? io->grad_loss : nullptr, per_token ? c.factor : nullptr,
+                     kUnit<T>, c.back};
   auto sums = [&](bool losses) {
-    hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, stream, n, c.labels, mean, losses ? c.row_loss : nullptr, io->loss, backward ? io->grad_loss : nullptr,
-                       per_token ? c.factor : nullptr, kUnit<T>, c.back);
+    SumsArgs now = totals;
+    if (!losses) now.rows = nullptr;
+    hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, stream, now);
     return launched("sums_kernel");
   };
   const bool early = backward && (per_token || !forward || n > h->piece);
@@ -634,12 +662,15 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
         t.lse = io->lse;
         t.loss = c.row_loss;
         t.e = c.e;
-        if (backward) hipLaunchKernelGGL((token_kernel<T, true>), dim3(now), dim3(256), 0, stream, p, t);
+        const unsigned slices = (unsigned)std::max(1, std::min(4 * kUnits / now, p.tiles * kTile / 4096));
+        if (backward) hipLaunchKernelGGL((token_kernel<T, true>), dim3(now, slices), dim3(256), 0, stream, p, t);
         else hipLaunchKernelGGL((token_kernel<T, false>), dim3(now), dim3(256), 0, stream, p, t);
         if ((rc = launched("token_kernel"))) return rc;
       }
     }
-    if (last && forward && !per_token && (rc = sums(true))) return rc;
+    const bool behind = last && forward && !per_token;  // the sums come now
+    const DxPlan plan = backward && now > 0 ? dx_plan(p, now, d.hidden) : DxPlan{};
+    if (behind && plan.parts <= 1 && (rc = sums(true))) return rc;
     if (!backward) continue;
     GradArgs g = {};
     g.g = c.e;
@@ -656,27 +687,24 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
     g.first = at == 0;
     g.last = last;
     if (now > 0) {
-      const DxPlan plan = dx_plan(p, now, d.hidden);
       g.token_tiles = plan.token_tiles;
       g.hidden_tiles = plan.hidden_tiles;
       g.split_steps = plan.split_steps;
       g.parts = plan.parts > 1 ? c.parts : nullptr;
+      g.count = plan.parts;
+      g.with_sums = g.parts && behind;
       auto go = [&](auto s) {
         typedef decltype(s) S;
-        hipLaunchKernelGGL((dx_kernel<T, S>), dim3((unsigned)(g.token_tiles * g.hidden_tiles), plan.parts), dim3(S::kThreads), 0, stream, p, g);
+        hipLaunchKernelGGL((dx_kernel<T, S>), dim3((unsigned)(g.token_tiles * g.hidden_tiles + g.with_sums), plan.parts), dim3(S::kThreads), 0, stream, p, g, totals);
         return launched("dx_kernel");
       };
       if ((rc = plan.shape == kLarge ? go(Large()) : plan.shape == kMiddle ? go(Middle()) : go(Few()))) return rc;
-      if (g.parts) {
-        hipLaunchKernelGGL((add_parts_kernel<T>), dim3((unsigned)(((int64_t)now * d.hidden + 1023) / 1024)), dim3(256), 0, stream, c.parts, plan.parts, now, d.hidden, g.dx,
-                           g.dx_stride, c.back);
-        if ((rc = launched("add_parts_kernel"))) return rc;
-      }
     }
     auto go = [&](auto s) {
       typedef decltype(s) S;
       g.hidden_tiles = tiles(d.hidden, S::kL);
-      hipLaunchKernelGGL((dw_kernel<T, S>), dim3((unsigned)(p.tiles * (kTile / S::kR) * g.hidden_tiles)), dim3(S::kThreads), 0, stream, p, c.grads, g);
+      g.adders = g.parts ? (int)std::min<int64_t>(2 * kUnits, ((int64_t)now * d.hidden / 4 + S::kThreads - 1) / S::kThreads) : 0;
+      hipLaunchKernelGGL((dw_kernel<T, S>), dim3((unsigned)(g.adders + p.tiles * (kTile / S::kR) * g.hidden_tiles)), dim3(S::kThreads), 0, stream, p, c.grads, g);
       return launched("dw_kernel");
     };
     if ((rc = dw_shape(p, now, d.hidden) == kLarge ? go(Large()) : go(Middle()))) return rc;

@@ -87,12 +87,12 @@ class VocabLossDesc(ctypes.Structure):
                 ("gradients", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
-class VocabLossIO(ctypes.Structure):
+class VocabLossIO(ctypes.Structure):  # weights, dweights: addresses of arrays of pointers
     _fields_ = [("tokens", ctypes.c_int64), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
-                ("weights", ctypes.POINTER(ctypes.c_void_p)), ("weight_stride", ctypes.c_int64),
+                ("weights", ctypes.c_void_p), ("weight_stride", ctypes.c_int64),
                 ("labels", ctypes.c_void_p), ("label_bytes", ctypes.c_int32), ("reserved", ctypes.c_int32),
                 ("loss", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("grad_loss", ctypes.c_void_p),
-                ("dx", ctypes.c_void_p), ("dx_stride", ctypes.c_int64), ("dweights", ctypes.POINTER(ctypes.c_void_p)), ("dweight_stride", ctypes.c_int64),
+                ("dx", ctypes.c_void_p), ("dx_stride", ctypes.c_int64), ("dweights", ctypes.c_void_p), ("dweight_stride", ctypes.c_int64),
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 

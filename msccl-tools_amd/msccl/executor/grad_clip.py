@@ -64,6 +64,8 @@ class GradientClip:
         if not torch.cuda.is_available():
             raise RuntimeError("gradient clipping needs a GPU; there is no CPU path")
         self._workspace = torch.zeros(self.workspace_bytes, dtype=torch.uint8, device=self.device)
+        self.device = self._workspace.device   # with its index
+        self._home = torch.cuda.current_stream(self.device).cuda_stream
         results = self._workspace[:8].view(torch.float32)
         self.norm, self.coefficient = results[0], results[1]   # of the last launch
 
@@ -77,8 +79,16 @@ class GradientClip:
                 raise ValueError(f"{what} {i} must have {n} elements of {name}, has {t.numel()} of {t.dtype}")
         return (ctypes.c_void_p * max(1, len(tensors)))(*[t.data_ptr() or None for t in tensors])
 
-    def _stream(self):
-        return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream or None)
+    def _call(self, entry, *args):
+        stream = torch.cuda.current_stream(self.device)
+        if stream.cuda_stream != self._home:   # the workspace is not given to others before this stream is done with it
+            self._workspace.record_stream(stream)
+        handle = ctypes.c_void_p(stream.cuda_stream or None)
+        if torch.cuda.current_device() == self.device.index:
+            binding._check(self.lib, entry(self.handle, *args, handle))
+        else:
+            with torch.cuda.device(self.device):
+                binding._check(self.lib, entry(self.handle, *args, handle))
 
     def bind(self, inputs, outputs=None):
         """Attach gradients, and the tensors that launch() clips into (None: the norm only; the inputs themselves: in place)."""
@@ -89,9 +99,7 @@ class GradientClip:
         ins = self._pointers("input", inputs, self.dtypes)
         outs = None if outputs is None else self._pointers("output", outputs, self.out_dtypes)
         self._keepalive = None
-        with torch.cuda.device(self.device):
-            binding._check(self.lib, self.lib.mscclx_grad_clip_bind(self.handle, ins, outs, ctypes.c_void_p(self._workspace.data_ptr()),
-                                                                    self.workspace_bytes, self._stream()))
+        self._call(self.lib.mscclx_grad_clip_bind, ins, outs, ctypes.c_void_p(self._workspace.data_ptr()), self.workspace_bytes)
         self._keepalive = (inputs, outputs)
         self._has_outputs = outputs is not None
 
@@ -104,8 +112,7 @@ class GradientClip:
             raise ValueError("max_norm must not be negative")
         if max_norm is not None and not self._has_outputs:
             raise RuntimeError("bind() was called without outputs")
-        with torch.cuda.device(self.device):
-            binding._check(self.lib, self.lib.mscclx_grad_clip_launch(self.handle, scale, -1.0 if max_norm is None else max_norm, self._stream()))
+        self._call(self.lib.mscclx_grad_clip_launch, scale, -1.0 if max_norm is None else max_norm)
 
     def run(self, inputs, outputs=None, max_norm=None, scale=1.0):
         """bind() and launch(); returns the norm as a tensor of its own."""

@@ -55,33 +55,47 @@ class VocabLoss:
         self.tokens, self.hidden, self.rank_rows, self.reduction = int(tokens), int(hidden), rows, reduction
         self.dtype = {"bfloat16": torch.bfloat16, "float16": torch.float16}[name]
         self.gradients, self.workspace_bytes, self.piece_tokens = bool(gradients), nbytes.value, piece.value
+        self._shapes = [torch.Size((r, self.hidden)) for r in rows]
         if not torch.cuda.is_available():
             raise RuntimeError("the vocabulary loss needs a GPU; there is no CPU path")
         self._workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=self.device)
+        self.device = self._workspace.device   # with its index
+        self._home = torch.cuda.current_stream(self.device).cuda_stream
+        # What the library reads of a call, filled in anew by each: a handle serves one thread at a time
+        io = self._io = VocabLossIO()
+        self._weights, self._dweights = ((ctypes.c_void_p * len(rows))() for _ in range(2))
+        io.weights, io.dweights = ctypes.addressof(self._weights), ctypes.addressof(self._dweights)
+        io.workspace, io.workspace_bytes = self._workspace.data_ptr(), self.workspace_bytes
 
-    def _matrix(self, what, t, rows):
-        if not isinstance(t, torch.Tensor) or t.device != self._workspace.device or t.dtype != self.dtype:
-            raise ValueError(f"{what} must be a {self.dtype} tensor on {self._workspace.device}")
-        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != self.hidden or t.stride(1) != 1:
-            raise ValueError(f"{what} must be [{rows}, {self.hidden}] with contiguous rows")
-        return self.hidden if rows < 2 else t.stride(0)   # the stride of a single row says nothing
+    # The checks are a few comparisons for each tensor: a call on a small problem is bound by the host.
+    def _matrix(self, what, t, shape):
+        """The row stride of a [rows, hidden] matrix."""
+        if type(t) is not torch.Tensor and not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what} must be a tensor")
+        if t.dtype is not self.dtype or t.device != self.device:
+            raise ValueError(f"{what} must be a {self.dtype} tensor on {self.device}")
+        if t.shape != shape or t.stride(1) != 1:
+            raise ValueError(f"{what} must be {list(shape)} with contiguous rows")
+        return t.stride(0) if shape[0] > 1 else self.hidden   # the stride of a single row says nothing
 
-    def _matrices(self, what, given):
-        if len(given) != len(self.rank_rows):
-            raise ValueError(f"{what}: {len(given)} for {len(self.rank_rows)} ranks")
-        strides = {self._matrix(f"{what} of rank {r}", t, n) for r, (t, n) in enumerate(zip(given, self.rank_rows)) if n > 1}
-        for r, (t, n) in enumerate(zip(given, self.rank_rows)):
-            if n == 1:
-                self._matrix(f"{what} of rank {r}", t, n)
-        if len(strides) > 1:
-            raise ValueError(f"{what}: all ranks' rows must be the same stride apart")
-        return (ctypes.c_void_p * len(given))(*[t.data_ptr() if n else None for t, n in zip(given, self.rank_rows)]), strides.pop() if strides else self.hidden
+    def _matrices(self, what, given, pointers):
+        if len(given) != len(self._shapes):
+            raise ValueError(f"{what}: {len(given)} for {len(self._shapes)} ranks")
+        common = None
+        for r, (t, shape) in enumerate(zip(given, self._shapes)):
+            stride = self._matrix(what, t, shape)
+            if shape[0] > 1:
+                if common is not None and stride != common:
+                    raise ValueError(f"{what}: all ranks' rows must be the same stride apart")
+                common = stride
+            pointers[r] = t.data_ptr()
+        return self.hidden if common is None else common
 
-    def _vector(self, what, t, n, dtypes=(torch.float32,)):
-        if not isinstance(t, torch.Tensor) or t.device != self._workspace.device or t.dtype not in dtypes:
-            raise ValueError(f"{what} must be a tensor of {' or '.join(map(str, dtypes))} on {self._workspace.device}")
-        if tuple(t.shape) != n or (t.dim() and t.numel() > 1 and t.stride(0) != 1):
-            raise ValueError(f"{what} must be contiguous of shape {n}")
+    def _vector(self, what, t, shape, dtypes=(torch.float32,)):
+        if not isinstance(t, torch.Tensor) or t.device != self.device or t.dtype not in dtypes:
+            raise ValueError(f"{what} must be a tensor of {' or '.join(map(str, dtypes))} on {self.device}")
+        if t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous of shape {shape}")
         return t.data_ptr()
 
     def _tokens(self, x):
@@ -93,20 +107,24 @@ class VocabLoss:
             raise ValueError(f"{x.shape[0]} tokens given, setup() was called for at most {self.tokens}")
         return x.shape[0]
 
-    def _io(self, x, weights, labels, lse):
-        n = self._tokens(x)
-        io = VocabLossIO()
-        io.tokens, io.x, io.x_stride = n, x.data_ptr(), self._matrix("x", x, n)
-        ptrs, io.weight_stride = self._matrices("weights", weights)
-        io.weights = ctypes.cast(ptrs, ctypes.POINTER(ctypes.c_void_p))
+    def _inputs(self, n, x, weights, labels, lse):
+        io = self._io
+        io.tokens, io.x, io.x_stride = n, x.data_ptr(), self._matrix("x", x, (n, self.hidden))
+        io.weight_stride = self._matrices("weights", weights, self._weights)
         io.labels, io.label_bytes = self._vector("labels", labels, (n,), (torch.int64, torch.int32)), labels.element_size()
-        io.lse = self._vector("lse", lse, (n,))
-        io.workspace, io.workspace_bytes = self._workspace.data_ptr(), self.workspace_bytes
-        return io, [ptrs]
+        io.lse = lse.data_ptr()
+        return io
 
     def _call(self, entry, io):
-        with torch.cuda.device(self.device):
-            binding._check(self.lib, entry(self.handle, ctypes.byref(io), ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream or None)))
+        stream = torch.cuda.current_stream(self.device)
+        if stream.cuda_stream != self._home:   # the workspace is not given to others before this stream is done with it
+            self._workspace.record_stream(stream)
+        handle = ctypes.c_void_p(stream.cuda_stream or None)
+        if torch.cuda.current_device() == self.device.index:
+            binding._check(self.lib, entry(self.handle, ctypes.byref(io), handle))
+        else:
+            with torch.cuda.device(self.device):
+                binding._check(self.lib, entry(self.handle, ctypes.byref(io), handle))
 
     def _shape(self, n):
         return (n,) if self.reduction == "none" else ()
@@ -114,25 +132,31 @@ class VocabLoss:
     def _new(self, shape, dtype=torch.float32):
         return torch.empty(shape, dtype=dtype, device=self.device)
 
-    def _gradients(self, io, keep, n, grad_loss, dx, dweights):
+    def _gradients(self, io, n, grad_loss, dx, dweights):
         if not self.gradients:
             raise RuntimeError("setup() was called with gradients=False")
-        if grad_loss is None:
+        if grad_loss is None:   # (given back to the allocator at the end of the call, in the order of this stream)
             grad_loss = torch.ones(self._shape(n), dtype=torch.float32, device=self.device)
-        dx = self._new((n, self.hidden), self.dtype) if dx is None else dx
-        dweights = [self._new((r, self.hidden), self.dtype) for r in self.rank_rows] if dweights is None else list(dweights)
         io.grad_loss = self._vector("grad_loss", grad_loss, self._shape(n))
-        io.dx, io.dx_stride = dx.data_ptr(), self._matrix("dx", dx, n)
-        ptrs, io.dweight_stride = self._matrices("dweights", dweights)
-        io.dweights = ctypes.cast(ptrs, ctypes.POINTER(ctypes.c_void_p))
-        keep += [ptrs, grad_loss]
+        if dx is None:
+            dx = self._new((n, self.hidden), self.dtype)
+            io.dx, io.dx_stride = dx.data_ptr(), self.hidden
+        else:
+            io.dx, io.dx_stride = dx.data_ptr(), self._matrix("dx", dx, (n, self.hidden))
+        if dweights is None:   # one allocation, a rank's rows behind the other's
+            dweights = list(self._new((sum(self.rank_rows), self.hidden), self.dtype).split(self.rank_rows))
+            self._dweights[:] = [t.data_ptr() for t in dweights]
+            io.dweight_stride = self.hidden
+        else:
+            dweights = list(dweights)
+            io.dweight_stride = self._matrices("dweights", dweights, self._dweights)
         return dx, dweights
 
     def forward(self, x, weights, labels):
         """(loss, lse): loss is one float32 number, or one per token with reduction="none"; lse one per token."""
-        lse = self._new(self._tokens(x))
-        io, keep = self._io(x, weights, labels, lse)
-        loss = self._new(self._shape(x.shape[0]))
+        n = self._tokens(x)
+        loss, lse = self._new(self._shape(n)), self._new(n)
+        io = self._inputs(n, x, weights, labels, lse)
         io.loss = loss.data_ptr()
         self._call(self.lib.mscclx_vocab_loss_forward, io)
         return loss, lse
@@ -140,17 +164,19 @@ class VocabLoss:
     def backward(self, x, weights, labels, lse, grad_loss=None, dx=None, dweights=None):
         """(dx, [dw of each rank]) from the lse of forward(); grad_loss: float32, one number or one per token (default 1).
         Computes the probabilities again; run() does not."""
-        io, keep = self._io(x, weights, labels, lse)
-        out = self._gradients(io, keep, x.shape[0], grad_loss, dx, dweights)
+        n = self._tokens(x)
+        self._vector("lse", lse, (n,))
+        io = self._inputs(n, x, weights, labels, lse)
+        out = self._gradients(io, n, grad_loss, dx, dweights)
         self._call(self.lib.mscclx_vocab_loss_backward, io)
         return out
 
     def run(self, x, weights, labels, grad_loss=None, dx=None, dweights=None):
         """(loss, lse, dx, [dw of each rank]) in one call."""
-        lse = self._new(self._tokens(x))
-        io, keep = self._io(x, weights, labels, lse)
-        loss = self._new(self._shape(x.shape[0]))
+        n = self._tokens(x)
+        loss, lse = self._new(self._shape(n)), self._new(n)
+        io = self._inputs(n, x, weights, labels, lse)
         io.loss = loss.data_ptr()
-        dx, dweights = self._gradients(io, keep, x.shape[0], grad_loss, dx, dweights)
+        dx, dweights = self._gradients(io, n, grad_loss, dx, dweights)
         self._call(self.lib.mscclx_vocab_loss_run, io)
         return loss, lse, dx, dweights

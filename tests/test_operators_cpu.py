@@ -46,8 +46,8 @@ def loss_io(nbytes, ranks=2, **changed):
     at = 1 << 20  # addresses that nothing dereferences: every call below is refused before a launch
     io = VocabLossIO()
     ptrs = (ctypes.c_void_p * ranks)(*[at] * ranks)
-    values = dict(tokens=100, x=at, x_stride=64, weights=ctypes.cast(ptrs, ctypes.POINTER(ctypes.c_void_p)), weight_stride=64, labels=at, label_bytes=8, loss=at,
-                  lse=at, grad_loss=at, dx=at, dx_stride=64, dweights=ctypes.cast(ptrs, ctypes.POINTER(ctypes.c_void_p)), dweight_stride=64, workspace=at,
+    values = dict(tokens=100, x=at, x_stride=64, weights=ctypes.addressof(ptrs), weight_stride=64, labels=at, label_bytes=8, loss=at,
+                  lse=at, grad_loss=at, dx=at, dx_stride=64, dweights=ctypes.addressof(ptrs), dweight_stride=64, workspace=at,
                   workspace_bytes=nbytes)
     for k, v in {**values, **changed}.items():
         setattr(io, k, v)
@@ -61,11 +61,11 @@ def test_vocab_loss_calls_refuse(mscclx_lib, entry):
     call = getattr(mscclx_lib, f"mscclx_vocab_loss_{entry}")
     null = (ctypes.c_void_p * 2)(None, 1 << 20)
     odd = (ctypes.c_void_p * 2)((1 << 20) + 8, 1 << 20)
-    as_ptr = lambda a: ctypes.cast(a, ctypes.POINTER(ctypes.c_void_p))  # noqa: E731
+    as_ptr = ctypes.addressof
     bad = [(dict(tokens=101), CAPACITY), (dict(tokens=-1), CAPACITY), (dict(workspace_bytes=nbytes - 1), CAPACITY), (dict(workspace=0), INVALID),
            (dict(workspace=(1 << 20) + 128), INVALID), (dict(x=0), INVALID), (dict(x=(1 << 20) + 2), INVALID), (dict(x_stride=63), INVALID), (dict(x_stride=60), INVALID),
            (dict(x_stride=68), INVALID), (dict(x_stride=1 << 23), INVALID), (dict(weights=as_ptr(null)), INVALID), (dict(weights=as_ptr(odd)), INVALID),
-           (dict(weights=ctypes.POINTER(ctypes.c_void_p)()), INVALID), (dict(weight_stride=32), INVALID), (dict(labels=0), INVALID),
+           (dict(weights=None), INVALID), (dict(weight_stride=32), INVALID), (dict(labels=0), INVALID),
            (dict(labels=(1 << 20) + 4), INVALID), (dict(label_bytes=2), INVALID), (dict(lse=0), INVALID), (dict(lse=(1 << 20) + 2), INVALID)]
     if entry != "backward":
         bad += [(dict(loss=0), INVALID), (dict(loss=(1 << 20) + 1), INVALID)]
