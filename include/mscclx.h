@@ -250,7 +250,7 @@ typedef enum { MSCCLX_LOSS_NONE = 0, MSCCLX_LOSS_SUM = 1, MSCCLX_LOSS_MEAN = 2 }
 typedef struct {
   int32_t ranks;
   int32_t hidden;           /* a multiple of 8                                                                */
-  const int64_t* rank_rows; /* rows of each rank's piece, 0 allowed; read by create only                      */
+  const int64_t* rank_rows; /* rows of each rank's piece, 0 allowed, less than 2^22 in all; read by create only */
   int64_t max_tokens;
   int32_t dtype;            /* MSCCLX_BF16 or MSCCLX_F16: x, weights and gradients                            */
   int32_t reduction;        /* mscclx_loss_reduction                                                          */

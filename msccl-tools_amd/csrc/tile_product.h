@@ -36,6 +36,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 constexpr int kStepK = 64;                      // values of k per step
 constexpr unsigned kOutside = 0x80000000u;      // a byte offset that no operand holds
 constexpr int kResourceBytes = 0x7ffffff0;      // range of the buffer resources: every valid offset is below, kOutside is not
+constexpr int kUnitRows = 64;                   // rows that have one base address, where a row operand's rows have several
 
 template <class T> struct Half;
 template <> struct Half<__bf16> {
@@ -59,9 +60,9 @@ template <> struct Half<_Float16> {
   }
 };
 
-// 16 bytes per lane from `resource` at `offset` (per lane) to LDS at m0 + 16 * lane.  Nothing else in these kernels uses m0.
-__device__ __forceinline__ void copy_to_lds(unsigned lds, unsigned offset, i32x4 resource) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(resource) : "memory");
+// 16 bytes per lane from `resource` at `offset` (per lane) + `further` to LDS at m0 + 16 * lane.  Nothing else in these kernels uses m0.
+__device__ __forceinline__ void copy_to_lds(unsigned lds, unsigned offset, i32x4 resource, int further) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(resource), "s"(further) : "memory");
 }
 __device__ __forceinline__ i32x4 resource_at(const char* p) {
   const uint64_t a = (uint64_t)p;
@@ -78,48 +79,56 @@ struct Lanes {
   static constexpr int kChunks = kBytes / kChunk;
   static constexpr int kUnitsPerLine = COL ? TILE / 8 : 8;       // 16-byte units of a line of LDS
   static constexpr int kLines = WAVES * 64 / kUnitsPerLine;      // lines per chunk
-  static_assert(kChunks >= 1 && (COL ? TILE >= 128 : kLines % 16 == 0), "a copy covers whole swizzle patterns");
+  static_assert(kChunks >= 1 && (COL ? TILE >= 128 : kLines % 16 == 0 && kUnitRows % kLines == 0), "a copy covers whole swizzle patterns");
   unsigned offset[kChunks];
   int k[COL ? kChunks : 1];                                      // the lane's k (its first) in the step
 
-  // `stride`: bytes between rows of memory; `valid`: rows (row) or columns (col) that exist
-  __device__ __forceinline__ void place(int thread, int64_t stride, int valid) {
+  // `stride`: bytes between rows of memory; `valid(unit)`: rows of the unit (row, counted from its base) or columns (col) that exist
+  template <class F> __device__ __forceinline__ void place(int thread, int64_t stride, F valid) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int line = i * kLines + thread / kUnitsPerLine, unit = thread % kUnitsPerLine;
+      int line = i * kLines + thread / kUnitsPerLine;
+      const int unit = thread % kUnitsPerLine;
       if constexpr (COL) {
         const int from = (((unit >> 1) ^ swizzle_of<SIDE>(line)) << 1) | (unit & 1);
-        offset[i] = from * 8 < valid ? (unsigned)(line * stride) + from * 16 : kOutside;
+        offset[i] = from * 8 < valid(0) ? (unsigned)(line * stride) + from * 16 : kOutside;
         k[i] = line;
       } else {
         const int from = unit ^ (line >> 1 & 7);
-        offset[i] = line < valid ? (unsigned)(line * stride) + from * 16 : kOutside;
         if (i == 0) k[0] = from * 8;   // a chunk is a multiple of 16 lines: the same for all
+        line %= kUnitRows;
+        offset[i] = line < valid(i * kLines / kUnitRows) ? (unsigned)(line * stride) + from * 16 : kOutside;
       }
     }
   }
   // copy `i` of a step that has `k_left` values of k
-  __device__ __forceinline__ void copy(int i, unsigned lds, i32x4 from, int k_left) const {
-    copy_to_lds(lds + i * kChunk, k[COL ? i : 0] < k_left ? offset[i] : kOutside, from);
+  __device__ __forceinline__ void copy(int i, unsigned lds, i32x4 from, int further, int k_left) const {
+    copy_to_lds(lds + i * kChunk, k[COL ? i : 0] < k_left ? offset[i] : kOutside, from, further);
   }
 };
 
-// Where an operand's steps begin.  k_left: values of k from there on.
-struct RowSource {  // k contiguous
-  const char* base;
-  int64_t k;
-  __device__ __forceinline__ const char* step(int s, int* k_left) {
-    *k_left = (int)min((int64_t)kStepK, k - (int64_t)s * kStepK);
-    return base + (int64_t)s * (kStepK * 2);
+// Where an operand's copies read: `base(i)`, the resource of the rows of unit i (row) or of all (col), for step after step `next()`; then
+// `further` is what they add to it, and `left` the values of k from the step's first on.  Behind the last step nothing is left.
+template <int TILE> struct RowSource {  // k contiguous
+  static constexpr int kUnits = (TILE + kUnitRows - 1) / kUnitRows;
+  i32x4 bases[kUnits];
+  int further = -2 * kStepK, left;
+  // at(i): the address of unit i's first row
+  template <class F> __device__ __forceinline__ RowSource(F at, int k) : left(k + kStepK) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) bases[i] = resource_at(at(i));
   }
+  __device__ __forceinline__ void next() { further += 2 * kStepK, left -= kStepK; }
+  __device__ __forceinline__ i32x4 base(int i) const { return bases[i]; }
 };
 struct ColSource {  // k strided
-  const char* base;
-  int64_t k, stride;
-  __device__ __forceinline__ const char* step(int s, int* k_left) {
-    *k_left = (int)min((int64_t)kStepK, k - (int64_t)s * kStepK);
-    return base + (int64_t)s * kStepK * stride;
-  }
+  static constexpr int further = 0;
+  const char* at;
+  int64_t stride;
+  int left;
+  __device__ __forceinline__ ColSource(const char* at, int k, int64_t stride) : at(at - kStepK * stride), stride(stride), left(k + kStepK) {}
+  __device__ __forceinline__ void next() { at += kStepK * stride, left -= kStepK; }
+  __device__ __forceinline__ i32x4 base(int) const { return resource_at(at); }
 };
 
 // TL x TR: the workgroup's tile, cut among WL x WR waves; SIDE: of the matrix instruction, 16 or 32; STAGES: steps held in LDS, a power of two.
@@ -172,21 +181,10 @@ struct TileProduct {
     const int l0 = wave % WL * (TL / WL), r0 = wave / WL * (TR / WR);
     typedef __attribute__((address_space(3))) char* lds_char;
     const unsigned lds = (unsigned)(uintptr_t)(lds_char)smem + wave * 1024;
-    struct Step {  // what the copies of a step read
-      unsigned lds;
-      i32x4 l, r;
-      int l_left, r_left;
-    };
-    auto step = [&](int s) {  // in order; behind the last step nothing is left and the copies write zeros
-      Step t;
-      t.lds = lds + s % STAGES * kStage;
-      t.l = resource_at(sl.step(s, &t.l_left));
-      t.r = resource_at(sr.step(s, &t.r_left));
-      return t;
-    };
-    auto copy = [&](const Step& t, int i) {
-      if (i < LLanes::kChunks) ll.copy(i, t.lds, t.l, t.l_left);
-      else rl.copy(i - LLanes::kChunks, t.lds + LLanes::kBytes, t.r, t.r_left);
+    auto copy = [&](int s, int i) {
+      const unsigned at = lds + s % STAGES * kStage;
+      if (i < LLanes::kChunks) ll.copy(i, at, sl.base(LCOL ? 0 : i * LLanes::kLines / kUnitRows), sl.further, sl.left);
+      else i -= LLanes::kChunks, rl.copy(i, at + LLanes::kBytes, sr.base(RCOL ? 0 : i * RLanes::kLines / kUnitRows), sr.further, sr.left);
     };
     struct Fragments {  // of half a step
       i16x8 a[kSlices][FL], b[kSlices][FR];
@@ -208,9 +206,9 @@ struct TileProduct {
     Fragments now, next;
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) {
-      const Step t = step(s);
+      sl.next(), sr.next();
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i) copy(t, i);
+      for (int i = 0; i < kCopies; ++i) copy(s, i);
     }
     // copies arrive in order: the awaited step's are there once only those of the steps behind it are under way
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * kCopies) : "memory");
@@ -226,11 +224,11 @@ struct TileProduct {
       }
       // the copies of the next step have arrived, and every wave has read all of this one: its buffer takes the step STAGES further
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * kCopies) : "memory");
-      const Step t = step(s + STAGES);
+      sl.next(), sr.next();
 #pragma unroll
       for (int l = 0; l < FL; ++l) {
 #pragma unroll
-        for (int i = l * kCopies / FL; i < (l + 1) * kCopies / FL; ++i) copy(t, i);
+        for (int i = l * kCopies / FL; i < (l + 1) * kCopies / FL; ++i) copy(s + STAGES, i);
 #pragma unroll
         for (int u = l * kUnits / FL; u < (l + 1) * kUnits / FL; ++u) read(now, s + 1, 0, u);  // (behind the last step: for nothing)
         multiply(next, l);

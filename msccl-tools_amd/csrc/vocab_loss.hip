@@ -30,22 +30,30 @@ namespace mscclx {
 namespace {
 
 constexpr int kMaxRanks = MSCCLX_VOCAB_LOSS_MAX_RANKS;
-constexpr int kTile = 256;              // rows of the vocabulary: a rank's piece is padded to whole tiles of G
+constexpr int kTile = 256;              // columns of G are padded to a multiple of it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// The ranks' pieces of the vocabulary, passed to the kernels by value.  Tiles of kTile rows; none spans two ranks.
+// The ranks' pieces of the vocabulary, passed to the kernels by value.  Units of kUnitRows rows; none spans two ranks, a tile may.
+// What pads a rank's last unit, or the last tile, counts as outside.
 struct Pieces {
   int ranks, tiles;
   int rows[kMaxRanks];
-  int tile0[kMaxRanks + 1];  // the rank's first tile
+  int unit0[kMaxRanks + 1];  // the rank's first unit
   int first[kMaxRanks];      // the rank's first row in the whole vocabulary
   const char* w[kMaxRanks];
-  __device__ __forceinline__ int rank_of(int tile) const {
-    int r = 0;
-    while (r + 1 < ranks && tile >= tile0[r + 1]) ++r;
-    return r;
+};
+
+// Unit `unit` of the padded vocabulary
+struct Unit {
+  int rank, row;  // its rank, and its first row there
+  int rows;       // from that row on; may be none, or less
+  __device__ __forceinline__ Unit(const Pieces& p, int unit) : rank(0) {
+    while (rank + 1 < p.ranks && unit >= p.unit0[rank + 1]) ++rank;
+    row = (unit - p.unit0[rank]) * kUnitRows;
+    rows = p.rows[rank] - row;
   }
 };
+
 struct Grads {
   char* dw[kMaxRanks];
 };
@@ -120,64 +128,82 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
   int tt, at;
   tile_of(blockIdx.x, a.token_tiles, pieces.tiles * (kTile / TL), &tt, &at);
-  const int vt = at / (kTile / TL), rank = pieces.rank_of(vt), row0 = at * TL - pieces.tile0[rank] * kTile;
-  const int rows = min(TL, pieces.rows[rank] - row0);  // none or less: the tile is padding
   const int n0 = tt * TR, tokens = min(TR, a.tokens - n0);
   typename Product::Acc acc[Product::FL][Product::FR] = {};
-  if (rows > 0) {
+  {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
-    ll.place(threadIdx.x, a.w_stride, rows);
-    rl.place(threadIdx.x, a.x_stride, tokens);
-    Product::run(smem, (a.hidden + kStepK - 1) / kStepK, ll, RowSource{pieces.w[rank] + row0 * a.w_stride, a.hidden}, rl,
-                 RowSource{a.x + n0 * a.x_stride, a.hidden}, acc);
+    ll.place(threadIdx.x, a.w_stride, [&](int i) { return Unit(pieces, at * (TL / kUnitRows) + i).rows; });
+    rl.place(threadIdx.x, a.x_stride, [&](int i) { return tokens - i * kUnitRows; });
+    Product::run(smem, (a.hidden + kStepK - 1) / kStepK, ll,
+                 RowSource<TL>([&](int i) {
+                   const Unit u(pieces, at * (TL / kUnitRows) + i);
+                   return pieces.w[u.rank] + u.row * a.w_stride;
+                 }, a.hidden),
+                 rl, RowSource<TR>([&](int i) { return a.x + (n0 + i * kUnitRows) * a.x_stride; }, a.hidden), acc);
   }
   const int64_t ld = (int64_t)pieces.tiles * kTile;
   const int lane = threadIdx.x & 63, part = (threadIdx.x >> 6) % Shape::kWavesL;
-  auto finish = [&](auto whole) {  // whole: no row of the tile is padding
+  // the wave's part of the vocabulary: whole units, or part of one
+  constexpr int kOfWave = kPart < kUnitRows ? kPart : kUnitRows, kWaveUnits = kPart / kOfWave, kUnitFragments = kOfWave / Shape::kSide;
+  int rows[kWaveUnits], first[kWaveUnits];  // of each: rows that exist, and the first one's number in the whole vocabulary
+  bool all = true;
+#pragma unroll
+  for (int j = 0; j < kWaveUnits; ++j) {
+    const int from = __builtin_amdgcn_readfirstlane(at * TL + part * kPart + j * kOfWave);
+    const Unit u(pieces, from / kUnitRows);
+    rows[j] = u.rows - from % kUnitRows;
+    first[j] = pieces.first[u.rank] + u.row + from % kUnitRows;
+    all &= rows[j] >= kOfWave;
+  }
+  auto finish = [&](auto whole) {  // whole: none of the wave's rows is padding
     constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
     for (int r = 0; r < Product::FR; ++r) {
       const int n = Product::r_of(threadIdx.x, r);
       const bool live = n < tokens;
       const int label = live ? a.labels.get(a.token0 + n0 + n) : -1;
-      const int want = label >= 0 ? label - pieces.first[rank] - row0 : -1;  // the label's row in the tile
-      const bool here = want >= part * kPart && want < min(rows, (part + 1) * kPart);
-      const bool any = __any(here);                                           // one wave in hundreds holds a label of its tokens
+      bool here = false;
+#pragma unroll
+      for (int j = 0; j < kWaveUnits; ++j) here |= label >= first[j] && label < first[j] + min(rows[j], kOfWave);
+      const bool any = __any(here);  // one wave in hundreds holds a label of its tokens
       T* out = (T*)a.e + (n0 + n) * ld + (int64_t)at * TL;
-      // the wave's logits of the token, in fours
+      // the wave's logits of the token, in fours: f(place in the tile, row in the unit, the unit's rows, the label's row in it, logits)
       auto each = [&](auto f) {
 #pragma unroll
         for (int l = 0; l < Product::FL; ++l)
 #pragma unroll
-          for (int q = 0; q < Product::kQuads; ++q) f(Product::l_of(threadIdx.x, l, q), Product::quad(acc[l][r], q));
+          for (int q = 0; q < Product::kQuads; ++q) {
+            const int v = Product::l_of(threadIdx.x, l, q), j = l / kUnitFragments;
+            f(v, v - part * kPart - j * kOfWave, rows[j], label - first[j], Product::quad(acc[l][r], q));
+          }
       };
       if constexpr (MODE == kGradient) {
         const float lse = live ? a.lse[a.token0 + n0 + n] * kLog2e : 0.f, g = live ? a.upstream.get(a.token0 + n0 + n, label) * kUnit<T> : 0.f;
-        each([&](int v, f32x4 z) {
+        each([&](int v, int row, int rows, int want, f32x4 z) {
           typename Half<T>::x4 o;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float p = exp2_of(__builtin_fmaf(z[i], kLog2e, -lse));
-            if (any) p -= v + i == want ? 1.f : 0.f;
-            o[i] = (T)((WHOLE || v + i < rows) && g != 0.f ? p * g : 0.f);
+            if (any) p -= here && row + i == want ? 1.f : 0.f;
+            o[i] = (T)((WHOLE || row + i < rows) && g != 0.f ? p * g : 0.f);
           }
           if (live) *(typename Half<T>::x4*)(out + v) = o;
         });
       } else {
         float m = -INFINITY;
-        each([&](int v, f32x4 z) {
+        each([&](int, int row, int rows, int, f32x4 z) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (WHOLE || v + i < rows) m = fmaxf(m, z[i]);
+            if (WHOLE || row + i < rows) m = fmaxf(m, z[i]);
         });
         if (any) {
           float z_label = 0.f;
           bool found = false;
-          each([&](int v, f32x4 z) {
+          each([&](int, int row, int rows, int want, f32x4 z) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (v + i == want && v + i < rows) z_label = z[i], found = true;
+              if (here && row + i == want && row + i < rows) z_label = z[i], found = true;
           });
           if (found) a.z_label[a.token0 + n0 + n] = z_label;
         }
@@ -186,11 +212,11 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces
         m *= kLog2e;
         const float base = m == -INFINITY ? 0.f : m;  // a part of nothing but -inf has sum 0
         float sum = 0.f;
-        each([&](int v, f32x4 z) {
+        each([&](int v, int row, int rows, int, f32x4 z) {
           typename Half<T>::x4 o;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float e = WHOLE || v + i < rows ? exp2_of(__builtin_fmaf(z[i], kLog2e, -base)) : 0.f;
+            const float e = WHOLE || row + i < rows ? exp2_of(__builtin_fmaf(z[i], kLog2e, -base)) : 0.f;
             sum += e;
             o[i] = (T)(e * kUnit<T>);
           }
@@ -202,7 +228,7 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces
       }
     }
   };
-  if (rows >= TL) finish(std::true_type());
+  if (all) finish(std::true_type());
   else finish(std::false_type());
 }
 
@@ -257,7 +283,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
     if (label >= 0) {
       int r = 0;
       while (r + 1 < pieces.ranks && label >= pieces.first[r + 1]) ++r;
-      want = (int64_t)pieces.tile0[r] * kTile + label - pieces.first[r];
+      want = (int64_t)pieces.unit0[r] * kUnitRows + label - pieces.first[r];
     }
     typedef typename Half<T>::x8 x8;
     T* e = (T*)a.e + blockIdx.x * ld;
@@ -320,38 +346,38 @@ __global__ void __launch_bounds__(1024) sums_kernel(const SumsArgs a) {
   sums_over_tokens(a, shared);
 }
 
-// The rows of all ranks' pieces as k of a product, in steps of kStepK; what pads a rank's last tile counts as outside.
+// The rows of all ranks' pieces as k of a product: a step is a unit.
 struct PieceSource {
+  static constexpr int further = 0;
   const Pieces* p;
   int64_t stride;
-  int col_bytes;
-  int rank = -1, left = 0, padded = 0;  // of the rank: rows behind this step's first, padding included or not
-  const char* at = nullptr;
-  __device__ __forceinline__ PieceSource(const Pieces* pieces, int64_t stride, int col_bytes, int row) : p(pieces), stride(stride), col_bytes(col_bytes) {
-    padded = -row;
-    next();
-    const int skip = (p->tile0[rank + 1] - p->tile0[rank]) * kTile - padded;
-    at += skip * stride;
-    left -= skip;
+  int col_bytes, rank, units, left;  // units: of the rank, behind the step's
+  const char* at;
+  __device__ __forceinline__ PieceSource(const Pieces& pieces, int64_t stride, int col_bytes, int unit) : p(&pieces), stride(stride), col_bytes(col_bytes) {
+    const Unit u(pieces, unit);
+    rank = u.rank;
+    units = pieces.unit0[rank + 1] - unit;
+    at = pieces.w[rank] + (u.row - kUnitRows) * stride + col_bytes;
+    left = u.rows + kUnitRows;
   }
-  __device__ __forceinline__ void next() {  // the rank that holds the row `-padded` rows behind this one's end
-    while (padded <= 0 && rank + 1 < p->ranks) {
-      ++rank;
-      padded += (p->tile0[rank + 1] - p->tile0[rank]) * kTile;
+  __device__ __forceinline__ void next() {
+    if (units == 0) {
+      while (rank + 1 < p->ranks && units == 0) {
+        ++rank;
+        units = p->unit0[rank + 1] - p->unit0[rank];
+      }
+      if (units) {
+        at = p->w[rank] - kUnitRows * stride + col_bytes;
+        left = p->rows[rank] + kUnitRows;
+      }
     }
-    left = p->rows[rank];
-    at = p->w[rank] + col_bytes;
+    --units;
+    at += kUnitRows * stride;
+    left -= kUnitRows;
   }
-  __device__ __forceinline__ const char* step(int, int* k_left) {
-    if (padded <= 0) next();
-    const char* here = at;
-    *k_left = left;
-    at += kStepK * stride;
-    left -= kStepK;
-    padded -= kStepK;
-    return here;
-  }
+  __device__ __forceinline__ i32x4 base(int) const { return resource_at(at); }
 };
+static_assert(kUnitRows == kStepK, "a step of dx's product is a unit");
 
 struct GradArgs {
   const void* g;     // [tokens][tiles * kTile]
@@ -395,10 +421,10 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dx_kernel(const Pieces pie
   {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
-    ll.place(threadIdx.x, a.w_stride, width);
-    rl.place(threadIdx.x, ld * 2, tokens);
-    Product::run(smem, steps, ll, PieceSource(&pieces, a.w_stride, d0 * 2, step0 * kStepK), rl,
-                 RowSource{(const char*)a.g + (n0 * ld + (int64_t)step0 * kStepK) * 2, ld}, acc);
+    ll.place(threadIdx.x, a.w_stride, [&](int) { return width; });
+    rl.place(threadIdx.x, ld * 2, [&](int i) { return tokens - i * kUnitRows; });
+    Product::run(smem, steps, ll, PieceSource(pieces, a.w_stride, d0 * 2, step0), rl,
+                 RowSource<TR>([&](int i) { return (const char*)a.g + ((n0 + i * kUnitRows) * ld + (int64_t)step0 * kStepK) * 2; }, steps * kStepK), acc);
   }
   const float back = a.parts ? 0.f : *a.back;  // (with parts the sums may still be under way)
 #pragma unroll
@@ -435,19 +461,20 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dw_kernel(const Pieces pie
   if ((int)blockIdx.x < a.adders) return add_parts<T>(a);
   int at, ht;
   tile_of(blockIdx.x - a.adders, pieces.tiles * (kTile / TR), a.hidden_tiles, &at, &ht);
-  const int rank = pieces.rank_of(at / (kTile / TR)), row0 = at * TR - pieces.tile0[rank] * kTile, rows = min(TR, pieces.rows[rank] - row0);
-  if (rows <= 0) return;  // padding
   const int d0 = ht * TL, width = min(TL, a.hidden - d0);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
   typename Product::Acc acc[Product::FL][Product::FR] = {};
   {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
-    ll.place(threadIdx.x, a.x_stride, width);
-    rl.place(threadIdx.x, ld * 2, TR);
-    Product::run(smem, (a.tokens + kStepK - 1) / kStepK, ll, ColSource{a.x + d0 * 2, a.tokens, a.x_stride}, rl,
-                 ColSource{(const char*)a.g + (int64_t)at * TR * 2, a.tokens, ld * 2}, acc);
+    ll.place(threadIdx.x, a.x_stride, [&](int) { return width; });
+    rl.place(threadIdx.x, ld * 2, [&](int) { return TR; });
+    Product::run(smem, (a.tokens + kStepK - 1) / kStepK, ll, ColSource(a.x + d0 * 2, a.tokens, a.x_stride), rl,
+                 ColSource((const char*)a.g + (int64_t)at * TR * 2, a.tokens, ld * 2), acc);
   }
+  static_assert(TR / Shape::kWavesR == kUnitRows, "a wave's rows are a unit");
+  const int unit0 = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) / Shape::kWavesL);
+  const Unit unit(pieces, at * (TR / kUnitRows) + unit0);
   const float back = *a.back;
 #pragma unroll
   for (int r = 0; r < Product::FR; ++r)
@@ -455,18 +482,18 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dw_kernel(const Pieces pie
     for (int l = 0; l < Product::FL; ++l)
 #pragma unroll
       for (int q = 0; q < Product::kQuads; ++q) {
-        const int v = Product::r_of(threadIdx.x, r), d = Product::l_of(threadIdx.x, l, q);
-        if (v >= rows || d >= width) continue;
+        const int at_tile = Product::r_of(threadIdx.x, r), v = at_tile - unit0 * kUnitRows, d = Product::l_of(threadIdx.x, l, q);
+        if (v >= unit.rows || d >= width) continue;
         f32x4 sum = Product::quad(acc[l][r], q);
         if (a.sums) {
-          f32x4* kept = (f32x4*)(a.sums + ((int64_t)at * TR + v) * a.hidden + d0 + d);
+          f32x4* kept = (f32x4*)(a.sums + ((int64_t)at * TR + at_tile) * a.hidden + d0 + d);
           if (!a.first) sum += *kept;
           if (!a.last) {
             *kept = sum;
             continue;
           }
         }
-        *(typename Half<T>::x4*)(grads.dw[rank] + (row0 + v) * a.dw_stride + (d0 + d) * 2) = narrow<T>(sum, back);
+        *(typename Half<T>::x4*)(grads.dw[unit.rank] + (unit.row + v) * a.dw_stride + (d0 + d) * 2) = narrow<T>(sum, back);
       }
 }
 
@@ -565,19 +592,19 @@ int check_call(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool 
 int tiles(int64_t n, int of = kTile) { return (int)((n + of - 1) / of); }
 
 enum { kLarge, kMiddle, kFew };
-constexpr int kUnits = 256;  // compute units
+constexpr int kComputeUnits = 256;
 
 // Which shape a product takes, by tokens x vocabulary x hidden (bf16, us with the shape / with the next best).
 // Logits: Few up to four rounds of its workgroups (128 x 8192 x 1024: 14.8 / 19.0 Middle; 40 x 65536 x 4096: 123 / 133) but not where W would be read
 // again from memory for every 32 tokens (128 x 65536 x 4096: 208 / 142 Middle); Large once its tiles fill the chip (384 x 32768 x 2048: 58 / 67
 // Middle) and are not half empty, else Middle (256 x 32768 x 2048: 44 / 52 Large).
 int logits_shape(const Pieces& p, int64_t tokens) {
-  if (tokens <= 256 && (int64_t)tiles(tokens, Few::kR) * p.tiles * (kTile / Few::kL) <= 4 * kUnits) return kFew;
-  return tokens <= 128 || (int64_t)tiles(tokens) * p.tiles < kUnits ? kMiddle : kLarge;
+  if (tokens <= 256 && (int64_t)tiles(tokens, Few::kR) * p.tiles * (kTile / Few::kL) <= 4 * kComputeUnits) return kFew;
+  return tokens <= 128 || (int64_t)tiles(tokens) * p.tiles < kComputeUnits ? kMiddle : kLarge;
 }
 // dw writes more than it reads where tokens are few: two workgroups per unit then hide each other's stores (dw's part of 128 x 65536 x 4096 is 75 us shorter
 // with Middle); 1021 x 32003 x 1288: Large 15 us shorter.
-int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 256 || (int64_t)p.tiles * tiles(hidden) < kUnits ? kMiddle : kLarge; }
+int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 256 || (int64_t)p.tiles * tiles(hidden) < kComputeUnits ? kMiddle : kLarge; }
 
 // dx: into how many parts the vocabulary is cut so that the tiles fill the chip, of at least eight steps each (with four, 1024 x 4096 x 512 takes 5 us
 // longer).  Few as long as reading W again for every 32 tokens costs little (128 x 8192 x 1024: 3 us shorter than Middle; 40 x 65536 x 4096: 26 us longer).
@@ -592,7 +619,7 @@ DxPlan dx_plan(const Pieces& p, int64_t tokens, int hidden) {
   const int l = d.shape == kLarge ? Large::kL : d.shape == kMiddle ? Middle::kL : Few::kL, r = d.shape == kLarge ? Large::kR : d.shape == kMiddle ? Middle::kR : Few::kR;
   d.token_tiles = tiles(tokens, r);
   d.hidden_tiles = tiles(hidden, l);
-  const int64_t slots = d.shape == kMiddle ? 2 * kUnits : kUnits;
+  const int64_t slots = d.shape == kMiddle ? 2 * kComputeUnits : kComputeUnits;
   const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, slots / ((int64_t)d.token_tiles * d.hidden_tiles)));
   d.split_steps = (steps + parts - 1) / parts;
   d.parts = (steps + d.split_steps - 1) / d.split_steps;
@@ -662,7 +689,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
         t.lse = io->lse;
         t.loss = c.row_loss;
         t.e = c.e;
-        const unsigned slices = (unsigned)std::max(1, std::min(4 * kUnits / now, p.tiles * kTile / 4096));
+        const unsigned slices = (unsigned)std::max(1, std::min(4 * kComputeUnits / now, p.tiles * kTile / 4096));
         if (backward) hipLaunchKernelGGL((token_kernel<T, true>), dim3(now, slices), dim3(256), 0, stream, p, t);
         else hipLaunchKernelGGL((token_kernel<T, false>), dim3(now), dim3(256), 0, stream, p, t);
         if ((rc = launched("token_kernel"))) return rc;
@@ -703,7 +730,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
     auto go = [&](auto s) {
       typedef decltype(s) S;
       g.hidden_tiles = tiles(d.hidden, S::kL);
-      g.adders = g.parts ? (int)std::min<int64_t>(2 * kUnits, ((int64_t)now * d.hidden / 4 + S::kThreads - 1) / S::kThreads) : 0;
+      g.adders = g.parts ? (int)std::min<int64_t>(2 * kComputeUnits, ((int64_t)now * d.hidden / 4 + S::kThreads - 1) / S::kThreads) : 0;
       hipLaunchKernelGGL((dw_kernel<T, S>), dim3((unsigned)(g.adders + p.tiles * (kTile / S::kR) * g.hidden_tiles)), dim3(S::kThreads), 0, stream, p, c.grads, g);
       return launched("dw_kernel");
     };
@@ -742,19 +769,21 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
     h->desc.rank_rows = nullptr;
     Pieces& p = h->pieces;
     p.ranks = d.ranks;
+    int units = 0;
     for (int r = 0; r < d.ranks; ++r) {
       const int64_t rows = d.rank_rows[r];
-      if (rows < 0 || h->vocab + rows > (1ll << 30)) {
+      if (rows < 0 || (int64_t)units * kUnitRows + rows > MSCCLX_VOCAB_LOSS_MAX_STRIDE - kTile) {  // (rows of G are addressed with 32-bit offsets, 64 at a time)
         delete h;
-        return fail(MSCCLX_ERR_INVALID_ARG, "the ranks' rows must not be negative and add up to at most 2^30");
+        return fail(MSCCLX_ERR_INVALID_ARG, "the ranks' rows must not be negative and, each rank's rounded up to 64, add up to less than 2^22");
       }
       p.rows[r] = (int)rows;
       p.first[r] = (int)h->vocab;
-      p.tile0[r] = p.tiles;
-      p.tiles += tiles(rows);
+      p.unit0[r] = units;
+      units += tiles(rows, kUnitRows);
       h->vocab += rows;
     }
-    p.tile0[d.ranks] = p.tiles;
+    p.unit0[d.ranks] = units;
+    p.tiles = tiles((int64_t)units * kUnitRows);
     if (h->vocab == 0) {
       delete h;
       return fail(MSCCLX_ERR_INVALID_ARG, "the vocabulary is empty");

@@ -50,7 +50,7 @@ def check_all(op, x, weights, labels, upstream, reduction):
 CASES = [  # tokens, hidden, rows
     (1, 8, [1]), (1, 64, [5, 3]), (2, 16, [0, 2, 0]), (3, 72, [257, 0, 255]), (16, 128, [128, 128]), (17, 64, [129]), (31, 200, [513, 31]),
     (64, 256, [300] * 5), (65, 64, [64] * 9), (255, 248, [256, 256]), (256, 256, [256]), (257, 264, [300]), (300, 136, [256, 1, 511]), (129, 1032, [640]),
-    (48, 64, [33] * 64)]
+    (48, 64, [33] * 64), (70, 64, [1] * 64), (300, 72, [65, 0, 190, 64, 63, 2, 0, 321]), (5, 64, [0, 0, 7]), (260, 328, [64, 64, 127, 1])]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -18,7 +18,7 @@ def create_loss(lib, rows=(300, 20), hidden=64, tokens=100, dtype=BF16, reductio
 
 
 @pytest.mark.parametrize("bad, code", [
-    (dict(rows=()), INVALID), (dict(rows=(1,) * 65), INVALID), (dict(rows=(0, 0)), INVALID), (dict(rows=(5, -1)), INVALID), (dict(rows=(1 << 30, 1)), INVALID),
+    (dict(rows=()), INVALID), (dict(rows=(1,) * 65), INVALID), (dict(rows=(0, 0)), INVALID), (dict(rows=(5, -1)), INVALID), (dict(rows=(1 << 30, 1)), INVALID), (dict(rows=(1 << 22,)), INVALID), (dict(rows=(1 << 21, 1 << 21)), INVALID),
     (dict(hidden=0), INVALID), (dict(hidden=12), INVALID), (dict(hidden=1 << 23), INVALID), (dict(tokens=-1), INVALID), (dict(tokens=1 << 31), INVALID),
     (dict(dtype=F32), UNSUPPORTED), (dict(dtype=I32), UNSUPPORTED), (dict(reduction=3), INVALID), (dict(reduction=-1), INVALID)])
 def test_vocab_loss_create_refuses(mscclx_lib, bad, code):
