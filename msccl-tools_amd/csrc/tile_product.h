@@ -10,7 +10,7 @@
 //   row operand: 128 bytes per row, the 16-byte unit u of row i sits at u ^ (i / 2 % 8): the sixteen rows that a
 //                fragment read touches at one unit then cover all 64 banks;
 //   col operand: one line of 2 * TILE bytes per k, 32-byte pair p of line k sits at p ^ swizzle_of(k): the transposing
-//                read takes 8 lines x 1 pair (16 x 16 instructions) or 4 lines x 2 pairs (32 x 32) per half wave, again all banks once.
+//                read takes 8 lines x 1 pair per half wave, again all banks once.
 // What lies outside an operand (rows behind the last, k behind the last) is asked for at an offset beyond the
 // buffer resource's range: the hardware writes zeros for it and touches no memory.
 #ifndef MSCCLX_TILE_PRODUCT_H
@@ -24,8 +24,9 @@
 namespace mscclx {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -45,18 +46,12 @@ template <> struct Half<__bf16> {
   static __device__ __forceinline__ f32x4 mfma(i16x8 a, i16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ f32x16 mfma(i16x8 a, i16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  }
 };
 template <> struct Half<_Float16> {
   typedef f16x4 x4;
   typedef f16x8 x8;
   static __device__ __forceinline__ f32x4 mfma(i16x8 a, i16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f32x16 mfma(i16x8 a, i16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
 };
 
@@ -69,10 +64,10 @@ __device__ __forceinline__ i32x4 resource_at(const char* p) {
   return i32x4{(int)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), (int)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)), kResourceBytes, 0x00020000};
 }
 
-template <int SIDE> __device__ __forceinline__ int swizzle_of(int k) { return SIDE == 16 ? (k & 3) | ((k >> 3 & 1) << 2) : (k & 3) << 1; }
+__device__ __forceinline__ int swizzle_of(int k) { return (k & 3) | ((k >> 3 & 1) << 2); }
 
 // The lanes' places in one operand's tile.  COL: k strided.  WAVES: waves of the workgroup.  CHUNKS copies make a step.
-template <bool COL, int TILE, int WAVES, int SIDE>
+template <bool COL, int TILE, int WAVES>
 struct Lanes {
   static constexpr int kBytes = TILE * kStepK * 2;
   static constexpr int kChunk = WAVES * 1024;
@@ -90,7 +85,7 @@ struct Lanes {
       int line = i * kLines + thread / kUnitsPerLine;
       const int unit = thread % kUnitsPerLine;
       if constexpr (COL) {
-        const int from = (((unit >> 1) ^ swizzle_of<SIDE>(line)) << 1) | (unit & 1);
+        const int from = (((unit >> 1) ^ swizzle_of(line)) << 1) | (unit & 1);
         offset[i] = from * 8 < valid(0) ? (unsigned)(line * stride) + from * 16 : kOutside;
         k[i] = line;
       } else {
@@ -112,13 +107,19 @@ struct Lanes {
 template <int TILE> struct RowSource {  // k contiguous
   static constexpr int kUnits = (TILE + kUnitRows - 1) / kUnitRows;
   i32x4 bases[kUnits];
-  int further = -2 * kStepK, left;
-  // at(i): the address of unit i's first row
-  template <class F> __device__ __forceinline__ RowSource(F at, int k) : left(k + kStepK) {
+  int further, left, turn, steps;
+  // at(i): the address of unit i's first row.  first: the step to begin with; those in front of it come last
+  template <class F> __device__ __forceinline__ RowSource(F at, int k, int first = 0) : steps((k + kStepK - 1) / kStepK) {
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) bases[i] = resource_at(at(i));
+    further = (first - 1) * 2 * kStepK;
+    left = k - (first - 1) * kStepK;
+    turn = first ? steps - first : -1;  // steps up to the first one again
   }
-  __device__ __forceinline__ void next() { further += 2 * kStepK, left -= kStepK; }
+  __device__ __forceinline__ void next() {
+    further += 2 * kStepK, left -= kStepK;
+    if (turn-- == 0) further -= steps * 2 * kStepK, left += steps * kStepK;
+  }
   __device__ __forceinline__ i32x4 base(int i) const { return bases[i]; }
 };
 struct ColSource {  // k strided
@@ -131,52 +132,53 @@ struct ColSource {  // k strided
   __device__ __forceinline__ i32x4 base(int) const { return resource_at(at); }
 };
 
-// TL x TR: the workgroup's tile, cut among WL x WR waves; SIDE: of the matrix instruction, 16 or 32; STAGES: steps held in LDS, a power of two.
-template <class T, int TL, int TR, int WL, int WR, int SIDE, int STAGES, bool LCOL, bool RCOL>
+// TL x TR: the workgroup's tile, cut among WL x WR waves; STAGES: steps held in LDS, a power of two.
+template <class T, int TL, int TR, int WL, int WR, int STAGES, bool LCOL, bool RCOL>
 struct TileProduct {
   static constexpr int kWaves = WL * WR, kThreads = kWaves * 64;
-  static constexpr int FL = TL / WL / SIDE, FR = TR / WR / SIDE;  // fragments of a wave
-  static constexpr int kSlices = SIDE / 16;                        // instructions for 32 values of k
-  static constexpr int kQuads = SIDE == 16 ? 1 : 4;                // groups of four neighbours that a lane holds of a fragment's result
-  typedef std::conditional_t<SIDE == 16, f32x4, f32x16> Acc;
-  typedef Lanes<LCOL, TL, kWaves, SIDE> LLanes;
-  typedef Lanes<RCOL, TR, kWaves, SIDE> RLanes;
+  static constexpr int FL = TL / WL / 16, FR = TR / WR / 16;  // fragments of a wave
+  typedef Lanes<LCOL, TL, kWaves> LLanes;
+  typedef Lanes<RCOL, TR, kWaves> RLanes;
   static constexpr int kStage = LLanes::kBytes + RLanes::kBytes;
   static constexpr int kLdsBytes = STAGES * kStage;
   static constexpr int kCopies = LLanes::kChunks + RLanes::kChunks;  // of a wave, per step
 
-  // where in the tile the lane's quads lie: l of fragment f's quad q (its first), r of fragment f
-  static __device__ __forceinline__ int l_of(int thread, int f, int q) {
-    const int lane = thread & 63;
-    return (thread >> 6) % WL * (TL / WL) + f * SIDE + (SIDE == 16 ? lane >> 4 : 2 * q + (lane >> 5)) * 4;
+  // where in the tile a lane's results of fragment f lie: l of the first of its four neighbours, and r
+  static __device__ __forceinline__ int l_of(int thread, int f) { return (thread >> 6) % WL * (TL / WL) + f * 16 + (thread >> 4 & 3) * 4; }
+  static __device__ __forceinline__ int r_of(int thread, int f) { return (thread >> 6) / WL * (TR / WR) + f * 16 + (thread & 15); }
+
+  // Stores want 16 bytes per lane.  A lane holds four neighbours of fragment f and four of f + 1; lanes 16 apart swap one of them, so that
+  // each has eight neighbours of one fragment: 64 bytes of an output row per store.  -> their place in the tile, l
+  static __device__ __forceinline__ int l_of_pair(int thread, int f) {
+    const int group = thread >> 4 & 3;
+    return (thread >> 6) % WL * (TL / WL) + (f + (group & 1)) * 16 + (group >> 1) * 8;
   }
-  static __device__ __forceinline__ int r_of(int thread, int f) { return (thread >> 6) / WL * (TR / WR) + f * SIDE + (thread & (SIDE - 1)); }
-  static __device__ __forceinline__ f32x4 quad(const Acc& a, int q) {
-    if constexpr (SIDE == 16) return a;
-    else return f32x4{a[q * 4], a[q * 4 + 1], a[q * 4 + 2], a[q * 4 + 3]};
+  template <class X4> static __device__ __forceinline__ u32x4 pair_up(X4 first, X4 second) {
+    const u32x2 a = __builtin_bit_cast(u32x2, first), b = __builtin_bit_cast(u32x2, second);
+    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false));
+    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false));
+    return u32x4{x[0], y[0], x[1], y[1]};
   }
 
-  // fragment f of slice s in a step's half
+  // fragment f of a step's half
   template <bool COL, int TILE>
-  static __device__ __forceinline__ i16x8 fragment(const char* lds, int first, int half, int lane, int s, int f) {
-    const int group = SIDE == 16 ? lane >> 4 : lane >> 5;  // of eight values of k
+  static __device__ __forceinline__ i16x8 fragment(const char* lds, int first, int half, int lane, int f) {
+    const int group = lane >> 4;  // of eight values of k
     if constexpr (COL) {
       typedef __attribute__((address_space(3))) i16x4* lds_ptr;
-      const int within = group * 8 + (lane >> 2 & 3), pair = (first >> 4) + (SIDE == 32 ? lane >> 4 & 1 : 0) + f * (SIDE / 16);
-      const int k = half * 32 + s * 16 + within;  // (a slice or a half further the swizzle is the same)
-      const char* p = lds + k * (TILE * 2) + ((pair ^ swizzle_of<SIDE>(within)) << 5) + (lane & 3) * 8;
+      const int within = group * 8 + (lane >> 2 & 3);  // (half a step further the swizzle is the same)
+      const char* p = lds + (half * 32 + within) * (TILE * 2) + ((((first >> 4) + f) ^ swizzle_of(within)) << 5) + (lane & 3) * 8;
       const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
       const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * TILE * 2));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
-      const int unit = (half * 4 + s * 2 + group) ^ (lane >> 1 & 7);
-      return *(const i16x8*)(lds + (first + f * SIDE + (lane & (SIDE - 1))) * 128 + unit * 16);
+      return *(const i16x8*)(lds + (first + f * 16 + (lane & 15)) * 128 + ((half * 4 + group) ^ (lane >> 1 & 7)) * 16);
     }
   }
 
   // acc[l][r] += the product over all steps.  Every wave of the workgroup calls this with the same sources.
   template <class SL, class SR>
-  static __device__ __forceinline__ void run(char* smem, int steps, const LLanes& ll, SL sl, const RLanes& rl, SR sr, Acc (&acc)[FL][FR]) {
+  static __device__ __forceinline__ void run(char* smem, int steps, const LLanes& ll, SL sl, const RLanes& rl, SR sr, f32x4 (&acc)[FL][FR]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l0 = wave % WL * (TL / WL), r0 = wave / WL * (TR / WR);
     typedef __attribute__((address_space(3))) char* lds_char;
@@ -187,22 +189,38 @@ struct TileProduct {
       else i -= LLanes::kChunks, rl.copy(i, at + LLanes::kBytes, sr.base(RCOL ? 0 : i * RLanes::kLines / kUnitRows), sr.further, sr.left);
     };
     struct Fragments {  // of half a step
-      i16x8 a[kSlices][FL], b[kSlices][FR];
+      i16x8 a[FL], b[FR];
     };
-    constexpr int kUnits = (FL + FR) * kSlices;
+    constexpr int kUnits = FL + FR;
     auto read = [&](Fragments& f, int s, int half, int u) {  // unit u: all of r, then of l, as the products want them
       const char* at = smem + s % STAGES * kStage;
-      if (u < FR * kSlices) f.b[u % kSlices][u / kSlices] = fragment<RCOL, TR>(at + LLanes::kBytes, r0, half, lane, u % kSlices, u / kSlices);
-      else u -= FR * kSlices, f.a[u % kSlices][u / kSlices] = fragment<LCOL, TL>(at, l0, half, lane, u % kSlices, u / kSlices);
+      if (u < FR) f.b[u] = fragment<RCOL, TR>(at + LLanes::kBytes, r0, half, lane, u);
+      else f.a[u - FR] = fragment<LCOL, TL>(at, l0, half, lane, u - FR);
     };
     // One fragment row of products after another; between them the next half's reads and, in the second half, the copies, so
     // that neither LDS nor the path to it gets all of a step's requests at once.
     auto multiply = [&](const Fragments& f, int l) {
 #pragma unroll
-      for (int s = 0; s < kSlices; ++s)
-#pragma unroll
-        for (int r = 0; r < FR; ++r) acc[l][r] = Half<T>::mfma(f.a[s][l], f.b[s][r], acc[l][r]);
+      for (int r = 0; r < FR; ++r) acc[l][r] = Half<T>::mfma(f.a[l], f.b[r], acc[l][r]);
     };
+    if constexpr (STAGES == 1) {  // nothing is read ahead: other workgroups of the compute unit fill the time
+      for (int s = 0; s < steps; ++s) {
+        sl.next(), sr.next();
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) copy(0, i);
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          Fragments f;
+#pragma unroll
+          for (int u = 0; u < kUnits; ++u) read(f, 0, half, u);
+#pragma unroll
+          for (int l = 0; l < FL; ++l) multiply(f, l);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      }
+      return;
+    }
     Fragments now, next;
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) {

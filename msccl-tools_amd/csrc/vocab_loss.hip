@@ -30,6 +30,7 @@ namespace mscclx {
 namespace {
 
 constexpr int kMaxRanks = MSCCLX_VOCAB_LOSS_MAX_RANKS;
+constexpr int kComputeUnits = 256;
 constexpr int kTile = 256;              // columns of G are padded to a multiple of it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -86,14 +87,16 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 template <class T> constexpr float kUnit = std::is_same_v<T, _Float16> ? 32768.0f : 1.0f;
 
 // How a workgroup's tile is cut.  Large: one workgroup of eight waves per compute unit.  Middle: two of four waves, for products whose large tiles
-// would not fill the chip.  Few: at most 32 tokens, with four steps of copies under way, because then memory is all that counts.
-template <int L, int R, int WL, int WR, int SIDE, int STAGES> struct Shape {
-  static constexpr int kL = L, kR = R, kWavesL = WL, kWavesR = WR, kThreads = WL * WR * 64, kSide = SIDE;
-  template <class T, bool LCOL, bool RCOL> using Product = TileProduct<T, L, R, WL, WR, SIDE, STAGES, LCOL, RCOL>;
+// would not fill the chip.  Thin: four of four waves, each one step at a time, for products that write more than they read.  Few: at most 32 tokens, with
+// four steps of copies under way, because then memory is all that counts.
+template <int L, int R, int WL, int WR, int STAGES, int WAVES> struct Shape {  // WAVES: per SIMD, at least
+  static constexpr int kL = L, kR = R, kWavesL = WL, kWavesR = WR, kThreads = WL * WR * 64, kWaves = WAVES;
+  template <class T, bool LCOL, bool RCOL> using Product = TileProduct<T, L, R, WL, WR, STAGES, LCOL, RCOL>;
 };
-typedef Shape<256, 256, 2, 4, 16, 2> Large;
-typedef Shape<128, 128, 2, 2, 16, 2> Middle;
-typedef Shape<128, 32, 4, 1, 16, 4> Few;
+typedef Shape<256, 256, 2, 4, 2, 2> Large;
+typedef Shape<128, 128, 2, 2, 2, 2> Middle;
+typedef Shape<128, 128, 2, 2, 1, 4> Thin;
+typedef Shape<128, 32, 4, 1, 4, 2> Few;
 
 enum { kStats = 0, kKeep = 1, kGradient = 2 };
 
@@ -122,30 +125,33 @@ __device__ __forceinline__ void tile_of(int id, int rows, int cols, int* row, in
 }
 
 template <class T, int MODE, class Shape>
-__global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces pieces, const LogitsArgs a) {
+__global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(const Pieces pieces, const LogitsArgs a) {
   typedef typename Shape::template Product<T, false, false> Product;
   constexpr int TL = Shape::kL, TR = Shape::kR, kPart = TL / Shape::kWavesL;  // vocabulary of a wave
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
   int tt, at;
   tile_of(blockIdx.x, a.token_tiles, pieces.tiles * (kTile / TL), &tt, &at);
   const int n0 = tt * TR, tokens = min(TR, a.tokens - n0);
-  typename Product::Acc acc[Product::FL][Product::FR] = {};
+  f32x4 acc[Product::FL][Product::FR] = {};
   {
+    // With one workgroup per compute unit all would ask for the same few bytes of each row of W at a time, which lie a power of two apart;
+    // each begins at another k (1 token x 32768 x 2048: 34 us in step, 30 so; with more workgroups it costs 3 %)
+    const int steps = (a.hidden + kStepK - 1) / kStepK, first = TR == Few::kR && gridDim.x <= kComputeUnits ? at % steps : 0;
     typename Product::LLanes ll;
     typename Product::RLanes rl;
     ll.place(threadIdx.x, a.w_stride, [&](int i) { return Unit(pieces, at * (TL / kUnitRows) + i).rows; });
     rl.place(threadIdx.x, a.x_stride, [&](int i) { return tokens - i * kUnitRows; });
-    Product::run(smem, (a.hidden + kStepK - 1) / kStepK, ll,
+    Product::run(smem, steps, ll,
                  RowSource<TL>([&](int i) {
                    const Unit u(pieces, at * (TL / kUnitRows) + i);
                    return pieces.w[u.rank] + u.row * a.w_stride;
-                 }, a.hidden),
-                 rl, RowSource<TR>([&](int i) { return a.x + (n0 + i * kUnitRows) * a.x_stride; }, a.hidden), acc);
+                 }, a.hidden, first),
+                 rl, RowSource<TR>([&](int i) { return a.x + (n0 + i * kUnitRows) * a.x_stride; }, a.hidden, first), acc);
   }
   const int64_t ld = (int64_t)pieces.tiles * kTile;
   const int lane = threadIdx.x & 63, part = (threadIdx.x >> 6) % Shape::kWavesL;
   // the wave's part of the vocabulary: whole units, or part of one
-  constexpr int kOfWave = kPart < kUnitRows ? kPart : kUnitRows, kWaveUnits = kPart / kOfWave, kUnitFragments = kOfWave / Shape::kSide;
+  constexpr int kOfWave = kPart < kUnitRows ? kPart : kUnitRows, kWaveUnits = kPart / kOfWave, kUnitFragments = kOfWave / 16;
   int rows[kWaveUnits], first[kWaveUnits];  // of each: rows that exist, and the first one's number in the whole vocabulary
   bool all = true;
 #pragma unroll
@@ -168,19 +174,33 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces
       for (int j = 0; j < kWaveUnits; ++j) here |= label >= first[j] && label < first[j] + min(rows[j], kOfWave);
       const bool any = __any(here);  // one wave in hundreds holds a label of its tokens
       T* out = (T*)a.e + (n0 + n) * ld + (int64_t)at * TL;
-      // the wave's logits of the token, in fours: f(place in the tile, row in the unit, the unit's rows, the label's row in it, logits)
+      // the wave's logits of the token, in fours: f(row in the unit, the unit's rows, the label's row in it, logits)
       auto each = [&](auto f) {
 #pragma unroll
-        for (int l = 0; l < Product::FL; ++l)
+        for (int l = 0; l < Product::FL; ++l) {
+          const int j = l / kUnitFragments;
+          f(Product::l_of(threadIdx.x, l) - part * kPart - j * kOfWave, rows[j], label - first[j], acc[l][r]);
+        }
+      };
+      // the same, and what f makes of them to G's row
+      auto each_stored = [&](auto f) {
 #pragma unroll
-          for (int q = 0; q < Product::kQuads; ++q) {
-            const int v = Product::l_of(threadIdx.x, l, q), j = l / kUnitFragments;
-            f(v, v - part * kPart - j * kOfWave, rows[j], label - first[j], Product::quad(acc[l][r], q));
+        for (int l = 0; l < Product::FL; l += 2) {
+          typename Half<T>::x4 o[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int v = Product::l_of(threadIdx.x, l + k), j = (l + k) / kUnitFragments;
+            o[k] = f(v - part * kPart - j * kOfWave, rows[j], label - first[j], acc[l + k][r]);
           }
+          if (MODE != kStats) {
+            const u32x4 row = Product::pair_up(o[0], o[1]);
+            if (live) *(u32x4*)(out + Product::l_of_pair(threadIdx.x, l)) = row;
+          }
+        }
       };
       if constexpr (MODE == kGradient) {
         const float lse = live ? a.lse[a.token0 + n0 + n] * kLog2e : 0.f, g = live ? a.upstream.get(a.token0 + n0 + n, label) * kUnit<T> : 0.f;
-        each([&](int v, int row, int rows, int want, f32x4 z) {
+        each_stored([&](int row, int rows, int want, f32x4 z) {
           typename Half<T>::x4 o;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -188,11 +208,11 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces
             if (any) p -= here && row + i == want ? 1.f : 0.f;
             o[i] = (T)((WHOLE || row + i < rows) && g != 0.f ? p * g : 0.f);
           }
-          if (live) *(typename Half<T>::x4*)(out + v) = o;
+          return o;
         });
       } else {
         float m = -INFINITY;
-        each([&](int, int row, int rows, int, f32x4 z) {
+        each([&](int row, int rows, int, f32x4 z) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (WHOLE || row + i < rows) m = fmaxf(m, z[i]);
@@ -200,7 +220,7 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces
         if (any) {
           float z_label = 0.f;
           bool found = false;
-          each([&](int, int row, int rows, int want, f32x4 z) {
+          each([&](int row, int rows, int want, f32x4 z) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               if (here && row + i == want && row + i < rows) z_label = z[i], found = true;
@@ -208,11 +228,11 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces
           if (found) a.z_label[a.token0 + n0 + n] = z_label;
         }
 #pragma unroll
-        for (int d = Shape::kSide; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+        for (int d = 16; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
         m *= kLog2e;
         const float base = m == -INFINITY ? 0.f : m;  // a part of nothing but -inf has sum 0
         float sum = 0.f;
-        each([&](int v, int row, int rows, int, f32x4 z) {
+        each_stored([&](int row, int rows, int, f32x4 z) {
           typename Half<T>::x4 o;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -220,11 +240,11 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) logits_kernel(const Pieces
             sum += e;
             o[i] = (T)(e * kUnit<T>);
           }
-          if (MODE == kKeep && live) *(typename Half<T>::x4*)(out + v) = o;
+          return o;
         });
 #pragma unroll
-        for (int d = Shape::kSide; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-        if (live && lane < Shape::kSide) a.stats[(n0 + n) * (ld / kPart) + at * TL / kPart + part] = make_float2(m, sum);
+        for (int d = 16; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+        if (live && lane < 16) a.stats[(n0 + n) * (ld / kPart) + at * TL / kPart + part] = make_float2(m, sum);
       }
     }
   };
@@ -404,7 +424,7 @@ template <class T> __device__ __forceinline__ typename Half<T>::x4 narrow(f32x4 
 }
 
 template <class T, class Shape>
-__global__ void __launch_bounds__(Shape::kThreads, 2) dx_kernel(const Pieces pieces, const GradArgs a, const SumsArgs sums) {
+__global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dx_kernel(const Pieces pieces, const GradArgs a, const SumsArgs sums) {
   typedef typename Shape::template Product<T, true, false> Product;
   constexpr int TL = Shape::kL, TR = Shape::kR;
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
@@ -417,7 +437,7 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dx_kernel(const Pieces pie
   const int n0 = tt * TR, d0 = ht * TL, tokens = min(TR, a.tokens - n0), width = min(TL, a.hidden - d0);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
   const int step0 = blockIdx.y * a.split_steps, steps = min(a.split_steps, pieces.tiles * (kTile / kStepK) - step0);
-  typename Product::Acc acc[Product::FL][Product::FR] = {};
+  f32x4 acc[Product::FL][Product::FR] = {};
   {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
@@ -428,17 +448,23 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dx_kernel(const Pieces pie
   }
   const float back = a.parts ? 0.f : *a.back;  // (with parts the sums may still be under way)
 #pragma unroll
-  for (int r = 0; r < Product::FR; ++r)
+  for (int r = 0; r < Product::FR; ++r) {
+    const int n = Product::r_of(threadIdx.x, r);
+    if (a.parts) {
 #pragma unroll
-    for (int l = 0; l < Product::FL; ++l)
-#pragma unroll
-      for (int q = 0; q < Product::kQuads; ++q) {
-        const int n = Product::r_of(threadIdx.x, r), d = Product::l_of(threadIdx.x, l, q);
-        if (n >= tokens || d >= width) continue;
-        const f32x4 sum = Product::quad(acc[l][r], q);
-        if (a.parts) *(f32x4*)(a.parts + ((int64_t)blockIdx.y * a.tokens + n0 + n) * a.hidden + d0 + d) = sum;
-        else *(typename Half<T>::x4*)(a.dx + (n0 + n) * a.dx_stride + (d0 + d) * 2) = narrow<T>(sum, back);
+      for (int l = 0; l < Product::FL; ++l) {
+        const int d = Product::l_of(threadIdx.x, l);
+        if (n < tokens && d < width) *(f32x4*)(a.parts + ((int64_t)blockIdx.y * a.tokens + n0 + n) * a.hidden + d0 + d) = acc[l][r];
       }
+    } else {
+#pragma unroll
+      for (int l = 0; l < Product::FL; l += 2) {
+        const u32x4 row = Product::pair_up(narrow<T>(acc[l][r], back), narrow<T>(acc[l + 1][r], back));
+        const int d = Product::l_of_pair(threadIdx.x, l);
+        if (n < tokens && d < width) *(u32x4*)(a.dx + (n0 + n) * a.dx_stride + (d0 + d) * 2) = row;
+      }
+    }
+  }
 }
 
 // dx from the parts of the vocabulary: four values per thread and turn
@@ -454,7 +480,7 @@ template <class T> __device__ __forceinline__ void add_parts(const GradArgs& a) 
 }
 
 template <class T, class Shape>
-__global__ void __launch_bounds__(Shape::kThreads, 2) dw_kernel(const Pieces pieces, const Grads grads, const GradArgs a) {
+__global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dw_kernel(const Pieces pieces, const Grads grads, const GradArgs a) {
   typedef typename Shape::template Product<T, true, true> Product;
   constexpr int TL = Shape::kL, TR = Shape::kR;
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
@@ -463,7 +489,7 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dw_kernel(const Pieces pie
   tile_of(blockIdx.x - a.adders, pieces.tiles * (kTile / TR), a.hidden_tiles, &at, &ht);
   const int d0 = ht * TL, width = min(TL, a.hidden - d0);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
-  typename Product::Acc acc[Product::FL][Product::FR] = {};
+  f32x4 acc[Product::FL][Product::FR] = {};
   {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
@@ -477,24 +503,26 @@ __global__ void __launch_bounds__(Shape::kThreads, 2) dw_kernel(const Pieces pie
   const Unit unit(pieces, at * (TR / kUnitRows) + unit0);
   const float back = *a.back;
 #pragma unroll
-  for (int r = 0; r < Product::FR; ++r)
+  for (int r = 0; r < Product::FR; ++r) {
+    const int at_tile = Product::r_of(threadIdx.x, r), v = at_tile - unit0 * kUnitRows;
+    if (a.sums) {  // of the pieces of tokens so far
 #pragma unroll
-    for (int l = 0; l < Product::FL; ++l)
-#pragma unroll
-      for (int q = 0; q < Product::kQuads; ++q) {
-        const int at_tile = Product::r_of(threadIdx.x, r), v = at_tile - unit0 * kUnitRows, d = Product::l_of(threadIdx.x, l, q);
+      for (int l = 0; l < Product::FL; ++l) {
+        const int d = Product::l_of(threadIdx.x, l);
+        f32x4* kept = (f32x4*)(a.sums + ((int64_t)at * TR + at_tile) * a.hidden + d0 + d);
         if (v >= unit.rows || d >= width) continue;
-        f32x4 sum = Product::quad(acc[l][r], q);
-        if (a.sums) {
-          f32x4* kept = (f32x4*)(a.sums + ((int64_t)at * TR + at_tile) * a.hidden + d0 + d);
-          if (!a.first) sum += *kept;
-          if (!a.last) {
-            *kept = sum;
-            continue;
-          }
-        }
-        *(typename Half<T>::x4*)(grads.dw[unit.rank] + (unit.row + v) * a.dw_stride + (d0 + d) * 2) = narrow<T>(sum, back);
+        if (!a.first) acc[l][r] += *kept;
+        if (!a.last) *kept = acc[l][r];
       }
+      if (!a.last) continue;
+    }
+#pragma unroll
+    for (int l = 0; l < Product::FL; l += 2) {
+      const u32x4 row = Product::pair_up(narrow<T>(acc[l][r], back), narrow<T>(acc[l + 1][r], back));
+      const int d = Product::l_of_pair(threadIdx.x, l);
+      if (v < unit.rows && d < width) *(u32x4*)(grads.dw[unit.rank] + (unit.row + v) * a.dw_stride + (d0 + d) * 2) = row;
+    }
+  }
 }
 
 int launched(const char* what) {
@@ -591,9 +619,7 @@ int check_call(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool 
 
 int tiles(int64_t n, int of = kTile) { return (int)((n + of - 1) / of); }
 
-enum { kLarge, kMiddle, kFew };
-constexpr int kComputeUnits = 256;
-
+enum { kLarge, kMiddle, kThin, kFew };
 // Which shape a product takes, by tokens x vocabulary x hidden (bf16, us with the shape / with the next best).
 // Logits: Few up to four rounds of its workgroups (128 x 8192 x 1024: 14.8 / 19.0 Middle; 40 x 65536 x 4096: 123 / 133) but not where W would be read
 // again from memory for every 32 tokens (128 x 65536 x 4096: 208 / 142 Middle); Large once its tiles fill the chip (384 x 32768 x 2048: 58 / 67
@@ -602,9 +628,10 @@ int logits_shape(const Pieces& p, int64_t tokens) {
   if (tokens <= 256 && (int64_t)tiles(tokens, Few::kR) * p.tiles * (kTile / Few::kL) <= 4 * kComputeUnits) return kFew;
   return tokens <= 128 || (int64_t)tiles(tokens) * p.tiles < kComputeUnits ? kMiddle : kLarge;
 }
-// dw writes more than it reads where tokens are few: two workgroups per unit then hide each other's stores (dw's part of 128 x 65536 x 4096 is 75 us shorter
-// with Middle); 1021 x 32003 x 1288: Large 15 us shorter.
-int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 256 || (int64_t)p.tiles * tiles(hidden) < kComputeUnits ? kMiddle : kLarge; }
+// dw writes more than it reads where tokens are few; workgroups then hide each other's loads and stores (dw's part, by tokens x vocabulary x hidden: 16 x 131072 x
+// 4096 210 us Thin / 304 Middle, 200 x 20000 x 3000 47 / 60, 300 x 20000 x 1024 26 / 32 Large; 500 x 32768 x 2048 92 / 85 Large).  1021 x 32003 x 1288: Large 15 us
+// shorter than Middle.
+int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 384 ? kThin : (int64_t)p.tiles * tiles(hidden) < kComputeUnits ? kMiddle : kLarge; }
 
 // dx: into how many parts the vocabulary is cut so that the tiles fill the chip, of at least eight steps each (with four, 1024 x 4096 x 512 takes 5 us
 // longer).  Few as long as reading W again for every 32 tokens costs little (128 x 8192 x 1024: 3 us shorter than Middle; 40 x 65536 x 4096: 26 us longer).
@@ -619,7 +646,7 @@ DxPlan dx_plan(const Pieces& p, int64_t tokens, int hidden) {
   const int l = d.shape == kLarge ? Large::kL : d.shape == kMiddle ? Middle::kL : Few::kL, r = d.shape == kLarge ? Large::kR : d.shape == kMiddle ? Middle::kR : Few::kR;
   d.token_tiles = tiles(tokens, r);
   d.hidden_tiles = tiles(hidden, l);
-  const int64_t slots = d.shape == kMiddle ? 2 * kComputeUnits : kComputeUnits;
+  const int64_t slots = d.shape == kLarge ? kComputeUnits : 2 * kComputeUnits;  // (Few with one per unit: 16 x 131072 x 4096 245 us instead of 190)
   const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, slots / ((int64_t)d.token_tiles * d.hidden_tiles)));
   d.split_steps = (steps + parts - 1) / parts;
   d.parts = (steps + d.split_steps - 1) / d.split_steps;
@@ -734,7 +761,8 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
       hipLaunchKernelGGL((dw_kernel<T, S>), dim3((unsigned)(g.adders + p.tiles * (kTile / S::kR) * g.hidden_tiles)), dim3(S::kThreads), 0, stream, p, c.grads, g);
       return launched("dw_kernel");
     };
-    if ((rc = dw_shape(p, now, d.hidden) == kLarge ? go(Large()) : go(Middle()))) return rc;
+    const int shape = dw_shape(p, now, d.hidden);
+    if ((rc = shape == kLarge ? go(Large()) : shape == kMiddle ? go(Middle()) : go(Thin()))) return rc;
   }
   if (n == 0 && forward && !per_token && !backward) return sums(true);
   return MSCCLX_OK;
