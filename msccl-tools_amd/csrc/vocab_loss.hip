@@ -40,16 +40,25 @@ struct Pieces {
   int ranks, tiles;
   int rows[kMaxRanks];
   int unit0[kMaxRanks + 1];  // the rank's first unit
-  int first[kMaxRanks];      // the rank's first row in the whole vocabulary
+  int first[kMaxRanks + 1];  // the rank's first row in the whole vocabulary
   const char* w[kMaxRanks];
+};
+
+// Which rank holds something: the ranks' ends, one in each lane, are compared at once.  (A loop over the ranks waits for memory at every turn.)
+struct Ends {
+  int end, ranks;
+  __device__ __forceinline__ Ends(const int* ends, int ranks) : ranks(ranks) {
+    const int lane = threadIdx.x & 63;
+    end = lane < ranks ? ends[lane] : 0x7fffffff;
+  }
+  __device__ __forceinline__ int rank_of(int at) const { return min((int)__popcll(__ballot(at >= end)), ranks - 1); }
 };
 
 // Unit `unit` of the padded vocabulary
 struct Unit {
   int rank, row;  // its rank, and its first row there
   int rows;       // from that row on; may be none, or less
-  __device__ __forceinline__ Unit(const Pieces& p, int unit) : rank(0) {
-    while (rank + 1 < p.ranks && unit >= p.unit0[rank + 1]) ++rank;
+  __device__ __forceinline__ Unit(const Pieces& p, const Ends& ends, int unit) : rank(__builtin_amdgcn_readfirstlane(ends.rank_of(unit))) {
     row = (unit - p.unit0[rank]) * kUnitRows;
     rows = p.rows[rank] - row;
   }
@@ -129,6 +138,7 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
   typedef typename Shape::template Product<T, false, false> Product;
   constexpr int TL = Shape::kL, TR = Shape::kR, kPart = TL / Shape::kWavesL;  // vocabulary of a wave
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
+  const Ends ends(pieces.unit0 + 1, pieces.ranks);
   int tt, at;
   tile_of(blockIdx.x, a.token_tiles, pieces.tiles * (kTile / TL), &tt, &at);
   const int n0 = tt * TR, tokens = min(TR, a.tokens - n0);
@@ -139,11 +149,11 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
     const int steps = (a.hidden + kStepK - 1) / kStepK, first = TR == Few::kR && gridDim.x <= kComputeUnits ? at % steps : 0;
     typename Product::LLanes ll;
     typename Product::RLanes rl;
-    ll.place(threadIdx.x, a.w_stride, [&](int i) { return Unit(pieces, at * (TL / kUnitRows) + i).rows; });
+    ll.place(threadIdx.x, a.w_stride, [&](int i) { return Unit(pieces, ends, at * (TL / kUnitRows) + i).rows; });
     rl.place(threadIdx.x, a.x_stride, [&](int i) { return tokens - i * kUnitRows; });
     Product::run(smem, steps, ll,
                  RowSource<TL>([&](int i) {
-                   const Unit u(pieces, at * (TL / kUnitRows) + i);
+                   const Unit u(pieces, ends, at * (TL / kUnitRows) + i);
                    return pieces.w[u.rank] + u.row * a.w_stride;
                  }, a.hidden, first),
                  rl, RowSource<TR>([&](int i) { return a.x + (n0 + i * kUnitRows) * a.x_stride; }, a.hidden, first), acc);
@@ -157,7 +167,7 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
 #pragma unroll
   for (int j = 0; j < kWaveUnits; ++j) {
     const int from = __builtin_amdgcn_readfirstlane(at * TL + part * kPart + j * kOfWave);
-    const Unit u(pieces, from / kUnitRows);
+    const Unit u(pieces, ends, from / kUnitRows);
     rows[j] = u.rows - from % kUnitRows;
     first[j] = pieces.first[u.rank] + u.row + from % kUnitRows;
     all &= rows[j] >= kOfWave;
@@ -301,8 +311,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
     const float g = a.upstream.get(at, label);
     int64_t want = -1;
     if (label >= 0) {
-      int r = 0;
-      while (r + 1 < pieces.ranks && label >= pieces.first[r + 1]) ++r;
+      const int r = Ends(pieces.first + 1, pieces.ranks).rank_of(label);
       want = (int64_t)pieces.unit0[r] * kUnitRows + label - pieces.first[r];
     }
     typedef typename Half<T>::x8 x8;
@@ -374,7 +383,7 @@ struct PieceSource {
   int col_bytes, rank, units, left;  // units: of the rank, behind the step's
   const char* at;
   __device__ __forceinline__ PieceSource(const Pieces& pieces, int64_t stride, int col_bytes, int unit) : p(&pieces), stride(stride), col_bytes(col_bytes) {
-    const Unit u(pieces, unit);
+    const Unit u(pieces, Ends(pieces.unit0 + 1, pieces.ranks), unit);
     rank = u.rank;
     units = pieces.unit0[rank + 1] - unit;
     at = pieces.w[rank] + (u.row - kUnitRows) * stride + col_bytes;
@@ -500,7 +509,7 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dw_kernel(cons
   }
   static_assert(TR / Shape::kWavesR == kUnitRows, "a wave's rows are a unit");
   const int unit0 = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) / Shape::kWavesL);
-  const Unit unit(pieces, at * (TR / kUnitRows) + unit0);
+  const Unit unit(pieces, Ends(pieces.unit0 + 1, pieces.ranks), at * (TR / kUnitRows) + unit0);
   const float back = *a.back;
 #pragma unroll
   for (int r = 0; r < Product::FR; ++r) {
@@ -811,6 +820,7 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
       h->vocab += rows;
     }
     p.unit0[d.ranks] = units;
+    p.first[d.ranks] = (int)h->vocab;
     p.tiles = tiles((int64_t)units * kUnitRows);
     if (h->vocab == 0) {
       delete h;
