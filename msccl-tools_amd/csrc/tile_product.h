@@ -78,16 +78,17 @@ struct Lanes {
   unsigned offset[kChunks];
   int k[COL ? kChunks : 1];                                      // the lane's k (its first) in the step
 
-  // `stride`: bytes between rows of memory; `valid(unit)`: rows of the unit (row, counted from its base) or columns (col) that exist
-  template <class F> __device__ __forceinline__ void place(int thread, int64_t stride, F valid) {
+  // `stride`: bytes between rows of memory; `valid(unit)`: rows of the unit (row, counted from its base) or columns (col) that exist.  A col operand's
+  // rows repeat themselves within a step with `period`, if it is less than a step.
+  template <class F> __device__ __forceinline__ void place(int thread, int64_t stride, F valid, int period = kStepK) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       int line = i * kLines + thread / kUnitsPerLine;
       const int unit = thread % kUnitsPerLine;
       if constexpr (COL) {
         const int from = (((unit >> 1) ^ swizzle_of(line)) << 1) | (unit & 1);
-        offset[i] = from * 8 < valid(0) ? (unsigned)(line * stride) + from * 16 : kOutside;
-        k[i] = line;
+        k[i] = line & (period - 1);
+        offset[i] = from * 8 < valid(0) ? (unsigned)(k[i] * stride) + from * 16 : kOutside;
       } else {
         const int from = unit ^ (line >> 1 & 7);
         if (i == 0) k[0] = from * 8;   // a chunk is a multiple of 16 lines: the same for all
@@ -126,9 +127,17 @@ struct ColSource {  // k strided
   static constexpr int further = 0;
   const char* at;
   int64_t stride;
-  int left;
-  __device__ __forceinline__ ColSource(const char* at, int k, int64_t stride) : at(at - kStepK * stride), stride(stride), left(k + kStepK) {}
-  __device__ __forceinline__ void next() { at += kStepK * stride, left -= kStepK; }
+  int left, k, turn;
+  // again: the rows are gone through a second time, behind whole steps
+  __device__ __forceinline__ ColSource(const char* at, int k, int64_t stride, bool again = false)
+      : at(at - kStepK * stride), stride(stride), left(k + kStepK), k(k), turn(again ? (k + kStepK - 1) / kStepK : -1) {}
+  __device__ __forceinline__ void next() {
+    at += kStepK * stride, left -= kStepK;
+    if (turn-- == 0) {
+      const int rows = (k + kStepK - 1) / kStepK * kStepK;
+      at -= rows * stride, left += rows;
+    }
+  }
   __device__ __forceinline__ i32x4 base(int) const { return resource_at(at); }
 };
 
@@ -232,7 +241,19 @@ struct TileProduct {
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * kCopies) : "memory");
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) read(now, 0, 0, u);
+    // Where registers are left, sums of four steps are added up, not one step to the sum of all before it: with few tokens one of them can make the whole
+    // loss, and its logit's rounding errors a large part of it.
+    constexpr bool kInTwo = STAGES > 2;
+    f32x4 total[kInTwo ? FL : 1][kInTwo ? FR : 1] = {};
+    auto add_up = [&] {
+#pragma unroll
+      for (int l = 0; l < FL; ++l)
+#pragma unroll
+        for (int r = 0; r < FR; ++r) total[l][r] += acc[l][r], acc[l][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
     for (int s = 0; s < steps; ++s) {
+      if constexpr (kInTwo)
+        if (s % 4 == 0) add_up();
 #pragma unroll
       for (int l = 0; l < FL; ++l) {
 #pragma unroll
@@ -254,6 +275,13 @@ struct TileProduct {
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup
+    if constexpr (kInTwo) {
+      add_up();
+#pragma unroll
+      for (int l = 0; l < FL; ++l)
+#pragma unroll
+        for (int r = 0; r < FR; ++r) acc[l][r] = total[l][r];
+    }
   }
 };
 

@@ -10,8 +10,14 @@
 //   tokens   a token's (m, sum) become its lse and loss, and its E becomes G in place: G = (E exp(m - lse) - [label]) g / max|g|;
 //   dx, dw   the two products, on G.  dx sums over the whole vocabulary: where its tiles do not fill the chip, that
 //            axis is cut and the parts are added by workgroups that dw's launch has more.
-// The 16-bit E and G are what the matrix cores take.  Both are rounded relative to their own size (bf16 2^-9 on average, as the outputs
-// are), with 2^15 as unit in fp16, so that probabilities down to 2^-29 are normal numbers; |g| is divided by its largest value for
+// Tokens whose label is ignored have rows of zeros in G.  With more than kWideTokens tokens they are left out: G, and a copy of x beside it, hold the others'
+// rows one behind the other, so that they cost nothing in the two products (of 8192 tokens x 131072 x 4096 with 15 % ignored: 20.4 -> 18.9 ms).  Their x is
+// never read for a gradient: the copy has zeros there, or nothing.
+// With few tokens, up to kWideTokens if they are few for each rank, memory and not the matrix cores sets the time, and nothing is lost to 16 bits on the way: the logits are kept in
+// 32 bits instead of E, and G is kept as two 16-bit numbers, itself rounded and what that left (16 bits of it in bf16, 22 in fp16).  The products take the second ones as
+// more rows.  (With so few tokens single values of G decide about a rank's dw, and some ranks hold no label: rounded once, dw was up to 1.9 times as far off as
+// with G in 32 bits.)  With more tokens E and G are both rounded, each relative to its own size (bf16 2^-9, fp16 2^-12 at the
+// most), with 2^15 as unit in fp16, so that probabilities down to 2^-29 are normal numbers; |g| is divided by its largest value for
 // the same reason and multiplied back in 32 bits behind the products.
 #include <hip/hip_runtime.h>
 
@@ -32,7 +38,8 @@ namespace {
 constexpr int kMaxRanks = MSCCLX_VOCAB_LOSS_MAX_RANKS;
 constexpr int kComputeUnits = 256;
 constexpr int kTile = 256;              // columns of G are padded to a multiple of it
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 1.0 / (double)kLog2e;  // what takes the rounded kLog2e back
 
 // The ranks' pieces of the vocabulary, passed to the kernels by value.  Units of kUnitRows rows; none spans two ranks, a tile may.
 // What pads a rank's last unit, or the last tile, counts as outside.
@@ -107,7 +114,8 @@ typedef Shape<128, 128, 2, 2, 2, 2> Middle;
 typedef Shape<128, 128, 2, 2, 1, 4> Thin;
 typedef Shape<128, 32, 4, 1, 4, 2> Few;
 
-enum { kStats = 0, kKeep = 1, kGradient = 2 };
+enum { kStats = 0, kKeep = 1, kGradient = 2, kLogits = 3 };
+constexpr int kWideTokens = 128;  // up to so many the logits are kept in 32 bits and G twice
 
 struct LogitsArgs {
   const char* x;
@@ -117,9 +125,10 @@ struct LogitsArgs {
   int64_t token0;    // of the labels, lse and factors
   Labels labels;
   Upstream upstream;
+  const int* pos;    // a token's row of E or G, -1: none; null: its own
   float2* stats;     // [tokens][waves' parts of the vocabulary]
   float* z_label;
-  void* e;           // [tokens][tiles * kTile]
+  void* e;           // [rows][tiles * kTile]: E or G, or with kLogits the logits in 32 bits
   const float* lse;
 };
 
@@ -183,7 +192,8 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
 #pragma unroll
       for (int j = 0; j < kWaveUnits; ++j) here |= label >= first[j] && label < first[j] + min(rows[j], kOfWave);
       const bool any = __any(here);  // one wave in hundreds holds a label of its tokens
-      T* out = (T*)a.e + (n0 + n) * ld + (int64_t)at * TL;
+      const int kept = (MODE == kKeep || MODE == kGradient) && live ? a.pos ? a.pos[a.token0 + n0 + n] : n0 + n : -1;
+      T* out = (T*)a.e + kept * ld + (int64_t)at * TL;
       // the wave's logits of the token, in fours: f(row in the unit, the unit's rows, the label's row in it, logits)
       auto each = [&](auto f) {
 #pragma unroll
@@ -202,9 +212,9 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
             const int v = Product::l_of(threadIdx.x, l + k), j = (l + k) / kUnitFragments;
             o[k] = f(v - part * kPart - j * kOfWave, rows[j], label - first[j], acc[l + k][r]);
           }
-          if (MODE != kStats) {
+          if (MODE == kKeep || MODE == kGradient) {
             const u32x4 row = Product::pair_up(o[0], o[1]);
-            if (live) *(u32x4*)(out + Product::l_of_pair(threadIdx.x, l)) = row;
+            if (kept >= 0) *(u32x4*)(out + Product::l_of_pair(threadIdx.x, l)) = row;
           }
         }
       };
@@ -236,6 +246,16 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
               if (here && row + i == want && row + i < rows) z_label = z[i], found = true;
           });
           if (found) a.z_label[a.token0 + n0 + n] = z_label;
+        }
+        if constexpr (MODE == kLogits) {
+#pragma unroll
+          for (int l = 0; l < Product::FL; ++l) {
+            const int v = Product::l_of(threadIdx.x, l), j = l / kUnitFragments, row = v - part * kPart - j * kOfWave;
+            f32x4 z;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] = WHOLE || row + i < rows[j] ? acc[l][r][i] : -INFINITY;  // padding: probability 0
+            if (live) *(f32x4*)((float*)a.e + (n0 + n) * ld + (int64_t)at * TL + v) = z;
+          }
         }
 #pragma unroll
         for (int d = 16; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
@@ -282,47 +302,91 @@ struct TokenArgs {
   const float* z_label;
   float *lse, *loss;
   void* e;
+  const float* logits;
+  const int* pos;
+  const char* x;
+  int64_t x_stride, dx_stride;
+  char *kept_x, *dx;   // [rows][hidden] for dw; and dx, where a token without a row has zeros
+  int hidden;
+  int tokens, second;  // kLogits: G's second rows begin at row `second`; rows between are zeros
+  int given;           // kLogits: the lse is an input
 };
 
-// A workgroup per token: its parts' (m, sum) -> lse and loss; KEEP: its E -> G in place.  Where tokens are few, several workgroups share one: each
-// works out the lse for itself (a thirtieth of what it then moves) and takes gridDim.y'ths of E.
-template <class T, bool KEEP>
+// A workgroup per token: its parts' (m, sum) -> lse and loss, and with gradients its row of x, and of G: kKeep from E, in place; kLogits from the logits; kGradient: G is
+// there and so is the lse.  Where tokens
+// are few, several workgroups share one: each works out the lse for itself (a thirtieth of what it then moves) and takes gridDim.y'ths of the row.
+// The label's own G = (p - 1) g comes from its logit in 32 bits: from a rounded p close to 1 next to nothing would be left of it.
+template <class T, int MODE>
 __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const TokenArgs a) {
   __shared__ float shared[4];
   const int64_t ld = (int64_t)pieces.tiles * kTile, at = a.token0 + blockIdx.x;
   const int parts = (int)(ld / a.part);
   const float2* stats = a.stats + (int64_t)blockIdx.x * parts;
-  float m = -INFINITY, sum = 0.f;
-  for (int h = threadIdx.x; h < parts; h += 256) m = fmaxf(m, stats[h].x);
-  m = block_reduce(m, [](float a, float b) { return fmaxf(a, b); }, shared);
-  const float base = m == -INFINITY ? 0.f : m;
-  for (int h = threadIdx.x; h < parts; h += 256) {
-    const float2 s = stats[h];
-    sum += s.y * exp2_of(s.x - base);
+  typedef typename Half<T>::x8 x8;
+  if (MODE == kLogits && (int)blockIdx.x >= a.tokens) {
+    for (int64_t v = (blockIdx.y * 256 + threadIdx.x) * 8; v < ld; v += gridDim.y * 256 * 8) *(x8*)((T*)a.e + blockIdx.x * ld + v) = x8{};
+    return;
   }
-  sum = block_reduce(sum, [](float a, float b) { return a + b; }, shared);
-  const float lse2 = base + log2f(sum), lse = lse2 * kLn2;
   const int label = a.labels.get(at);
-  if (threadIdx.x == 0 && blockIdx.y == 0) {
-    a.lse[at] = lse;
-    a.loss[at] = label == -1 ? 0.f : label < 0 ? NAN : lse - a.z_label[at];
+  const float z_label = label >= 0 ? a.z_label[at] : 0.f;
+  float base, log_sum = 0.f, m = -INFINITY;  // lse is their sum, in units of log 2
+  if (MODE == kGradient || (MODE == kLogits && a.given)) {
+    base = a.lse[at] * kLog2e;
+  } else {
+    float sum = 0.f;
+    for (int h = threadIdx.x; h < parts; h += 256) m = fmaxf(m, stats[h].x);
+    m = block_reduce(m, [](float a, float b) { return fmaxf(a, b); }, shared);
+    base = m == -INFINITY ? 0.f : m;
+    for (int h = threadIdx.x; h < parts; h += 256) {
+      const float2 s = stats[h];
+      sum += s.y * exp2_of(s.x - base);
+    }
+    sum = block_reduce(sum, [](float a, float b) { return a + b; }, shared);
+    log_sum = log2f(sum);
+    if (threadIdx.x == 0 && blockIdx.y == 0) {
+      // in 64 bits, each rounded once; the loss not from the rounded lse, whose error may be larger than a small loss
+      a.lse[at] = (float)(((double)base + log_sum) * kLn2);
+      a.loss[at] = label == -1 ? 0.f : label < 0 ? NAN : (float)(((double)base - (double)z_label * kLog2e + log_sum) * kLn2);
+    }
   }
-  if constexpr (KEEP) {
-    const float g = a.upstream.get(at, label);
+  if constexpr (MODE != kStats) {
+    const int row = a.pos ? a.pos[at] : (int)blockIdx.x;
+    for (int d = (blockIdx.y * 256 + threadIdx.x) * 8; d < a.hidden; d += gridDim.y * 256 * 8) {
+      if (row >= 0) *(x8*)(a.kept_x + ((int64_t)row * a.hidden + d) * 2) = label == -1 ? x8{} : *(const x8*)(a.x + blockIdx.x * a.x_stride + d * 2);
+      else *(x8*)(a.dx + blockIdx.x * a.dx_stride + d * 2) = x8{};
+    }
+    if (MODE == kGradient || row < 0) return;
+    const float g = a.upstream.get(at, label), lse2 = base + log_sum;
     int64_t want = -1;
+    float of_label = 0.f;
     if (label >= 0) {
       const int r = Ends(pieces.first + 1, pieces.ranks).rank_of(label);
       want = (int64_t)pieces.unit0[r] * kUnitRows + label - pieces.first[r];
+      of_label = expm1f((__builtin_fmaf(z_label, kLog2e, -base) - log_sum) * (float)kLn2) * g * kUnit<T>;
     }
-    typedef typename Half<T>::x8 x8;
-    T* e = (T*)a.e + blockIdx.x * ld;
+    T* e = (T*)a.e + row * ld;
     for (int64_t v = (blockIdx.y * 256 + threadIdx.x) * 8; v < ld; v += gridDim.y * 256 * 8) {
-      const float top = stats[v / a.part].x;
-      const float f = top == -INFINITY ? 0.f : exp2_of(top - lse2) * g;
-      x8 o = *(x8*)(e + v);
+      float p[8];
+      if constexpr (MODE != kLogits) {
+        const float top = stats[v / a.part].x;
+        const float f = top == -INFINITY ? 0.f : exp2_of(top - lse2) * g;
+        const x8 kept = *(const x8*)(e + v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = (T)(g == 0.f ? 0.f : (float)o[i] * f - (v + i == want ? kUnit<T> * g : 0.f));
+        for (int i = 0; i < 8; ++i) p[i] = (float)kept[i] * f;
+      } else {
+        const float* z = a.logits + blockIdx.x * ld + v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = exp2_of(__builtin_fmaf(z[i], kLog2e, -base) - log_sum) * (g * kUnit<T>);
+      }
+      x8 o, rest;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float whole = g == 0.f ? 0.f : v + i == want ? of_label : p[i];
+        o[i] = (T)whole;
+        rest[i] = (T)(whole - (float)o[i]);
+      }
       *(x8*)(e + v) = o;
+      if (MODE == kLogits) *(x8*)(e + a.second * ld + v) = rest;
     }
   }
 }
@@ -370,8 +434,43 @@ __device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shar
   }
   if (threadIdx.x == 0) *a.back = (float)((double)top / count / a.unit);
 }
-__global__ void __launch_bounds__(1024) sums_kernel(const SumsArgs a) {
+
+struct OrderArgs {
+  int64_t piece;  // tokens of a piece
+  int *pos, *idx;  // a token's row among its piece's, -1: ignored; and the token (in the piece) of a row
+  int* live;      // per piece: rows
+};
+
+// The rows of the tokens that are not ignored, in the tokens' order.
+__device__ __forceinline__ void order_tokens(const OrderArgs& o, int64_t tokens, const Labels& labels, int* shared) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  for (int64_t from = 0; from < tokens; from += o.piece) {
+    const int64_t to = min(from + o.piece, tokens);
+    int rows = 0;
+    for (int64_t c = from; c < to; c += blockDim.x) {
+      const int64_t n = c + threadIdx.x;
+      const bool keep = n < to && labels.get(n) != -1;
+      const unsigned long long kept = __ballot(keep);
+      if (lane == 0) shared[wave] = __popcll(kept);
+      __syncthreads();
+      int before = rows, all = 0;
+      for (int w = 0; w < waves; ++w) {
+        if (w < wave) before += shared[w];
+        all += shared[w];
+      }
+      before += __popcll(kept & ((1ull << lane) - 1));
+      if (n < to) o.pos[n] = keep ? before : -1;
+      if (keep) o.idx[from + before] = (int)(n - from);
+      rows += all;
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) o.live[from / o.piece] = rows;
+  }
+}
+
+__global__ void __launch_bounds__(1024) sums_kernel(const SumsArgs a, const OrderArgs o) {
   __shared__ double shared[16];
+  if (o.pos) order_tokens(o, a.tokens, a.labels, (int*)shared);
   sums_over_tokens(a, shared);
 }
 
@@ -409,12 +508,16 @@ struct PieceSource {
 static_assert(kUnitRows == kStepK, "a step of dx's product is a unit");
 
 struct GradArgs {
-  const void* g;     // [tokens][tiles * kTile]
-  const char* x;
+  const void* g;     // [rows][tiles * kTile]
+  const char* x;     // [rows][hidden]
+  const int *live, *idx;  // rows, and a row's token; null: all tokens, in order
+  Labels labels;
+  int64_t token0;
   int64_t x_stride, w_stride;
   int hidden, tokens, token_tiles, hidden_tiles;
+  int second, rows;  // G's second rows begin at row `second` (0: there are none); rows of G in all
   int split_steps;   // dx: steps of kStepK for each part of the vocabulary
-  float* parts;      // dx: [parts][tokens][hidden]; null: one part
+  float* parts;      // dx: [parts][rows][hidden]; null: dx itself is written
   int count;         // of parts
   int with_sums;     // dx: one workgroup more, for the sums over tokens
   int adders;        // dw: so many workgroups more, in front, that add dx's parts
@@ -441,9 +544,11 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dx_kernel(cons
     if (blockIdx.y == 0) sums_over_tokens(sums, (double*)smem);
     return;
   }
+  const int all = a.live ? *a.live : a.rows, token_tiles = (all + TR - 1) / TR;
+  if ((int)blockIdx.x >= token_tiles * a.hidden_tiles) return;
   int tt, ht;
-  tile_of(blockIdx.x, a.token_tiles, a.hidden_tiles, &tt, &ht);
-  const int n0 = tt * TR, d0 = ht * TL, tokens = min(TR, a.tokens - n0), width = min(TL, a.hidden - d0);
+  tile_of(blockIdx.x, token_tiles, a.hidden_tiles, &tt, &ht);
+  const int n0 = tt * TR, d0 = ht * TL, tokens = min(TR, all - n0), width = min(TL, a.hidden - d0);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
   const int step0 = blockIdx.y * a.split_steps, steps = min(a.split_steps, pieces.tiles * (kTile / kStepK) - step0);
   f32x4 acc[Product::FL][Product::FR] = {};
@@ -463,14 +568,15 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dx_kernel(cons
 #pragma unroll
       for (int l = 0; l < Product::FL; ++l) {
         const int d = Product::l_of(threadIdx.x, l);
-        if (n < tokens && d < width) *(f32x4*)(a.parts + ((int64_t)blockIdx.y * a.tokens + n0 + n) * a.hidden + d0 + d) = acc[l][r];
+        if (n < tokens && d < width) *(f32x4*)(a.parts + ((int64_t)blockIdx.y * a.rows + n0 + n) * a.hidden + d0 + d) = acc[l][r];
       }
     } else {
+      const int64_t token = a.live && n < tokens ? a.idx[n0 + n] : n0 + n;
 #pragma unroll
       for (int l = 0; l < Product::FL; l += 2) {
         const u32x4 row = Product::pair_up(narrow<T>(acc[l][r], back), narrow<T>(acc[l + 1][r], back));
         const int d = Product::l_of_pair(threadIdx.x, l);
-        if (n < tokens && d < width) *(u32x4*)(a.dx + (n0 + n) * a.dx_stride + (d0 + d) * 2) = row;
+        if (n < tokens && d < width) *(u32x4*)(a.dx + token * a.dx_stride + (d0 + d) * 2) = row;
       }
     }
   }
@@ -478,13 +584,20 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dx_kernel(cons
 
 // dx from the parts of the vocabulary: four values per thread and turn
 template <class T> __device__ __forceinline__ void add_parts(const GradArgs& a) {
-  const int64_t size = (int64_t)a.tokens * a.hidden;
+  const int64_t size = (int64_t)(a.live ? *a.live : a.tokens) * a.hidden;
   const float back = *a.back;
   for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4; i < size; i += (int64_t)a.adders * blockDim.x * 4) {
-    f32x4 sum = {};
+    f32x4 sum = {}, rest = {};
+    const float* from = a.parts + i;
 #pragma unroll 8
-    for (int p = 0; p < a.count; ++p) sum += *(const f32x4*)(a.parts + p * size + i);
-    *(typename Half<T>::x4*)(a.dx + i / a.hidden * a.dx_stride + i % a.hidden * 2) = narrow<T>(sum, back);
+    for (int p = 0; p < a.count; ++p, from += (int64_t)a.rows * a.hidden) {
+      sum += *(const f32x4*)from;
+      if (a.second) rest += *(const f32x4*)(from + (int64_t)a.second * a.hidden);
+    }
+    sum += rest;
+    const int64_t row = i / a.hidden, token = a.live ? a.idx[row] : row;
+    if (!a.live && a.labels.get(a.token0 + token) == -1) sum = f32x4{0.f, 0.f, 0.f, 0.f};  // (zero times what W holds may be no zero)
+    *(typename Half<T>::x4*)(a.dx + token * a.dx_stride + i % a.hidden * 2) = narrow<T>(sum, back);
   }
 }
 
@@ -502,10 +615,12 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dw_kernel(cons
   {
     typename Product::LLanes ll;
     typename Product::RLanes rl;
-    ll.place(threadIdx.x, a.x_stride, [&](int) { return width; });
+    // x's rows once more for G's second rows: within a step, or behind the steps of the first
+    ll.place(threadIdx.x, a.x_stride, [&](int) { return width; }, a.second && a.second < kStepK ? a.second : kStepK);
     rl.place(threadIdx.x, ld * 2, [&](int) { return TR; });
-    Product::run(smem, (a.tokens + kStepK - 1) / kStepK, ll, ColSource(a.x + d0 * 2, a.tokens, a.x_stride), rl,
-                 ColSource((const char*)a.g + (int64_t)at * TR * 2, a.tokens, ld * 2), acc);
+    const int all = a.live ? *a.live : a.rows;
+    Product::run(smem, (all + kStepK - 1) / kStepK, ll, ColSource(a.x + d0 * 2, a.live ? all : a.tokens, a.x_stride, a.second >= kStepK), rl,
+                 ColSource((const char*)a.g + (int64_t)at * TR * 2, all, ld * 2), acc);
   }
   static_assert(TR / Shape::kWavesR == kUnitRows, "a wave's rows are a unit");
   const int unit0 = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) / Shape::kWavesL);
@@ -549,7 +664,7 @@ struct mscclx_vocab_loss {
   Pieces pieces;          // without pointers
   int64_t vocab = 0;
   int64_t piece = 0;      // tokens per piece
-  uint64_t off_z = 0, off_loss = 0, off_factor = 0, off_back = 0, off_stats = 0, off_e = 0, off_sums = 0, off_parts = 0, bytes = 0;
+  uint64_t off_z = 0, off_loss = 0, off_factor = 0, off_back = 0, off_stats = 0, off_e = 0, off_sums = 0, off_parts = 0, off_logits = 0, off_x = 0, off_pos = 0, off_idx = 0, off_live = 0, bytes = 0;
 };
 
 namespace {
@@ -577,9 +692,11 @@ struct Call {
   Pieces pieces;
   Grads grads;
   Labels labels;
-  float *z_label, *row_loss, *factor, *back, *sums, *parts;
+  float *z_label, *row_loss, *factor, *back, *sums, *parts, *logits;
   float2* stats;
   void* e;
+  char* x;
+  OrderArgs order;
 };
 
 int check_call(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool forward, bool backward, Call* c) {
@@ -622,6 +739,9 @@ int check_call(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool 
   c->stats = (float2*)(ws + h->off_stats);
   c->e = ws + h->off_e;
   c->parts = (float*)(ws + h->off_parts);
+  c->logits = (float*)(ws + h->off_logits);
+  c->x = ws + h->off_x;
+  c->order = OrderArgs{h->piece, (int*)(ws + h->off_pos), (int*)(ws + h->off_idx), (int*)(ws + h->off_live)};
   c->sums = h->off_sums ? (float*)(ws + h->off_sums) : nullptr;
   return MSCCLX_OK;
 }
@@ -642,12 +762,16 @@ int logits_shape(const Pieces& p, int64_t tokens) {
 // shorter than Middle.
 int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 384 ? kThin : (int64_t)p.tiles * tiles(hidden) < kComputeUnits ? kMiddle : kLarge; }
 
+// Where G's second rows begin, so that no step of dw's product and no tile of dx's has more of them than need be; rows behind the first ones are zeros.
+int second_row(int64_t tokens) { return tokens <= 16 ? 16 : tokens <= 32 ? 32 : (int)((tokens + kStepK - 1) / kStepK * kStepK); }
+
 // dx: into how many parts the vocabulary is cut so that the tiles fill the chip, of at least eight steps each (with four, 1024 x 4096 x 512 takes 5 us
 // longer).  Few as long as reading W again for every 32 tokens costs little (128 x 8192 x 1024: 3 us shorter than Middle; 40 x 65536 x 4096: 26 us longer).
 struct DxPlan {
   int shape, token_tiles, hidden_tiles, parts, split_steps;
+  bool separate;  // the parts are kept and added
 };
-DxPlan dx_plan(const Pieces& p, int64_t tokens, int hidden) {
+DxPlan dx_plan(const Pieces& p, int64_t tokens, int hidden, bool separate) {
   DxPlan d;
   const int steps = p.tiles * (kTile / kStepK);
   const int64_t again = (int64_t)(tiles(tokens, Few::kR) - 1) * p.tiles * kTile * hidden * 2;
@@ -659,6 +783,7 @@ DxPlan dx_plan(const Pieces& p, int64_t tokens, int hidden) {
   const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, slots / ((int64_t)d.token_tiles * d.hidden_tiles)));
   d.split_steps = (steps + parts - 1) / parts;
   d.parts = (steps + d.split_steps - 1) / d.split_steps;
+  d.separate = separate || d.parts > 1;
   return d;
 }
 
@@ -681,18 +806,20 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
   const int mean = d.reduction == MSCCLX_LOSS_MEAN, per_token = d.reduction == MSCCLX_LOSS_NONE;
   const Upstream upstream = {io->grad_loss, per_token ? c.factor : nullptr};
   int rc;
-  // The sums over tokens.  One number: with the losses, behind the last piece's tokens and in front of its gradients (or beside them: dx's
-  // parts do without); else first of all.
-  SumsArgs totals = {n, c.labels, mean, forward && !per_token ? c.row_loss : nullptr, io->loss, backward ? io->grad_loss : nullptr, per_token ? c.factor : nullptr,
-                     kUnit<T>, c.back};
-  auto sums = [&](bool losses) {
-    SumsArgs now = totals;
-    if (!losses) now.rows = nullptr;
-    hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, stream, now);
+  // Twice where that decides about a rank's dw: with few tokens, or few for each rank
+  const bool wide = backward && (n <= 32 || (n <= kWideTokens && n < 16 * d.ranks));
+  // The sums over tokens: for the gradients in front of everything, unless that is one number and nothing in front of the products asks for it; for the loss as one
+  // number behind the last piece's tokens (beside its gradients, where dx has parts).
+  // Up to kWideTokens tokens, rows of zeros cost less than the launch that finds out which they are
+  const bool ordered = backward && n > kWideTokens;
+  const bool early = backward && (per_token || !forward || ordered);
+  SumsArgs first = {n, c.labels, mean, nullptr, nullptr, io->grad_loss, per_token ? c.factor : nullptr, kUnit<T>, c.back};
+  SumsArgs totals = {n, c.labels, mean, forward && !per_token ? c.row_loss : nullptr, io->loss, backward && !early ? io->grad_loss : nullptr, nullptr, kUnit<T>, c.back};
+  auto sums = [&](const SumsArgs& what, const OrderArgs& order) {
+    hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, stream, what, order);
     return launched("sums_kernel");
   };
-  const bool early = backward && (per_token || !forward || n > h->piece);
-  if (early && (rc = sums(false))) return rc;
+  if (early && (rc = sums(first, ordered ? c.order : OrderArgs{}))) return rc;
   const int64_t all = std::max<int64_t>(n, backward ? 1 : 0);  // no tokens: dw is still written, with zeros
   for (int64_t at = 0; at < all; at += h->piece) {
     const int now = (int)std::min(h->piece, n - at);
@@ -706,42 +833,61 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
     a.token0 = at;
     a.labels = c.labels;
     a.upstream = upstream;
+    a.pos = ordered ? c.order.pos : nullptr;
     a.stats = c.stats;
     a.z_label = c.z_label;
     a.e = c.e;
     a.lse = io->lse;
     if (now > 0) {
       const int shape = logits_shape(p, now);
-      if ((rc = !forward ? launch_logits<T, kGradient>(shape, p, a, stream) : backward ? launch_logits<T, kKeep>(shape, p, a, stream) : launch_logits<T, kStats>(shape, p, a, stream)))
+      if (wide) a.e = c.logits;
+      if ((rc = wide ? launch_logits<T, kLogits>(shape, p, a, stream) : !forward ? launch_logits<T, kGradient>(shape, p, a, stream) : backward ? launch_logits<T, kKeep>(shape, p, a, stream) : launch_logits<T, kStats>(shape, p, a, stream)))
         return rc;
-      if (forward) {
-        TokenArgs t = {};
-        t.stats = c.stats;
-        t.part = shape == kLarge ? Large::kL / Large::kWavesL : shape == kMiddle ? Middle::kL / Middle::kWavesL : Few::kL / Few::kWavesL;
-        t.token0 = at;
-        t.labels = c.labels;
-        t.upstream = upstream;
-        t.z_label = c.z_label;
-        t.lse = io->lse;
-        t.loss = c.row_loss;
-        t.e = c.e;
-        const unsigned slices = (unsigned)std::max(1, std::min(4 * kComputeUnits / now, p.tiles * kTile / 4096));
-        if (backward) hipLaunchKernelGGL((token_kernel<T, true>), dim3(now, slices), dim3(256), 0, stream, p, t);
-        else hipLaunchKernelGGL((token_kernel<T, false>), dim3(now), dim3(256), 0, stream, p, t);
-        if ((rc = launched("token_kernel"))) return rc;
-      }
+      TokenArgs t = {};
+      t.stats = c.stats;
+      t.part = shape == kLarge ? Large::kL / Large::kWavesL : shape == kMiddle ? Middle::kL / Middle::kWavesL : Few::kL / Few::kWavesL;
+      t.token0 = at;
+      t.labels = c.labels;
+      t.upstream = upstream;
+      t.z_label = c.z_label;
+      t.lse = io->lse;
+      t.loss = c.row_loss;
+      t.e = c.e;
+      t.logits = c.logits;
+      t.pos = a.pos;
+      t.x = a.x;
+      t.x_stride = a.x_stride;
+      t.kept_x = c.x;
+      t.dx = (char*)io->dx + at * io->dx_stride * 2;
+      t.dx_stride = io->dx_stride * 2;
+      t.hidden = d.hidden;
+      t.tokens = now;
+      t.second = second_row(now);
+      t.given = !forward;
+      const unsigned slices = (unsigned)std::max(1, std::min(4 * kComputeUnits / now, p.tiles * kTile / 4096));
+      if (wide) hipLaunchKernelGGL((token_kernel<T, kLogits>), dim3(t.second, slices), dim3(256), 0, stream, p, t);
+      else if (!forward) hipLaunchKernelGGL((token_kernel<T, kGradient>), dim3(now), dim3(256), 0, stream, p, t);
+      else if (backward) hipLaunchKernelGGL((token_kernel<T, kKeep>), dim3(now, slices), dim3(256), 0, stream, p, t);
+      else hipLaunchKernelGGL((token_kernel<T, kStats>), dim3(now), dim3(256), 0, stream, p, t);
+      if ((rc = launched("token_kernel"))) return rc;
     }
     const bool behind = last && forward && !per_token;  // the sums come now
-    const DxPlan plan = backward && now > 0 ? dx_plan(p, now, d.hidden) : DxPlan{};
-    if (behind && plan.parts <= 1 && (rc = sums(true))) return rc;
+    const int second = wide && now > 0 ? second_row(now) : 0, rows = second + now;
+    const DxPlan plan = backward && now > 0 ? dx_plan(p, rows, d.hidden, !ordered) : DxPlan{};
+    if (behind && !plan.separate && (rc = sums(totals, OrderArgs{}))) return rc;
     if (!backward) continue;
     GradArgs g = {};
     g.g = c.e;
-    g.x = a.x;
-    g.x_stride = a.x_stride;
+    g.x = c.x;
+    g.x_stride = (int64_t)d.hidden * 2;
+    if (ordered) g.live = c.order.live + at / h->piece, g.idx = c.order.idx + at;
+    g.labels = c.labels;
+    g.token0 = at;
     g.w_stride = a.w_stride;
     g.hidden = d.hidden;
     g.tokens = now;
+    g.second = second;
+    g.rows = rows;
     g.dx = (char*)io->dx + at * io->dx_stride * 2;
     g.dx_stride = io->dx_stride * 2;
     g.dw_stride = io->dweight_stride * 2;
@@ -753,7 +899,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
       g.token_tiles = plan.token_tiles;
       g.hidden_tiles = plan.hidden_tiles;
       g.split_steps = plan.split_steps;
-      g.parts = plan.parts > 1 ? c.parts : nullptr;
+      g.parts = plan.separate ? c.parts : nullptr;
       g.count = plan.parts;
       g.with_sums = g.parts && behind;
       auto go = [&](auto s) {
@@ -773,7 +919,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
     const int shape = dw_shape(p, now, d.hidden);
     if ((rc = shape == kLarge ? go(Large()) : shape == kMiddle ? go(Middle()) : go(Thin()))) return rc;
   }
-  if (n == 0 && forward && !per_token && !backward) return sums(true);
+  if (n == 0 && forward && !per_token && !backward) return sums(totals, OrderArgs{});
   return MSCCLX_OK;
 }
 
@@ -841,15 +987,22 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
     h->off_z = take(n * 4);
     h->off_loss = take(n * 4);
     h->off_factor = take(n * 4);
+    h->off_pos = take(n * 4);
+    h->off_idx = take(n * 4);
+    h->off_live = take((n / h->piece + 1) * 4);
+    h->off_x = d.gradients ? take((uint64_t)h->piece * d.hidden * 2) : 0;
     const uint64_t wide = (uint64_t)p.tiles * kTile;
     h->off_stats = take(std::max(std::min<uint64_t>(h->piece, 256) * (wide / (Few::kL / Few::kWavesL)), (uint64_t)h->piece * (wide / (Middle::kL / Middle::kWavesL))) * sizeof(float2));
-    h->off_e = d.gradients ? take((uint64_t)h->piece * row) : 0;
+    h->off_logits = d.gradients ? take(std::min<uint64_t>(n, kWideTokens) * wide * 4) : 0;
+    h->off_e = d.gradients ? take(std::max<uint64_t>(h->piece, std::min<uint64_t>(n, kWideTokens) + kWideTokens) * row) : 0;
     h->off_sums = d.gradients && d.max_tokens > h->piece ? take((uint64_t)p.tiles * kTile * d.hidden * 4) : 0;
-    uint64_t parts = 0;  // dx's parts at the token count that needs most of them; its plan is the same for (32 k, 32 k + 32] tokens
-    for (int64_t t = 0; d.gradients && t < h->piece; t += Few::kR) {
-      const DxPlan plan = dx_plan(p, t + 1, d.hidden);
-      if (plan.parts > 1) parts = std::max(parts, (uint64_t)plan.parts * std::min<int64_t>(h->piece, t + Few::kR) * d.hidden * 4);
-    }
+    uint64_t parts = 0;  // dx's parts at the token count that needs most of them
+    auto need = [&](int64_t rows, bool separate) {
+      const DxPlan plan = dx_plan(p, rows, d.hidden, separate);
+      if (plan.separate) parts = std::max(parts, (uint64_t)plan.parts * rows * d.hidden * 4);
+    };
+    for (int64_t t = 1; d.gradients && t <= std::min<int64_t>(h->piece, kWideTokens); ++t) need(t, true), need(second_row(t) + t, true);
+    for (int64_t t = 32; d.gradients && t - 31 <= h->piece; t += 32) need(std::min(t, h->piece), false);  // (the plan is the same from t - 31 on)
     h->off_parts = take(parts);
     h->bytes = at;
     if (workspace_bytes) *workspace_bytes = at;

@@ -49,7 +49,7 @@ def check_all(op, x, weights, labels, upstream, reduction):
 
 CASES = [  # tokens, hidden, rows
     (1, 8, [1]), (1, 64, [5, 3]), (2, 16, [0, 2, 0]), (3, 72, [257, 0, 255]), (16, 128, [128, 128]), (17, 64, [129]), (31, 200, [513, 31]),
-    (64, 256, [300] * 5), (65, 64, [64] * 9), (255, 248, [256, 256]), (256, 256, [256]), (257, 264, [300]), (300, 136, [256, 1, 511]), (129, 1032, [640]),
+    (64, 256, [300] * 5), (65, 64, [64] * 9), (255, 248, [256, 256]), (256, 256, [256]), (257, 264, [300]), (33, 64, [200, 57]), (48, 64, [100] * 3), (100, 136, [40] * 8), (128, 64, [31] * 10), (129, 64, [31] * 10), (300, 136, [256, 1, 511]), (129, 1032, [640]),
     (48, 64, [33] * 64), (70, 64, [1] * 64), (300, 72, [65, 0, 190, 64, 63, 2, 0, 321]), (5, 64, [0, 0, 7]), (260, 328, [64, 64, 127, 1])]
 
 
@@ -63,11 +63,11 @@ def test_against_the_64_bit_form(tokens, hidden, rows, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["none", "mean"])
-@pytest.mark.parametrize("tokens", [256, 257, 512, 700])
+@pytest.mark.parametrize("tokens", [129, 256, 257, 512, 700])
 def test_several_pieces_of_tokens(tokens, reduction, dtype):
     rows = [300, 200]
     op = operator(tokens, 128, rows, dtype, reduction=reduction, piece_bytes=1)
-    assert op.piece_tokens == 256
+    assert op.piece_tokens == min(256, tokens)
     check_all(op, *make(tokens, 128, rows, DTYPES[dtype], seed=5), reduction)
 
 
@@ -105,6 +105,35 @@ def test_strides_labels_of_32_bits_and_what_lies_beside(dtype):
     for b in [dx, *dw]:  # nothing is written around the rows
         inner(b).fill_(float("nan"))
         assert bool(torch.isnan(b).all())
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("tokens, rows", [(9, [100, 30]), (30, [257]), (90, [64] * 9), (140, [100, 30]), (600, [300, 500])])
+def test_what_stands_in_ignored_tokens_reaches_nothing(tokens, rows, reduction):
+    """Padding holds anything: NaN and infinities there change no loss and no gradient, and its own dx is 0, also where W holds infinities."""
+    x, weights, labels, upstream = make(tokens, 72, rows, torch.bfloat16, ignored=0.4)
+    labels[0], labels[-1] = IGNORE, IGNORE
+    up = upstream if reduction == "none" else torch.tensor(0.7, device="cuda")
+    op = operator(tokens, 72, rows, "bfloat16", reduction=reduction, piece_bytes=1)
+    clean = op.run(x, weights, labels, up)
+    bad = x.clone()
+    gone = labels == IGNORE
+    values = torch.tensor([float("nan"), float("inf"), float("-inf"), 3e38], dtype=torch.bfloat16, device="cuda")
+    bad[gone] = values[torch.arange(int(gone.sum()), device="cuda") % 4].unsqueeze(1)
+    for way in ("run", "backward"):
+        if way == "run":
+            loss, _, dx, dw = op.run(bad, weights, labels, up)
+            assert torch.equal(loss, clean[0])
+        else:
+            dx, dw = op.backward(bad, weights, labels, clean[1], up)
+        assert float(dx[gone].abs().sum()) == 0
+        if way == "run":
+            assert torch.equal(dx, clean[2]) and all(torch.equal(a, b) for a, b in zip(dw, clean[3]))
+        else:
+            assert bool(torch.isfinite(dx).all()) and all(bool(torch.isfinite(t).all()) for t in dw)
+    weights[0][0, 5] = float("inf")
+    _, _, dx, _ = op.run(x, weights, labels, up)
+    assert float(dx[gone].abs().sum()) == 0
 
 
 def test_labels_outside_the_vocabulary():
