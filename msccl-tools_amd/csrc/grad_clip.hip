@@ -314,14 +314,17 @@ int mscclx_grad_clip_bind(mscclx_grad_clip* h, const void* const* in, void* cons
     }
     char* ws = (char*)workspace;
     hipStream_t s = (hipStream_t)stream;
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &capturing) != hipSuccess || capturing != hipStreamCaptureStatusNone) {
+      (void)hipGetLastError();
+      return fail(MSCCLX_ERR_STATE, "tensors are bound before a stream is captured, not meanwhile");
+    }
+    h->workspace = nullptr;  // (until the new table is there)
     const Header zeros = {};
     hipError_t e = hipMemcpyAsync(ws, &zeros, sizeof(Header), hipMemcpyHostToDevice, s);
     if (e == hipSuccess && !chunks.empty()) e = hipMemcpyAsync(ws + h->off_chunks, chunks.data(), chunks.size() * sizeof(Chunk), hipMemcpyHostToDevice, s);
     if (e == hipSuccess) e = hipStreamSynchronize(s);
-    if (e != hipSuccess) {
-      h->workspace = nullptr;
-      return fail(MSCCLX_ERR_HIP, std::string("uploading the table of gradients: ") + hipGetErrorString(e));
-    }
+    if (e != hipSuccess) return fail(MSCCLX_ERR_HIP, std::string("uploading the table of gradients: ") + hipGetErrorString(e));
     h->workspace = ws;
     h->outputs = out != nullptr;
     return (int)MSCCLX_OK;

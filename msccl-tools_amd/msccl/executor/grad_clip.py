@@ -17,7 +17,10 @@ NORM_CODES = {"l2": 0, "max": 1}
 
 
 class GradientClip:
-    """clip = GradientClip(); clip.setup(sizes, dtype); clip.bind(gradients); clip.launch(max_norm=1.0); clip.norm"""
+    """clip = GradientClip(); clip.setup(sizes, dtype); clip.bind(gradients, gradients); clip.launch(max_norm=1.0); clip.norm
+
+    norm = |scale| sqrt(sum g^2) or |scale| max |g|;  out = g scale min(1, max_norm / (norm + 1e-6)).  launch() only enqueues kernels and can be captured in
+    a HIP graph, which needs binding and handle as they were at its capture; launches of one handle follow each other on one stream, or are ordered by events."""
 
     def __init__(self, device="cuda:0"):
         self.device = torch.device(device)
@@ -58,6 +61,7 @@ class GradientClip:
             n, array(ctypes.c_uint64, sizes), *(array(ctypes.c_int32, [DTYPE_CODES[d] for d in names]) for names in codes),
             None if counted is None else array(ctypes.c_uint8, [int(bool(c)) for c in counted]), NORM_CODES[norm], ctypes.byref(handle), ctypes.byref(nbytes)))
         self.close()
+        self._workspace = None   # (until the new one is there no call is let through)
         self.handle = handle
         self.sizes, self.dtypes, self.out_dtypes, self.workspace_bytes = sizes, codes[0], codes[1], nbytes.value
         self._keepalive = None

@@ -1,7 +1,7 @@
 """Softmax cross entropy over a vocabulary that is cut into the ranks' pieces, with its gradients.
 
 The output layer of a model whose vocabulary the ranks share: rank r holds rows of the output matrix, the softmax's maximum
-and sum are taken over all ranks' pieces.  The logits are never kept (kernels in csrc/vocab_loss.hip).
+and sum are taken over all ranks' pieces.  The logits of more than a few tokens are never kept (kernels in csrc/vocab_loss.hip).
 """
 from __future__ import annotations
 
@@ -20,7 +20,10 @@ class VocabLoss:
     """loss = VocabLoss(); loss.setup(tokens, hidden, rank_rows, dtype); loss.run(x, weights, labels).
 
     With z = x @ cat(weights).T: lse = logsumexp(z), loss = lse - z[label]; tokens whose label is `ignore_index` have loss 0
-    and no gradient, a label outside the vocabulary makes loss and gradients NaN."""
+    and no gradient, a label outside the vocabulary makes loss and gradients NaN.
+
+    Calls only enqueue kernels on the current stream and can be captured in a HIP graph, which needs the handle as it was at its capture.  A handle has one
+    workspace: its calls follow each other on one stream, or are ordered by events, and come from one thread at a time."""
 
     def __init__(self, device="cuda:0"):
         self.device = torch.device(device)
@@ -51,6 +54,7 @@ class VocabLoss:
         handle, nbytes, piece = ctypes.c_void_p(), ctypes.c_uint64(), ctypes.c_int64()
         binding._check(self.lib, self.lib.mscclx_vocab_loss_create(ctypes.byref(desc), ctypes.byref(handle), ctypes.byref(nbytes), ctypes.byref(piece)))
         self.close()
+        self._workspace = None   # (until the new one is there no call is let through)
         self.handle = handle
         self.tokens, self.hidden, self.rank_rows, self.reduction = int(tokens), int(hidden), rows, reduction
         self.dtype = {"bfloat16": torch.bfloat16, "float16": torch.float16}[name]

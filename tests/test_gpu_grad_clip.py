@@ -134,6 +134,34 @@ def test_same_bits_another_stream_and_a_replayed_graph():
         assert torch.equal(norm, clip.norm) and all(torch.equal(a, b) for a, b in zip(want, outs))
 
 
+def test_bound_again_and_set_up_again():
+    """The newest binding counts, also after one that was refused; a graph's binding is not made while it is captured."""
+    from msccl.executor import GradientClip, MscclxError
+    clip = GradientClip()
+    clip.setup([1000], "float32")
+    a, b, out = torch.full((1000,), 2.0, device="cuda"), torch.full((1000,), 3.0, device="cuda"), torch.empty(1000, device="cuda")
+    for g in (a, b, a):
+        assert float(clip.run([g], [out], max_norm=1.0)) == pytest.approx(float(g.square().sum().sqrt()), rel=1e-6)
+        with pytest.raises(ValueError):
+            clip.bind([g[:10]], [out])
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        clip.launch(max_norm=2.0)
+        with pytest.raises(MscclxError, match="STATE"):
+            clip.bind([b], [out])
+    with pytest.raises(RuntimeError, match="bind"):
+        clip.launch()
+    clip.bind([a], [out])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(out.square().sum().sqrt()) == pytest.approx(2.0, rel=1e-5)
+    clip.setup([10, 20], "float16")
+    with pytest.raises(RuntimeError, match="bind"):
+        clip.launch()
+    assert float(clip.run([torch.ones(10, dtype=torch.half, device="cuda"), torch.zeros(20, dtype=torch.half, device="cuda")])) == pytest.approx(10 ** 0.5, rel=1e-6)
+
+
 def test_refusals_of_tensors():
     from msccl.executor import GradientClip, MscclxError
     clip = GradientClip()

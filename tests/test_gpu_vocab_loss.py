@@ -264,6 +264,16 @@ def test_another_stream_and_a_replayed_graph():
         assert torch.equal(eager[2], ref[2])
 
 
+def test_set_up_again():
+    op = operator(40, 64, [100, 30], "bfloat16", reduction="none")
+    check_all(op, *make(40, 64, [100, 30], torch.bfloat16), "none")
+    op.setup(300, 136, [70, 0, 400, 9], "float16", reduction="sum")
+    check_all(op, *make(300, 136, [70, 0, 400, 9], torch.float16), "sum")
+    op.setup(10, 64, [100], "float16", reduction="mean", gradients=False)
+    x, weights, labels, upstream = make(10, 64, [100], torch.float16)
+    check("loss", op.forward(x, weights, labels)[0], loss_forms(x, weights, labels, "mean", IGNORE, 1.0)["loss"])
+
+
 def test_refusals_of_tensors():
     op = operator(40, 64, [100, 30], "bfloat16", reduction="mean")
     x, weights, labels, upstream = make(40, 64, [100, 30], torch.bfloat16)
