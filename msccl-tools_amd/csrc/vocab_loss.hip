@@ -110,6 +110,9 @@ template <int L, int R, int WL, int WR, int STAGES, int WAVES> struct Shape {  /
   template <class T, bool LCOL, bool RCOL> using Product = TileProduct<T, L, R, WL, WR, STAGES, LCOL, RCOL>;
 };
 typedef Shape<256, 256, 2, 4, 2, 2> Large;
+// dx's l is W^T, whose fragments take two reads of shared memory and r's one: with 4 x 2 waves each takes half as many
+// of them.  At 8192 tokens of 4096 and 32768 rows dx takes 1547 us, with 2 x 4 waves 1577.
+typedef Shape<256, 256, 4, 2, 2, 2> LargeDx;
 typedef Shape<128, 128, 2, 2, 2, 2> Middle;
 typedef Shape<128, 128, 2, 2, 1, 4> Thin;
 typedef Shape<128, 32, 4, 1, 4, 2> Few;
@@ -133,11 +136,13 @@ struct LogitsArgs {
 };
 
 // Tiles in an order that keeps the workgroups of one XCD (every eighth of the grid) on neighbouring tiles: columns of
-// up to eight row tiles share what they read.
+// up to kBand row tiles share what they read.  Of 8, 4 and 2, at 8192 tokens of 4096 and 32768 rows: logits kept 1697,
+// 1651 and 1690 us, not kept 1522, 1511 and 1571; dx 1597, 1577 and 1578; dw 1622, 1607 and 1632.
+constexpr int kBand = 4;
 __device__ __forceinline__ void tile_of(int id, int rows, int cols, int* row, int* col) {
   const int total = rows * cols, per = total / 8;
   if (id < per * 8) id = id % 8 * per + id / 8;
-  const int band = 8 * cols, at = id / band * 8, high = min(8, rows - at), in = id % band;
+  const int band = kBand * cols, at = id / band * kBand, high = min(kBand, rows - at), in = id % band;
   *row = at + in % high;
   *col = in / high;
 }
@@ -907,7 +912,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
         hipLaunchKernelGGL((dx_kernel<T, S>), dim3((unsigned)(g.token_tiles * g.hidden_tiles + g.with_sums), plan.parts), dim3(S::kThreads), 0, stream, p, g, totals);
         return launched("dx_kernel");
       };
-      if ((rc = plan.shape == kLarge ? go(Large()) : plan.shape == kMiddle ? go(Middle()) : go(Few()))) return rc;
+      if ((rc = plan.shape == kLarge ? go(LargeDx()) : plan.shape == kMiddle ? go(Middle()) : go(Few()))) return rc;
     }
     auto go = [&](auto s) {
       typedef decltype(s) S;
