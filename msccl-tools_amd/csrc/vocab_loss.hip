@@ -417,7 +417,10 @@ __device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shar
     const int label = a.labels.get(n);
     count += label != -1;
     if (a.rows) sum += a.rows[n];
-    if (a.factor && label >= 0) top = fmaxf(top, fabsf(a.upstream[n]));
+    if (a.factor && label >= 0) {  // an infinite one is its token's own affair
+      const float g = fabsf(a.upstream[n]);
+      if (g < INFINITY) top = fmaxf(top, g);
+    }
   }
   auto add = [](double a, double b) { return a + b; };
   if (a.mean) count = fmax(block_reduce(count, add, shared), 1.0);

@@ -197,6 +197,24 @@ def test_upstream_of_any_size(scale):
     check("dw", torch.cat(dw), forms["dw"])
 
 
+@pytest.mark.parametrize("tokens, rows", [(20, [100, 30]), (100, [257]), (300, [300, 77])])
+@pytest.mark.parametrize("value", ["inf", "-inf", "nan"])
+def test_a_non_finite_upstream_spoils_no_other_token(tokens, rows, value):
+    x, weights, labels, upstream = make(tokens, 72, rows, torch.bfloat16, ignored=0.0)
+    upstream[5] = upstream[tokens - 2] = 0.0
+    op = operator(tokens, 72, rows, "bfloat16", reduction="none")
+    clean = op.run(x, weights, labels, upstream)[2]
+    upstream[5] = upstream[tokens - 2] = float(value)
+    bad = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    bad[[5, tokens - 2]] = True
+    _, lse, dx, dw = op.run(x, weights, labels, upstream)
+    again, dw_again = op.backward(x, weights, labels, lse, upstream)
+    for got, got_dw in ((dx, dw), (again, dw_again)):
+        assert not bool(torch.isfinite(got[bad]).any()) and not bool(torch.isfinite(torch.cat(got_dw)).any())
+        assert bool(torch.isfinite(got[~bad]).all())
+    assert torch.equal(dx[~bad], clean[~bad])
+
+
 def test_gradient_against_differences():
     """Central differences of the kernel's own loss along one direction of x and of w.  x, w and the steps are multiples of 2^-6, exact in
     fp16.  A difference over 2h is off by h^2/6 times the third derivative, at most the cube of the direction's logit range per token,
