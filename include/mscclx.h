@@ -240,6 +240,8 @@ int mscclx_plan_time(mscclx_plan* plan, void* stream, int32_t iters, float* ms_o
  * A token whose label is `ignore_index` has loss 0 and adds nothing to either gradient, whatever its x holds; one whose label lies outside the
  * vocabulary otherwise has loss and gradients NaN (and every dw is NaN then).  MEAN divides by the number of tokens that are not
  * ignored, or by 1 if all are.  A non-finite grad_loss makes its token's dx, and every dw, non-finite; no other token's dx.
+ * What a call writes (loss, lse, dx, dweights, the workspace) may not overlap any other of its buffers (ALIASED); two
+ * inputs may, and matrices whose rows are equally far apart may lie side by side in one buffer.
  * Every call only enqueues kernels on `stream`: it can be captured in a HIP graph and replayed.  Calls that share a
  * workspace must follow each other on one stream (or be ordered by events). */
 #define MSCCLX_VOCAB_LOSS_MAX_RANKS 64
@@ -272,7 +274,7 @@ typedef struct {
   float* loss;                 /* NONE: [tokens], else one number                                             */
   float* lse;                  /* [tokens]: written by forward and run, read by backward                      */
   const float* grad_loss;      /* NONE: [tokens], else one number                                             */
-  void* dx;                    /* [tokens][hidden]; must not overlap any other buffer                         */
+  void* dx;                    /* [tokens][hidden]                                                            */
   int64_t dx_stride;
   void* const* dweights;       /* per rank [rank_rows][hidden]                                                */
   int64_t dweight_stride;

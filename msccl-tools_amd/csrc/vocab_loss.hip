@@ -696,6 +696,37 @@ int check_matrix(const char* what, const void* p, int64_t stride, int32_t hidden
   return MSCCLX_OK;
 }
 
+// A matrix, or a vector as one row of it, that a call reads or writes.
+struct Span {
+  uintptr_t from;
+  int64_t bytes, stride, rows;
+  const char* what;
+  int rank;
+  bool written;
+  uintptr_t to() const { return from + (rows - 1) * stride + bytes; }
+};
+
+// Two spans that share bytes, one of them written.  Matrices whose rows are equally far apart may lie side by side in one
+// buffer.
+bool collide(const Span& a, const Span& b) {
+  if (!(a.written || b.written) || a.to() <= b.from || b.to() <= a.from) return false;
+  if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) return true;
+  if (a.rows <= 1 && b.rows <= 1) return true;
+  const int64_t stride = a.rows > 1 ? a.stride : b.stride, off = (int64_t)((b.from - a.from) % stride + stride) % stride;
+  return off < a.bytes || off + b.bytes > stride;
+}
+
+int check_spans(std::vector<Span>& spans) {
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+  for (size_t i = 0; i < spans.size(); ++i)
+    for (size_t j = i + 1; j < spans.size() && spans[j].from < spans[i].to(); ++j)
+      if (collide(spans[i], spans[j])) {
+        auto name = [](const Span& s) { return s.rank < 0 ? std::string(s.what) : std::string(s.what) + " of rank " + std::to_string(s.rank); };
+        return fail(MSCCLX_ERR_ALIASED, name(spans[i]) + " and " + name(spans[j]) + " overlap, and one of them is written");
+      }
+  return MSCCLX_OK;
+}
+
 struct Call {
   Pieces pieces;
   Grads grads;
@@ -738,6 +769,24 @@ int check_call(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool 
       c->grads.dw[r] = (char*)io->dweights[r];
     }
   }
+  std::vector<Span> spans;
+  spans.reserve(2 * kMaxRanks + 8);
+  auto use = [&](const char* what, const void* p, int64_t rows, int64_t columns, int64_t stride, int size, bool written, int rank = -1) {
+    if (rows > 0 && columns > 0) spans.push_back({(uintptr_t)p, columns * size, stride * size, rows, what, rank, written});
+  };
+  const int64_t losses = d.reduction == MSCCLX_LOSS_NONE ? io->tokens : 1;
+  use("the workspace", io->workspace, 1, (int64_t)h->bytes, 0, 1, true);
+  use("x", io->x, io->tokens, d.hidden, io->x_stride, 2, false);
+  use("labels", io->labels, 1, io->tokens, 0, io->label_bytes, false);
+  use("lse", io->lse, 1, io->tokens, 0, 4, forward);
+  if (forward) use("loss", io->loss, 1, losses, 0, 4, true);
+  if (backward) use("grad_loss", io->grad_loss, 1, losses, 0, 4, false);
+  if (backward) use("dx", io->dx, io->tokens, d.hidden, io->dx_stride, 2, true);
+  for (int r = 0; r < d.ranks; ++r) {
+    use("weights", io->weights[r], h->pieces.rows[r], d.hidden, io->weight_stride, 2, false, r);
+    if (backward) use("dweights", io->dweights[r], h->pieces.rows[r], d.hidden, io->dweight_stride, 2, true, r);
+  }
+  if ((rc = check_spans(spans))) return rc;
   c->labels = Labels{io->labels, io->label_bytes == 8, d.ignore_index, h->vocab};
   char* ws = (char*)io->workspace;
   c->z_label = (float*)(ws + h->off_z);

@@ -107,6 +107,29 @@ def test_strides_labels_of_32_bits_and_what_lies_beside(dtype):
         assert bool(torch.isnan(b).all())
 
 
+def test_matrices_side_by_side_in_one_buffer():
+    """x and dx, and each rank's weights and dw, as columns of one buffer; the ranks' weights twice the same memory.  A dw for two ranks is refused."""
+    from msccl.executor import MscclxError
+    tokens, hidden, rows = 150, 64, [90, 90]
+    x, weights, labels, upstream = make(tokens, hidden, rows, torch.bfloat16)
+    weights = [weights[0], weights[0]]
+    forms = loss_forms(x, weights, labels, "none", IGNORE, upstream)
+    both = torch.zeros(tokens, 2 * hidden, dtype=x.dtype, device="cuda")
+    table = torch.zeros(sum(rows), 2 * hidden, dtype=x.dtype, device="cuda")
+    both[:, hidden:] = x
+    table[:90, :hidden] = weights[0]
+    dw = list(table[:, hidden:].split(rows))
+    op = operator(tokens, hidden, rows, "bfloat16", reduction="none")
+    loss, _, dx, dw = op.run(both[:, hidden:], [table[:90, :hidden]] * 2, labels, upstream, dx=both[:, :hidden], dweights=dw)
+    check("loss", loss, forms["loss"])
+    check("dx", dx, forms["dx"])
+    check("dw", torch.cat(dw), forms["dw"])
+    assert torch.equal(both[:, hidden:], x) and torch.equal(table[:90, :hidden], weights[0]) and not bool(table[90:, :hidden].any())
+    for more in (dict(dx=x), dict(dweights=[dw[0], dw[0]]), dict(dweights=[dw[0], weights[0]])):
+        with pytest.raises((MscclxError, ValueError), match="overlap|stride"):
+            op.run(x, weights, labels, upstream, **more)
+
+
 @pytest.mark.parametrize("reduction", ["none", "mean"])
 @pytest.mark.parametrize("tokens, rows", [(9, [100, 30]), (30, [257]), (90, [64] * 9), (140, [100, 30]), (600, [300, 500])])
 def test_what_stands_in_ignored_tokens_reaches_nothing(tokens, rows, reduction):

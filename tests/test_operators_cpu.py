@@ -83,6 +83,38 @@ def test_vocab_loss_calls_refuse(mscclx_lib, entry):
     mscclx_lib.mscclx_vocab_loss_destroy(handle)
 
 
+def apart(nbytes, **changed):
+    """A call whose buffers lie 16 MiB apart: x, labels, lse, loss, grad_loss, dx, workspace, then two ranks' weights and dweights."""
+    at = lambda i: (i + 1) << 24  # noqa: E731
+    weights, dweights = (ctypes.c_void_p * 2)(at(8), at(9)), (ctypes.c_void_p * 2)(at(10), at(11))
+    for name, array in (("w", weights), ("dw", dweights)):
+        for r in range(2):
+            if f"{name}{r}" in changed:
+                array[r] = changed.pop(f"{name}{r}")
+    values = dict(x=at(0), labels=at(1), lse=at(2), loss=at(3), grad_loss=at(4), dx=at(5), workspace=at(6), x_stride=128, dx_stride=128,
+                  weight_stride=128, dweight_stride=128, weights=ctypes.addressof(weights), dweights=ctypes.addressof(dweights))
+    return loss_io(nbytes, **{**values, **changed})[0], (weights, dweights)
+
+
+def test_vocab_loss_refuses_overlaps(mscclx_lib):
+    """100 tokens and rows of 64 values, 128 apart; ranks of 300 and 20 rows."""
+    rc, handle, nbytes, _ = create_loss(mscclx_lib)
+    assert rc == 0 and nbytes < 1 << 24
+    at = lambda i: (i + 1) << 24  # noqa: E731
+    row = 256  # bytes
+    both = [dict(loss=at(2)), dict(loss=at(0) + 16), dict(lse=at(1) + 396), dict(lse=at(6)), dict(loss=at(6) + nbytes - 4), dict(x=at(6) + 256),
+            dict(w0=at(6)), dict(lse=at(8) + 299 * row + 124)]
+    grads = [dict(dx=at(0)), dict(dx=at(0) + 99 * row), dict(dx=at(0) + 112), dict(dx=at(0) + 144), dict(dx=at(0) + 128, dx_stride=64),
+             dict(dx=at(8)), dict(dw0=at(8)), dict(dw1=at(10)), dict(dw1=at(10) + 299 * row), dict(dw0=at(0) + 16), dict(dw1=at(6)),
+             dict(dx=at(1)), dict(dx=at(4)), dict(dw1=at(2)), dict(dx=at(11))]
+    for entry, cases in (("forward", both), ("run", both + grads), ("backward", [c for c in both if "loss" not in c and "lse" not in c] + grads)):
+        for changed in cases:
+            io, keep = apart(nbytes, **changed)
+            assert getattr(mscclx_lib, f"mscclx_vocab_loss_{entry}")(handle, ctypes.byref(io), None) == ALIASED, (entry, changed)
+            assert b"overlap" in mscclx_lib.mscclx_last_error()
+    mscclx_lib.mscclx_vocab_loss_destroy(handle)
+
+
 def create_clip(lib, sizes=(10, 0, 7), dtype=F32, out=None, norm=0, counted=None):
     n = len(sizes)
     handle, nbytes = ctypes.c_void_p(), ctypes.c_uint64()
