@@ -309,7 +309,7 @@ int mscclx_grad_clip_create(int32_t ntensors, const uint64_t* sizes, const int32
                             int32_t norm, mscclx_grad_clip** out, uint64_t* workspace_bytes);
 int mscclx_grad_clip_destroy(mscclx_grad_clip* clip);
 /* Uploads the table of tensors into the workspace and waits for it.  Buffers start on a boundary of their element type.
- * out = NULL: norms only; out[i] = in[i]: in place.  Otherwise no output may overlap another buffer (ALIASED).  Not while a launch of
+ * out = NULL: norms only; out[i] = in[i]: in place.  Otherwise no output may overlap another buffer, and none the workspace (ALIASED).  Not while a launch of
  * the previous binding is in flight, and not while `stream` is being captured. */
 int mscclx_grad_clip_bind(mscclx_grad_clip* clip, const void* const* in, void* const* out, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Enqueues one kernel (the norm only: max_norm < 0) or two on `stream`; can be captured in a HIP graph.  The results are the two floats at

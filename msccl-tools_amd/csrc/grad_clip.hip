@@ -305,11 +305,13 @@ int mscclx_grad_clip_bind(mscclx_grad_clip* h, const void* const* in, void* cons
         chunks.push_back({(const void*)(a + from * in_size), out ? (void*)(b + from * out_size) : nullptr, (uint32_t)std::min(h->chunk, t.n - from), (uint8_t)t.in_type,
                           (uint8_t)t.out_type, (uint8_t)t.counted, {}});
     }
-    // what one tensor writes no other may read or write (two inputs may share memory)
+    spans.push_back({(uintptr_t)workspace, (uintptr_t)workspace + h->bytes, -1, true});
+    // what one tensor writes, and the workspace, no other may read or write (two inputs may share memory)
     std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
     uintptr_t read_to = 0, written_to = 0;
     for (const Span& s : spans) {
-      if (s.from < written_to || (s.written && s.from < read_to)) return fail(MSCCLX_ERR_ALIASED, "tensor " + std::to_string(s.tensor) + ": its memory overlaps another buffer, one of them an output");
+      if (s.from < written_to || (s.written && s.from < read_to))
+        return fail(MSCCLX_ERR_ALIASED, (s.tensor < 0 ? "the workspace" : "tensor " + std::to_string(s.tensor)) + ": its memory overlaps another buffer, one of them written");
       (s.written ? written_to : read_to) = std::max(s.written ? written_to : read_to, s.to);
     }
     char* ws = (char*)workspace;

@@ -152,6 +152,9 @@ def test_grad_clip_bind_and_launch_refuse(mscclx_lib):
     assert bind(fine, ptrs(at + 4, None, at + 4096)) == ALIASED
     assert bind(fine, ptrs(at + 4096, None, at + 4096)) == ALIASED
     assert bind(ptrs(at, None, at), ptrs(at, None, at)) == ALIASED
+    # the workspace is written as well
+    for i, o in ((fine, None), (ptrs(at + 8192, None, at + nbytes + 4096), ptrs(at + nbytes - 4, None, at + nbytes + 4096)), (ptrs(at - 36, None, at - 100), None)):
+        assert bind(i, o) == ALIASED, lib.mscclx_last_error()
     lib.mscclx_grad_clip_destroy(handle)
     rc, handle, nbytes = create_clip(lib, dtype=BF16, out=F32)
     assert rc == 0 and bind(fine, fine) == ALIASED
