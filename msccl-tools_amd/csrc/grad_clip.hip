@@ -3,14 +3,15 @@
 //   norm = |scale| sqrt(sum g^2)  or  |scale| max |g|      over all tensors that count
 //   c    = min(1, max_norm / (norm + 1e-6)),   out = g scale c
 //
-// Tensors are cut into chunks; a table in the workspace holds each chunk's addresses, so that a workgroup is two dependent loads from its
-// data.  Workgroup b takes chunks b, b + grid, ...
+// Tensors are cut into chunks; a table in the workspace holds each chunk's addresses, so that a workgroup is two
+// dependent loads from its data.  Workgroup b takes chunks b, b + grid, ...
 //
 // The first kernel reads every counted chunk once: squares are added in 64 bits (they are exact there, so no large
-// gradient overflows and no small one is lost; two conversions and a multiply-add per element, a fifth of what memory takes), magnitudes are
-// compared as unsigned integers, in which NaN is above infinity.  Each workgroup leaves one partial result.
-// The norm alone: the last workgroup to arrive adds the partial results, in one order.  Clipping: a second kernel, in which
-// every workgroup adds them, in the same order, and scales its chunks.  No sum goes through an atomic: the same bits at every call.
+// gradient overflows and no small one is lost; two conversions and a multiply-add per element, a fifth of what memory
+// takes), magnitudes are compared as unsigned integers, in which NaN is above infinity.  Each workgroup leaves one
+// partial result.  The norm alone: the last workgroup to arrive adds the partial results, in one order.  Clipping: a
+// second kernel, in which every workgroup adds them, in the same order, and scales its chunks.  No sum goes through an
+// atomic: the same bits at every call.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -135,10 +136,10 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const Chunk* chunks, int
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
     return;
   }
-  // Who arrives last adds: of the workgroups of a counter, then of the counters.  Release and acquire would write back and drop this XCD's cache for every
-  // workgroup (norm over 256 MiB: 101 us instead of 42).  They are not needed: the partial result is exchanged, not stored, so its old value
-  // comes back only when the new one is where all XCDs see it, and each next atomic waits for the value of the one before; the loads
-  // below go to the same place.
+  // Who arrives last adds: of the workgroups of a counter, then of the counters.  Release and acquire would write back
+  // and drop this XCD's cache for every workgroup (norm over 256 MiB: 101 us instead of 42).  They are not needed: the
+  // partial result is exchanged, not stored, so its old value comes back only when the new one is where all XCDs see
+  // it, and each next atomic waits for the value of the one before; the loads below go to the same place.
   __shared__ int last;
   if (threadIdx.x == 0) {
     typedef std::conditional_t<sizeof(V) == 8, unsigned long long, unsigned> Bits;
@@ -252,7 +253,8 @@ int mscclx_grad_clip_create(int32_t ntensors, const uint64_t* sizes, const int32
       if (total > (1ull << 44)) return fail(MSCCLX_ERR_CAPACITY, "more than 2^44 gradients");
       h->tensors.push_back({sizes[i], in_dtypes[i], out_dtypes[i], !counted || counted[i]});
     }
-    // eight chunks for each workgroup of a full grid, so that the last ones are short against the whole; of at least one pass of its threads
+    // eight chunks for each workgroup of a full grid, so that the last ones are short against the whole; of at least
+    // one pass of its threads
     while (h->chunk < kMaxChunk && h->chunk * kMaxGrid * 8 < total) h->chunk *= 2;
     for (const auto& t : h->tensors) h->chunks += (t.n + h->chunk - 1) / h->chunk;
     uint64_t at = (sizeof(Header) + 255) / 256 * 256;

@@ -5,8 +5,8 @@
 // contiguous ("row": one row of memory per l or r) or with k strided ("col": one row of memory per k).
 //
 // Data path: a workgroup copies the next 64 values of k of both operands from memory into LDS without passing through
-// registers (16 bytes per lane), while its waves feed the matrix cores from the copy before.  The copies write LDS in lane order, so
-// the bank swizzle is applied to the addresses they read from:
+// registers (16 bytes per lane), while its waves feed the matrix cores from the copy before.  The copies write LDS in
+// lane order, so the bank swizzle is applied to the addresses they read from:
 //   row operand: 128 bytes per row, the 16-byte unit u of row i sits at u ^ (i / 2 % 8): the sixteen rows that a
 //                fragment read touches at one unit then cover all 64 banks;
 //   col operand: one line of 2 * TILE bytes per k, 32-byte pair p of line k sits at p ^ swizzle_of(k): the transposing
@@ -55,7 +55,8 @@ template <> struct Half<_Float16> {
   }
 };
 
-// 16 bytes per lane from `resource` at `offset` (per lane) + `further` to LDS at m0 + 16 * lane.  Nothing else in these kernels uses m0.
+// 16 bytes per lane from `resource` at `offset` (per lane) + `further` to LDS at m0 + 16 * lane.  Nothing else in these
+// kernels uses m0.
 __device__ __forceinline__ void copy_to_lds(unsigned lds, unsigned offset, i32x4 resource, int further) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(resource), "s"(further) : "memory");
 }
@@ -78,8 +79,8 @@ struct Lanes {
   unsigned offset[kChunks];
   int k[COL ? kChunks : 1];                                      // the lane's k (its first) in the step
 
-  // `stride`: bytes between rows of memory; `valid(unit)`: rows of the unit (row, counted from its base) or columns (col) that exist.  A col operand's
-  // rows repeat themselves within a step with `period`, if it is less than a step.
+  // `stride`: bytes between rows of memory; `valid(unit)`: rows of the unit (row, counted from its base) or columns
+  // (col) that exist.  A col operand's rows repeat themselves within a step with `period`, if it is less than a step.
   template <class F> __device__ __forceinline__ void place(int thread, int64_t stride, F valid, int period = kStepK) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
@@ -103,8 +104,9 @@ struct Lanes {
   }
 };
 
-// Where an operand's copies read: `base(i)`, the resource of the rows of unit i (row) or of all (col), for step after step `next()`; then
-// `further` is what they add to it, and `left` the values of k from the step's first on.  Behind the last step nothing is left.
+// Where an operand's copies read: `base(i)`, the resource of the rows of unit i (row) or of all (col), for step after
+// step `next()`; then `further` is what they add to it, and `left` the values of k from the step's first on.  Behind
+// the last step nothing is left.
 template <int TILE> struct RowSource {  // k contiguous
   static constexpr int kUnits = (TILE + kUnitRows - 1) / kUnitRows;
   i32x4 bases[kUnits];
@@ -156,8 +158,9 @@ struct TileProduct {
   static __device__ __forceinline__ int l_of(int thread, int f) { return (thread >> 6) % WL * (TL / WL) + f * 16 + (thread >> 4 & 3) * 4; }
   static __device__ __forceinline__ int r_of(int thread, int f) { return (thread >> 6) / WL * (TR / WR) + f * 16 + (thread & 15); }
 
-  // Stores want 16 bytes per lane.  A lane holds four neighbours of fragment f and four of f + 1; lanes 16 apart swap one of them, so that
-  // each has eight neighbours of one fragment: 64 bytes of an output row per store.  -> their place in the tile, l
+  // Stores want 16 bytes per lane.  A lane holds four neighbours of fragment f and four of f + 1; lanes 16 apart swap
+  // one of them, so that each has eight neighbours of one fragment: 64 bytes of an output row per store.  -> their
+  // place in the tile, l
   static __device__ __forceinline__ int l_of_pair(int thread, int f) {
     const int group = thread >> 4 & 3;
     return (thread >> 6) % WL * (TL / WL) + (f + (group & 1)) * 16 + (group >> 1) * 8;
@@ -206,8 +209,8 @@ struct TileProduct {
       if (u < FR) f.b[u] = fragment<RCOL, TR>(at + LLanes::kBytes, r0, half, lane, u);
       else f.a[u - FR] = fragment<LCOL, TL>(at, l0, half, lane, u - FR);
     };
-    // One fragment row of products after another; between them the next half's reads and, in the second half, the copies, so
-    // that neither LDS nor the path to it gets all of a step's requests at once.
+    // One fragment row of products after another; between them the next half's reads and, in the second half, the
+    // copies, so that neither LDS nor the path to it gets all of a step's requests at once.
     auto multiply = [&](const Fragments& f, int l) {
 #pragma unroll
       for (int r = 0; r < FR; ++r) acc[l][r] = Half<T>::mfma(f.a[l], f.b[r], acc[l][r]);
@@ -241,8 +244,8 @@ struct TileProduct {
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * kCopies) : "memory");
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) read(now, 0, 0, u);
-    // Where registers are left, sums of four steps are added up, not one step to the sum of all before it: with few tokens one of them can make the whole
-    // loss, and its logit's rounding errors a large part of it.
+    // Where registers are left, sums of four steps are added up, not one step to the sum of all before it: with few
+    // tokens one of them can make the whole loss, and its logit's rounding errors a large part of it.
     constexpr bool kInTwo = STAGES > 2;
     f32x4 total[kInTwo ? FL : 1][kInTwo ? FR : 1] = {};
     auto add_up = [&] {
@@ -261,7 +264,8 @@ struct TileProduct {
         multiply(now, l);
         __builtin_amdgcn_sched_barrier(0);
       }
-      // the copies of the next step have arrived, and every wave has read all of this one: its buffer takes the step STAGES further
+      // the copies of the next step have arrived, and every wave has read all of this one: its buffer takes the step
+      // STAGES further
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * kCopies) : "memory");
       sl.next(), sr.next();
 #pragma unroll

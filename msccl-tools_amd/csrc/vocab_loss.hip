@@ -1,4 +1,5 @@
-// Softmax cross entropy over a vocabulary that is cut into the ranks' pieces, with its gradients, without keeping the logits.
+// Softmax cross entropy over a vocabulary that is cut into the ranks' pieces, with its gradients, without keeping the
+// logits.
 //
 //   z[n][v]  = sum over d of x[n][d] w[v][d]        w: the ranks' rows one under the other
 //   lse[n]   = log sum over v of exp z[n][v],   loss[n] = lse[n] - z[n][label[n]]
@@ -10,15 +11,18 @@
 //   tokens   a token's (m, sum) become its lse and loss, and its E becomes G in place: G = (E exp(m - lse) - [label]) g / max|g|;
 //   dx, dw   the two products, on G.  dx sums over the whole vocabulary: where its tiles do not fill the chip, that
 //            axis is cut and the parts are added by workgroups that dw's launch has more.
-// Tokens whose label is ignored have rows of zeros in G.  With more than kWideTokens tokens they are left out: G, and a copy of x beside it, hold the others'
-// rows one behind the other, so that they cost nothing in the two products (of 8192 tokens x 131072 x 4096 with 15 % ignored: 20.4 -> 18.9 ms).  Their x is
-// never read for a gradient: the copy has zeros there, or nothing.
-// With few tokens, up to kWideTokens if they are few for each rank, memory and not the matrix cores sets the time, and nothing is lost to 16 bits on the way: the logits are kept in
-// 32 bits instead of E, and G is kept as two 16-bit numbers, itself rounded and what that left (16 bits of it in bf16, 22 in fp16).  The products take the second ones as
-// more rows.  (With so few tokens single values of G decide about a rank's dw, and some ranks hold no label: rounded once, dw was up to 1.9 times as far off as
-// with G in 32 bits.)  With more tokens E and G are both rounded, each relative to its own size (bf16 2^-9, fp16 2^-12 at the
-// most), with 2^15 as unit in fp16, so that probabilities down to 2^-29 are normal numbers; |g| is divided by its largest value for
-// the same reason and multiplied back in 32 bits behind the products.
+// Tokens whose label is ignored have rows of zeros in G.  With more than kWideTokens tokens they are left out: G, and a
+// copy of x beside it, hold the others' rows one behind the other, so that they cost nothing in the two products (of
+// 8192 tokens x 131072 x 4096 with 15 % ignored: 20.4 -> 18.9 ms).  Their x is never read for a gradient: the copy has
+// zeros there, or nothing.
+// With few tokens, up to kWideTokens if they are few for each rank, memory and not the matrix cores sets the time, and
+// nothing is lost to 16 bits on the way: the logits are kept in 32 bits instead of E, and G is kept as two 16-bit
+// numbers, itself rounded and what that left (16 bits of it in bf16, 22 in fp16).  The products take the second ones as
+// more rows.  (With so few tokens single values of G decide about a rank's dw, and some ranks hold no label: rounded
+// once, dw was up to 1.9 times as far off as with G in 32 bits.)  With more tokens E and G are both rounded, each
+// relative to its own size (bf16 2^-8, fp16 2^-11 at the most), with 2^15 as unit in fp16, so that probabilities down
+// to 2^-29 are normal numbers; |g| is divided by its largest value for the same reason and multiplied back in 32 bits
+// behind the products.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -41,8 +45,8 @@ constexpr int kTile = 256;              // columns of G are padded to a multiple
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 1.0 / (double)kLog2e;  // what takes the rounded kLog2e back
 
-// The ranks' pieces of the vocabulary, passed to the kernels by value.  Units of kUnitRows rows; none spans two ranks, a tile may.
-// What pads a rank's last unit, or the last tile, counts as outside.
+// The ranks' pieces of the vocabulary, passed to the kernels by value.  Units of kUnitRows rows; none spans two ranks,
+// a tile may.  What pads a rank's last unit, or the last tile, counts as outside.
 struct Pieces {
   int ranks, tiles;
   int rows[kMaxRanks];
@@ -51,7 +55,8 @@ struct Pieces {
   const char* w[kMaxRanks];
 };
 
-// Which rank holds something: the ranks' ends, one in each lane, are compared at once.  (A loop over the ranks waits for memory at every turn.)
+// Which rank holds something: the ranks' ends, one in each lane, are compared at once.  (A loop over the ranks waits
+// for memory at every turn.)
 struct Ends {
   int end, ranks;
   __device__ __forceinline__ Ends(const int* ends, int ranks) : ranks(ranks) {
@@ -98,13 +103,15 @@ struct Upstream {
   }
 };
 
-// Exponents are kept in units of log 2: exp(z - m) = exp2(z log2(e) - M) with M = m log2(e), one multiply-add and one instruction.
+// Exponents are kept in units of log 2: exp(z - m) = exp2(z log2(e) - M) with M = m log2(e), one multiply-add and one
+// instruction.
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 template <class T> constexpr float kUnit = std::is_same_v<T, _Float16> ? 32768.0f : 1.0f;
 
-// How a workgroup's tile is cut.  Large: one workgroup of eight waves per compute unit.  Middle: two of four waves, for products whose large tiles
-// would not fill the chip.  Thin: four of four waves, each one step at a time, for products that write more than they read.  Few: at most 32 tokens, with
-// four steps of copies under way, because then memory is all that counts.
+// How a workgroup's tile is cut.  Large: one workgroup of eight waves per compute unit.  Middle: two of four waves, for
+// products whose large tiles would not fill the chip.  Thin: four of four waves, each one step at a time, for products
+// that write more than they read.  Few: at most 32 tokens, with four steps of copies under way, because then memory is
+// all that counts.
 template <int L, int R, int WL, int WR, int STAGES, int WAVES> struct Shape {  // WAVES: per SIMD, at least
   static constexpr int kL = L, kR = R, kWavesL = WL, kWavesR = WR, kThreads = WL * WR * 64, kWaves = WAVES;
   template <class T, bool LCOL, bool RCOL> using Product = TileProduct<T, L, R, WL, WR, STAGES, LCOL, RCOL>;
@@ -158,8 +165,9 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
   const int n0 = tt * TR, tokens = min(TR, a.tokens - n0);
   f32x4 acc[Product::FL][Product::FR] = {};
   {
-    // With one workgroup per compute unit all would ask for the same few bytes of each row of W at a time, which lie a power of two apart;
-    // each begins at another k (1 token x 32768 x 2048: 34 us in step, 30 so; with more workgroups it costs 3 %)
+    // With one workgroup per compute unit all would ask for the same few bytes of each row of W at a time, which lie a
+    // power of two apart; each begins at another k (the loss of 1 token x 32768 x 2048: 36.2 us in step, 32.2 so; with
+    // more workgroups it costs 3 %)
     const int steps = (a.hidden + kStepK - 1) / kStepK, first = TR == Few::kR && gridDim.x <= kComputeUnits ? at % steps : 0;
     typename Product::LLanes ll;
     typename Product::RLanes rl;
@@ -317,10 +325,11 @@ struct TokenArgs {
   int given;           // kLogits: the lse is an input
 };
 
-// A workgroup per token: its parts' (m, sum) -> lse and loss, and with gradients its row of x, and of G: kKeep from E, in place; kLogits from the logits; kGradient: G is
-// there and so is the lse.  Where tokens
-// are few, several workgroups share one: each works out the lse for itself (a thirtieth of what it then moves) and takes gridDim.y'ths of the row.
-// The label's own G = (p - 1) g comes from its logit in 32 bits: from a rounded p close to 1 next to nothing would be left of it.
+// A workgroup per token: its parts' (m, sum) -> lse and loss, and with gradients its row of x, and of G: kKeep from E,
+// in place; kLogits from the logits; kGradient: G is there and so is the lse.  Where tokens are few, several workgroups
+// share one: each works out the lse for itself (a thirtieth of what it then moves) and takes gridDim.y'ths of the row.
+// The label's own G = (p - 1) g comes from its logit in 32 bits: from a rounded p close to 1 next to nothing would be
+// left of it.
 template <class T, int MODE>
 __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const TokenArgs a) {
   __shared__ float shared[4];
@@ -408,8 +417,9 @@ struct SumsArgs {
   float* back;
 };
 
-// One workgroup over all tokens: the loss as one number, in 64 bits and in one order; with gradients what the products are
-// multiplied by, max |g| (over the mean's count) over the unit, and with a number per token factor[n] = g[n] / max |g|.
+// One workgroup over all tokens: the loss as one number, in 64 bits and in one order; with gradients what the products
+// are multiplied by, max |g| (over the mean's count) over the unit, and with a number per token factor[n] = g[n] / max
+// |g|.
 __device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shared) {
   double sum = 0, count = 0;
   float top = 0.f;
@@ -706,8 +716,8 @@ struct Span {
   uintptr_t to() const { return from + (rows - 1) * stride + bytes; }
 };
 
-// Two spans that share bytes, one of them written.  Matrices whose rows are equally far apart may lie side by side in one
-// buffer.
+// Two spans that share bytes, one of them written.  Matrices whose rows are equally far apart may lie side by
+// side in one buffer.
 bool collide(const Span& a, const Span& b) {
   if (!(a.written || b.written) || a.to() <= b.from || b.to() <= a.from) return false;
   if (a.rows > 1 && b.rows > 1 && a.stride != b.stride) return true;
@@ -806,24 +816,29 @@ int check_call(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool 
 int tiles(int64_t n, int of = kTile) { return (int)((n + of - 1) / of); }
 
 enum { kLarge, kMiddle, kThin, kFew };
-// Which shape a product takes, by tokens x vocabulary x hidden (bf16, us with the shape / with the next best).
-// Logits: Few up to four rounds of its workgroups (128 x 8192 x 1024: 14.8 / 19.0 Middle; 40 x 65536 x 4096: 123 / 133) but not where W would be read
-// again from memory for every 32 tokens (128 x 65536 x 4096: 208 / 142 Middle); Large once its tiles fill the chip (384 x 32768 x 2048: 58 / 67
-// Middle) and are not half empty, else Middle (256 x 32768 x 2048: 44 / 52 Large).
+// Which shape a product takes.  Figures: us of the kernel with the shape / with the next best, by tokens x vocabulary x
+// hidden in bf16, W from memory.  Logits: Few up to four rounds of its workgroups (128 x 8192 x 1024: 10.4 / 17.9
+// Middle; 1 x 32768 x 4096: 80 / 101; 40 x 65536 x 4096: 168 / 182) but not where W would be read again from memory for
+// every 32 tokens (128 x 65536 x 4096: 245 / 187 Middle); Large once its tiles fill the chip (384 x 32768 x 2048: 71 /
+// 91 Middle) and are not half empty, else Middle (256 x 32768 x 2048: 60 / 73 Large).
 int logits_shape(const Pieces& p, int64_t tokens) {
   if (tokens <= 256 && (int64_t)tiles(tokens, Few::kR) * p.tiles * (kTile / Few::kL) <= 4 * kComputeUnits) return kFew;
   return tokens <= 128 || (int64_t)tiles(tokens) * p.tiles < kComputeUnits ? kMiddle : kLarge;
 }
-// dw writes more than it reads where tokens are few; workgroups then hide each other's loads and stores (dw's part, by tokens x vocabulary x hidden: 16 x 131072 x
-// 4096 210 us Thin / 304 Middle, 200 x 20000 x 3000 47 / 60, 300 x 20000 x 1024 26 / 32 Large; 500 x 32768 x 2048 92 / 85 Large).  1021 x 32003 x 1288: Large 15 us
-// shorter than Middle.
+// dw writes more than it reads where tokens are few; workgroups then hide each other's loads and stores (16 x 131072 x
+// 4096: 222 Thin / 285 Large, 200 x 20000 x 3000 47 / 55, 300 x 20000 x 1024 25 / 28 Middle; 500 x 32768 x 2048 80 / 82
+// Large, 1021 x 32003 x 1288 100 / 93).  More tokens: Large once its tiles fill the chip (1021 x 32003 x 1288: 93 / 110
+// Middle; 1024 x 4096 x 512: 29 / 20 Middle).
 int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 384 ? kThin : (int64_t)p.tiles * tiles(hidden) < kComputeUnits ? kMiddle : kLarge; }
 
-// Where G's second rows begin, so that no step of dw's product and no tile of dx's has more of them than need be; rows behind the first ones are zeros.
+// Where G's second rows begin, so that no step of dw's product and no tile of dx's has more of them than need be; rows
+// behind the first ones are zeros.
 int second_row(int64_t tokens) { return tokens <= 16 ? 16 : tokens <= 32 ? 32 : (int)((tokens + kStepK - 1) / kStepK * kStepK); }
 
-// dx: into how many parts the vocabulary is cut so that the tiles fill the chip, of at least eight steps each (with four, 1024 x 4096 x 512 takes 5 us
-// longer).  Few as long as reading W again for every 32 tokens costs little (128 x 8192 x 1024: 3 us shorter than Middle; 40 x 65536 x 4096: 26 us longer).
+// dx: into how many parts the vocabulary is cut so that the tiles fill the chip, of at least eight steps each (with
+// four, 1024 x 4096 x 512 takes 3 us longer to add them).  Few as long as reading W again for every 32 tokens costs
+// little (1 x 32768 x 2048: 29 us / 34 Middle, 1 x 65536 x 2048 54 / 63, 32 x 131072 x 4096 225 / 227; 40 x 65536 x 4096
+// 137 / 106 Middle); Large from 24 tiles on (1021 x 32003 x 1288: 95 / 107 Middle; 256 x 32768 x 2048: 73 / 47 Middle).
 struct DxPlan {
   int shape, token_tiles, hidden_tiles, parts, split_steps;
   bool separate;  // the parts are kept and added
@@ -836,7 +851,7 @@ DxPlan dx_plan(const Pieces& p, int64_t tokens, int hidden, bool separate) {
   const int l = d.shape == kLarge ? Large::kL : d.shape == kMiddle ? Middle::kL : Few::kL, r = d.shape == kLarge ? Large::kR : d.shape == kMiddle ? Middle::kR : Few::kR;
   d.token_tiles = tiles(tokens, r);
   d.hidden_tiles = tiles(hidden, l);
-  const int64_t slots = d.shape == kLarge ? kComputeUnits : 2 * kComputeUnits;  // (Few with one per unit: 16 x 131072 x 4096 245 us instead of 190)
+  const int64_t slots = d.shape == kLarge ? kComputeUnits : 2 * kComputeUnits;  // (Few with one per unit: 16 x 131072 x 4096 258 us instead of 199)
   const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, slots / ((int64_t)d.token_tiles * d.hidden_tiles)));
   d.split_steps = (steps + parts - 1) / parts;
   d.parts = (steps + d.split_steps - 1) / d.split_steps;
@@ -852,7 +867,9 @@ int launch_logits(int shape, const Pieces& p, LogitsArgs& a, hipStream_t stream)
     hipLaunchKernelGGL((logits_kernel<T, MODE, S>), dim3((unsigned)(a.token_tiles * p.tiles * (kTile / S::kL))), dim3(S::kThreads), 0, stream, p, a);
     return launched("logits_kernel");
   };
-  return shape == kLarge ? go(Large()) : shape == kMiddle ? go(Middle()) : go(Few());
+  if constexpr (MODE != kLogits)  // (up to kWideTokens tokens)
+    if (shape == kLarge) return go(Large());
+  return shape == kMiddle ? go(Middle()) : go(Few());
 }
 
 template <class T>
@@ -865,9 +882,9 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
   int rc;
   // Twice where that decides about a rank's dw: with few tokens, or few for each rank
   const bool wide = backward && (n <= 32 || (n <= kWideTokens && n < 16 * d.ranks));
-  // The sums over tokens: for the gradients in front of everything, unless that is one number and nothing in front of the products asks for it; for the loss as one
-  // number behind the last piece's tokens (beside its gradients, where dx has parts).
-  // Up to kWideTokens tokens, rows of zeros cost less than the launch that finds out which they are
+  // The sums over tokens: for the gradients in front of everything, unless that is one number and nothing in front of
+  // the products asks for it; for the loss as one number behind the last piece's tokens (beside its gradients, where dx
+  // has parts). Up to kWideTokens tokens, rows of zeros cost less than the launch that finds out which they are
   const bool ordered = backward && n > kWideTokens;
   const bool early = backward && (per_token || !forward || ordered);
   SumsArgs first = {n, c.labels, mean, nullptr, nullptr, io->grad_loss, per_token ? c.factor : nullptr, kUnit<T>, c.back};
