@@ -417,14 +417,20 @@ struct SumsArgs {
   float* back;
 };
 
+struct OrderArgs {
+  int64_t piece;  // tokens of a piece
+  int *pos, *idx;  // a token's row among its piece's, -1: ignored; and the token (in the piece) of a row
+  int* live;      // per piece: rows
+};
+
 // One workgroup over all tokens: the loss as one number, in 64 bits and in one order; with gradients what the products
 // are multiplied by, max |g| (over the mean's count) over the unit, and with a number per token factor[n] = g[n] / max
 // |g|.
-__device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shared) {
+__device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shared, int64_t kept = -1) {
   double sum = 0, count = 0;
   float top = 0.f;
   for (int64_t n = threadIdx.x; n < a.tokens; n += blockDim.x) {
-    const int label = a.labels.get(n);
+    const int label = kept < 0 || a.factor ? a.labels.get(n) : 0;
     count += label != -1;
     if (a.rows) sum += a.rows[n];
     if (a.factor && label >= 0) {  // an infinite one is its token's own affair
@@ -433,15 +439,16 @@ __device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shar
     }
   }
   auto add = [](double a, double b) { return a + b; };
-  if (a.mean) count = fmax(block_reduce(count, add, shared), 1.0);
-  else count = 1.0;
+  if (!a.mean) count = 1.0;
+  else if (kept >= 0) count = fmax((double)kept, 1.0);
+  else count = fmax(block_reduce(count, add, shared), 1.0);
   if (a.rows) {
     sum = block_reduce(sum, add, shared);
     if (threadIdx.x == 0) *a.loss = (float)(sum / count);
   }
   if (!a.upstream) return;
   if (a.factor) {
-    top = (float)block_reduce((double)top, [](double a, double b) { return fmax(a, b); }, shared);
+    top = block_reduce(top, [](float a, float b) { return fmaxf(a, b); }, (float*)shared);
     for (int64_t n = threadIdx.x; n < a.tokens; n += blockDim.x) {
       const int label = a.labels.get(n);
       const float g = a.upstream[n];
@@ -453,43 +460,61 @@ __device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shar
   if (threadIdx.x == 0) *a.back = (float)((double)top / count / a.unit);
 }
 
-struct OrderArgs {
-  int64_t piece;  // tokens of a piece
-  int *pos, *idx;  // a token's row among its piece's, -1: ignored; and the token (in the piece) of a row
-  int* live;      // per piece: rows
-};
+constexpr int kSumsThreads = 1024, kSumsWaves = kSumsThreads / 64;
 
-// The rows of the tokens that are not ignored, in the tokens' order.
-__device__ __forceinline__ void order_tokens(const OrderArgs& o, int64_t tokens, const Labels& labels, int* shared) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+// The rows of the tokens that are not ignored, in the tokens' order.  Each thread takes eight neighbours, so that a chunk
+// of 8192 tokens waits for memory once.  -> how many there are
+__device__ __forceinline__ int64_t order_tokens(const OrderArgs& o, int64_t tokens, const Labels& labels, int (*shared)[kSumsWaves]) {
+  constexpr int kEach = 8;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t kept = 0;
+  int turn = 0;  // of the two halves of shared: whoever writes one again has met everyone at the other's barrier
   for (int64_t from = 0; from < tokens; from += o.piece) {
     const int64_t to = min(from + o.piece, tokens);
     int rows = 0;
-    for (int64_t c = from; c < to; c += blockDim.x) {
-      const int64_t n = c + threadIdx.x;
-      const bool keep = n < to && labels.get(n) != -1;
-      const unsigned long long kept = __ballot(keep);
-      if (lane == 0) shared[wave] = __popcll(kept);
-      __syncthreads();
-      int before = rows, all = 0;
-      for (int w = 0; w < waves; ++w) {
-        if (w < wave) before += shared[w];
-        all += shared[w];
+    for (int64_t c = from; c < to; c += kSumsThreads * kEach, turn ^= 1) {
+      const int64_t n = c + threadIdx.x * kEach;
+      bool keep[kEach];
+      int count = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) keep[j] = n + j < to && labels.get(n + j) != -1;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) count += keep[j];
+      int upto = count;  // of the wave's threads up to this one, then of the waves
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int other = __shfl_up(upto, d);
+        if (lane >= d) upto += other;
       }
-      before += __popcll(kept & ((1ull << lane) - 1));
-      if (n < to) o.pos[n] = keep ? before : -1;
-      if (keep) o.idx[from + before] = (int)(n - from);
-      rows += all;
+      if (lane == 63) shared[turn][wave] = upto;
       __syncthreads();
+      int waves = lane < kSumsWaves ? shared[turn][lane] : 0;
+#pragma unroll
+      for (int d = 1; d < kSumsWaves; d *= 2) {
+        const int other = __shfl_up(waves, d);
+        if (lane >= d) waves += other;
+      }
+      const int front = __shfl(waves, max(wave - 1, 0));
+      int at = rows + (wave ? front : 0) + upto - count;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        if (n + j < to) o.pos[n + j] = keep[j] ? at : -1;
+        if (keep[j]) o.idx[from + at++] = (int)(n + j - from);
+      }
+      rows += __shfl(waves, kSumsWaves - 1);
     }
     if (threadIdx.x == 0) o.live[from / o.piece] = rows;
+    kept += rows;
   }
+  return kept;
 }
 
-__global__ void __launch_bounds__(1024) sums_kernel(const SumsArgs a, const OrderArgs o) {
-  __shared__ double shared[16];
-  if (o.pos) order_tokens(o, a.tokens, a.labels, (int*)shared);
-  sums_over_tokens(a, shared);
+__global__ void __launch_bounds__(kSumsThreads) sums_kernel(const SumsArgs a, const OrderArgs o) {
+  __shared__ double shared[kSumsWaves];
+  __shared__ int counts[2][kSumsWaves];
+  int64_t kept = -1;
+  if (o.pos) kept = order_tokens(o, a.tokens, a.labels, counts);
+  sums_over_tokens(a, shared, kept);
 }
 
 // The rows of all ranks' pieces as k of a product: a step is a unit.
@@ -890,7 +915,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
   SumsArgs first = {n, c.labels, mean, nullptr, nullptr, io->grad_loss, per_token ? c.factor : nullptr, kUnit<T>, c.back};
   SumsArgs totals = {n, c.labels, mean, forward && !per_token ? c.row_loss : nullptr, io->loss, backward && !early ? io->grad_loss : nullptr, nullptr, kUnit<T>, c.back};
   auto sums = [&](const SumsArgs& what, const OrderArgs& order) {
-    hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(1024), 0, stream, what, order);
+    hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(kSumsThreads), 0, stream, what, order);
     return launched("sums_kernel");
   };
   if (early && (rc = sums(first, ordered ? c.order : OrderArgs{}))) return rc;
