@@ -146,13 +146,16 @@ struct LogitsArgs {
 // up to kBand row tiles share what they read.  Of 8, 4 and 2, at 8192 tokens of 4096 and 32768 rows: logits kept 1697,
 // 1651 and 1690 us, not kept 1522, 1511 and 1571; dx 1597, 1577 and 1578; dw 1622, 1607 and 1632.
 constexpr int kBand = 4;
-__device__ __forceinline__ void tile_of(int id, int rows, int cols, int* row, int* col) {
-  const int total = rows * cols, per = total / 8;
-  if (id < per * 8) id = id % 8 * per + id / 8;
+__device__ __forceinline__ int xcd_order(int id, int total) {
+  const int per = total / 8;
+  return id < per * 8 ? id % 8 * per + id / 8 : id;
+}
+__device__ __forceinline__ void tile_in_band(int id, int rows, int cols, int* row, int* col) {
   const int band = kBand * cols, at = id / band * kBand, high = min(kBand, rows - at), in = id % band;
   *row = at + in % high;
   *col = in / high;
 }
+__device__ __forceinline__ void tile_of(int id, int rows, int cols, int* row, int* col) { tile_in_band(xcd_order(id, rows * cols), rows, cols, row, col); }
 
 template <class T, int MODE, class Shape>
 __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(const Pieces pieces, const LogitsArgs a) {
@@ -583,17 +586,16 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dx_kernel(cons
   typedef typename Shape::template Product<T, true, false> Product;
   constexpr int TL = Shape::kL, TR = Shape::kR;
   __shared__ __attribute__((aligned(1024))) char smem[Product::kLdsBytes];
-  if (blockIdx.x == a.token_tiles * a.hidden_tiles) {
-    if (blockIdx.y == 0) sums_over_tokens(sums, (double*)smem);
-    return;
-  }
-  const int all = a.live ? *a.live : a.rows, token_tiles = (all + TR - 1) / TR;
-  if ((int)blockIdx.x >= token_tiles * a.hidden_tiles) return;
+  if ((int)blockIdx.x == a.token_tiles * a.hidden_tiles * a.count) return sums_over_tokens(sums, (double*)smem);
+  // All tiles of a part of the vocabulary follow each other in one XCD, which then reads the part of G and W once
+  const int all = a.live ? *a.live : a.rows, token_tiles = (all + TR - 1) / TR, tiles = token_tiles * a.hidden_tiles;
+  if ((int)blockIdx.x >= tiles * a.count) return;
+  const int in_order = xcd_order(blockIdx.x, tiles * a.count), part = in_order / tiles;
   int tt, ht;
-  tile_of(blockIdx.x, token_tiles, a.hidden_tiles, &tt, &ht);
+  tile_in_band(in_order % tiles, token_tiles, a.hidden_tiles, &tt, &ht);
   const int n0 = tt * TR, d0 = ht * TL, tokens = min(TR, all - n0), width = min(TL, a.hidden - d0);
   const int64_t ld = (int64_t)pieces.tiles * kTile;
-  const int step0 = blockIdx.y * a.split_steps, steps = min(a.split_steps, pieces.tiles * (kTile / kStepK) - step0);
+  const int step0 = part * a.split_steps, steps = min(a.split_steps, pieces.tiles * (kTile / kStepK) - step0);
   f32x4 acc[Product::FL][Product::FR] = {};
   {
     typename Product::LLanes ll;
@@ -611,7 +613,7 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dx_kernel(cons
 #pragma unroll
       for (int l = 0; l < Product::FL; ++l) {
         const int d = Product::l_of(threadIdx.x, l);
-        if (n < tokens && d < width) *(f32x4*)(a.parts + ((int64_t)blockIdx.y * a.rows + n0 + n) * a.hidden + d0 + d) = acc[l][r];
+        if (n < tokens && d < width) *(f32x4*)(a.parts + ((int64_t)part * a.rows + n0 + n) * a.hidden + d0 + d) = acc[l][r];
       }
     } else {
       const int64_t token = a.live && n < tokens ? a.idx[n0 + n] : n0 + n;
@@ -860,10 +862,12 @@ int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 384
 // behind the first ones are zeros.
 int second_row(int64_t tokens) { return tokens <= 16 ? 16 : tokens <= 32 ? 32 : (int)((tokens + kStepK - 1) / kStepK * kStepK); }
 
-// dx: into how many parts the vocabulary is cut so that the tiles fill the chip, of at least eight steps each (with
-// four, 1024 x 4096 x 512 takes 3 us longer to add them).  Few as long as reading W again for every 32 tokens costs
-// little (1 x 32768 x 2048: 29 us / 34 Middle, 1 x 65536 x 2048 54 / 63, 32 x 131072 x 4096 225 / 227; 40 x 65536 x 4096
-// 137 / 106 Middle); Large from 24 tiles on (1021 x 32003 x 1288: 95 / 107 Middle; 256 x 32768 x 2048: 73 / 47 Middle).
+// dx: into how many parts the vocabulary is cut so that the tiles fill the chip, of at least eight steps each (with 16,
+// 353 x 18813 x 592 takes 22.5 us, so 18.3).  Few where that is a few microseconds, as long as W, which it reads again for
+// every 32 tokens, is small (1 x 8192 x 1024: 7.4 us / 10.5 Middle, 128 x 8192 x 1024 12.2 / 13.9; 1 x 32768 x 2048 26.6 /
+// 24.8, 40 x 65536 x 4096 139 / 105); Large where each compute unit has twenty of its steps or more, if not most of a
+// tile is empty (412 x 21975 x 2512: 54 / 60 Middle, 96 x 65536 x 4096 117 / 121, 1021 x 32003 x 1288 79 / 98; 1024 x
+// 16384 x 1024, with 16 steps, 38.4 / 37.6, 353 x 18813 x 592, with seven, 23.6 / 18.3).
 struct DxPlan {
   int shape, token_tiles, hidden_tiles, parts, split_steps;
   bool separate;  // the parts are kept and added
@@ -871,12 +875,13 @@ struct DxPlan {
 DxPlan dx_plan(const Pieces& p, int64_t tokens, int hidden, bool separate) {
   DxPlan d;
   const int steps = p.tiles * (kTile / kStepK);
-  const int64_t again = (int64_t)(tiles(tokens, Few::kR) - 1) * p.tiles * kTile * hidden * 2;
-  d.shape = again <= 64 << 20 && tokens <= 256 ? kFew : tiles(tokens) * tiles(hidden) < 24 ? kMiddle : kLarge;
+  const int64_t w_reads = (int64_t)tiles(tokens, Few::kR) * p.tiles * kTile * hidden * 2;
+  const int64_t large_steps = (int64_t)tiles(tokens) * tiles(hidden) * steps;
+  d.shape = tokens <= 256 && w_reads <= 96 << 20 ? kFew : tokens > 96 && large_steps >= 20 * kComputeUnits ? kLarge : kMiddle;
   const int l = d.shape == kLarge ? Large::kL : d.shape == kMiddle ? Middle::kL : Few::kL, r = d.shape == kLarge ? Large::kR : d.shape == kMiddle ? Middle::kR : Few::kR;
   d.token_tiles = tiles(tokens, r);
   d.hidden_tiles = tiles(hidden, l);
-  const int64_t slots = d.shape == kLarge ? kComputeUnits : 2 * kComputeUnits;  // (Few with one per unit: 16 x 131072 x 4096 258 us instead of 199)
+  const int64_t slots = d.shape == kLarge ? kComputeUnits : 2 * kComputeUnits;  // (Middle with one per unit: 171 x 34664 x 1640 54 us instead of 40)
   const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, slots / ((int64_t)d.token_tiles * d.hidden_tiles)));
   d.split_steps = (steps + parts - 1) / parts;
   d.parts = (steps + d.split_steps - 1) / d.split_steps;
@@ -1003,7 +1008,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
       g.with_sums = g.parts && behind;
       auto go = [&](auto s) {
         typedef decltype(s) S;
-        hipLaunchKernelGGL((dx_kernel<T, S>), dim3((unsigned)(g.token_tiles * g.hidden_tiles + g.with_sums), plan.parts), dim3(S::kThreads), 0, stream, p, g, totals);
+        hipLaunchKernelGGL((dx_kernel<T, S>), dim3((unsigned)(g.token_tiles * g.hidden_tiles * plan.parts + g.with_sums)), dim3(S::kThreads), 0, stream, p, g, totals);
         return launched("dx_kernel");
       };
       if ((rc = plan.shape == kLarge ? go(LargeDx()) : plan.shape == kMiddle ? go(Middle()) : go(Few()))) return rc;
