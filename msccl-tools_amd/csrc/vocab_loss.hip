@@ -321,7 +321,7 @@ struct TokenArgs {
   const float* logits;
   const int* pos;
   const char* x;
-  int64_t x_stride, dx_stride;
+  int64_t x_stride, kept_stride, dx_stride;
   char *kept_x, *dx;   // [rows][hidden] for dw; and dx, where a token without a row has zeros
   int hidden;
   int tokens, second;  // kLogits: G's second rows begin at row `second`; rows between are zeros
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
   if constexpr (MODE != kStats) {
     const int row = a.pos ? a.pos[at] : (int)blockIdx.x;
     for (int d = (blockIdx.y * 256 + threadIdx.x) * 8; d < a.hidden; d += gridDim.y * 256 * 8) {
-      if (row >= 0) *(x8*)(a.kept_x + ((int64_t)row * a.hidden + d) * 2) = label == -1 ? x8{} : *(const x8*)(a.x + blockIdx.x * a.x_stride + d * 2);
+      if (row >= 0) *(x8*)(a.kept_x + row * a.kept_stride + d * 2) = label == -1 ? x8{} : *(const x8*)(a.x + blockIdx.x * a.x_stride + d * 2);
       else *(x8*)(a.dx + blockIdx.x * a.dx_stride + d * 2) = x8{};
     }
     if (MODE == kGradient || row < 0) return;
@@ -555,7 +555,7 @@ static_assert(kUnitRows == kStepK, "a step of dx's product is a unit");
 
 struct GradArgs {
   const void* g;     // [rows][tiles * kTile]
-  const char* x;     // [rows][hidden]
+  const char* x;     // the kept one
   const int *live, *idx;  // rows, and a row's token; null: all tokens, in order
   Labels labels;
   int64_t token0;
@@ -840,17 +840,21 @@ int check_call(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool 
   return MSCCLX_OK;
 }
 
+// Rows of the kept x begin on cache lines.
+int64_t kept_stride(int hidden) { return ((int64_t)hidden * 2 + 127) / 128 * 128; }
+
 int tiles(int64_t n, int of = kTile) { return (int)((n + of - 1) / of); }
 
 enum { kLarge, kMiddle, kThin, kFew };
 // Which shape a product takes.  Figures: us of the kernel with the shape / with the next best, by tokens x vocabulary x
 // hidden in bf16, W from memory.  Logits: Few up to four rounds of its workgroups (128 x 8192 x 1024: 10.4 / 17.9
 // Middle; 1 x 32768 x 4096: 80 / 101; 40 x 65536 x 4096: 168 / 182) but not where W would be read again from memory for
-// every 32 tokens (128 x 65536 x 4096: 245 / 187 Middle); Large once its tiles fill the chip (384 x 32768 x 2048: 71 /
-// 91 Middle) and are not half empty, else Middle (256 x 32768 x 2048: 60 / 73 Large).
+// every 32 tokens (128 x 65536 x 4096: 245 / 187 Middle); Middle for as long as its tiles are one round (256 x 32768 x
+// 2048: 60 / 73 Large, 300 x 20000 x 1024 23 / 31), Large from there on (171 x 34664 x 1640: 67 / 80 Middle, 1200 x 12000 x
+// 4000 129 / 158, 500 x 32768 x 2048 74 / 97).
 int logits_shape(const Pieces& p, int64_t tokens) {
   if (tokens <= 256 && (int64_t)tiles(tokens, Few::kR) * p.tiles * (kTile / Few::kL) <= 4 * kComputeUnits) return kFew;
-  return tokens <= 128 || (int64_t)tiles(tokens) * p.tiles < kComputeUnits ? kMiddle : kLarge;
+  return tokens <= 128 || (int64_t)tiles(tokens, Middle::kR) * p.tiles * (kTile / Middle::kL) <= 2 * kComputeUnits ? kMiddle : kLarge;
 }
 // dw writes more than it reads where tokens are few; workgroups then hide each other's loads and stores (16 x 131072 x
 // 4096: 222 Thin / 285 Large, 200 x 20000 x 3000 47 / 55, 300 x 20000 x 1024 25 / 28 Middle; 500 x 32768 x 2048 80 / 82
@@ -862,31 +866,44 @@ int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 384
 // behind the first ones are zeros.
 int second_row(int64_t tokens) { return tokens <= 16 ? 16 : tokens <= 32 ? 32 : (int)((tokens + kStepK - 1) / kStepK * kStepK); }
 
-// dx: into how many parts the vocabulary is cut so that the tiles fill the chip, of at least eight steps each (with 16,
-// 353 x 18813 x 592 takes 22.5 us, so 18.3).  Few where that is a few microseconds, as long as W, which it reads again for
-// every 32 tokens, is small (1 x 8192 x 1024: 7.4 us / 10.5 Middle, 128 x 8192 x 1024 12.2 / 13.9; 1 x 32768 x 2048 26.6 /
-// 24.8, 40 x 65536 x 4096 139 / 105); Large where each compute unit has twenty of its steps or more, if not most of a
-// tile is empty (412 x 21975 x 2512: 54 / 60 Middle, 96 x 65536 x 4096 117 / 121, 1021 x 32003 x 1288 79 / 98; 1024 x
-// 16384 x 1024, with 16 steps, 38.4 / 37.6, 353 x 18813 x 592, with seven, 23.6 / 18.3).
+// dx: the shape, and into how many parts the vocabulary is cut so that the last round of tiles fills the chip, by what
+// each would take: rounds of the slots, each of split_steps steps and 6 us around them, and the parts written and added.
+// A step takes 1.25 us in Large, 0.9 in Middle with two workgroups on a unit (1.5 in a long product, which slows the clock,
+// but then for both).  By tokens x vocabulary x hidden: 4096 x 32768 x 4104, 272 large tiles, 1100 us and 70 to add in four
+// parts, 1625 in one; 6000 x 8000 x 3504, 336 large tiles, 340 in one part, 306 and 84 to add in two.  412 x 21975 x 2512:
+// Large 54 us / Middle 60, 1021 x 32003 x 1288 79 / 98, 353 x 18813 x 592 24 / 18, 8192 x 2048 x 1024 45 / 37.  No part has
+// less than eight steps (the adding is dw's: with four, 1024 x 4096 x 512 takes 3 us longer there).  Large not where most
+// of its tile would be empty (64 x 131072 x 4096: 209 / 203 Middle).  Few where all is a few microseconds, as long as W,
+// which it reads again for every 32 tokens, is small (1 x 8192 x 1024: 7.4 us / 10.5 Middle, 128 x 8192 x 1024 12.2 / 13.9;
+// 1 x 32768 x 2048 26.6 / 24.8, 40 x 65536 x 4096 139 / 105).
 struct DxPlan {
   int shape, token_tiles, hidden_tiles, parts, split_steps;
   bool separate;  // the parts are kept and added
 };
 DxPlan dx_plan(const Pieces& p, int64_t tokens, int hidden, bool separate) {
-  DxPlan d;
   const int steps = p.tiles * (kTile / kStepK);
   const int64_t w_reads = (int64_t)tiles(tokens, Few::kR) * p.tiles * kTile * hidden * 2;
-  const int64_t large_steps = (int64_t)tiles(tokens) * tiles(hidden) * steps;
-  d.shape = tokens <= 256 && w_reads <= 96 << 20 ? kFew : tokens > 96 && large_steps >= 20 * kComputeUnits ? kLarge : kMiddle;
-  const int l = d.shape == kLarge ? Large::kL : d.shape == kMiddle ? Middle::kL : Few::kL, r = d.shape == kLarge ? Large::kR : d.shape == kMiddle ? Middle::kR : Few::kR;
-  d.token_tiles = tiles(tokens, r);
-  d.hidden_tiles = tiles(hidden, l);
-  const int64_t slots = d.shape == kLarge ? kComputeUnits : 2 * kComputeUnits;  // (Middle with one per unit: 171 x 34664 x 1640 54 us instead of 40)
-  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(steps / 8, slots / ((int64_t)d.token_tiles * d.hidden_tiles)));
-  d.split_steps = (steps + parts - 1) / parts;
-  d.parts = (steps + d.split_steps - 1) / d.split_steps;
-  d.separate = separate || d.parts > 1;
-  return d;
+  // one part in 32 bits, written and read; the same for 32 counts of tokens, as all of a plan is
+  const double part_us = (double)tiles(tokens, 32) * 32 * hidden * 8 / 3.5e6;
+  DxPlan best;
+  double best_us = INFINITY;
+  auto consider = [&](int shape, int l, int r, int slots, double step_us, bool fill_once) {
+    const int64_t token_tiles = tiles(tokens, r), hidden_tiles = tiles(hidden, l), all = token_tiles * hidden_tiles;
+    for (int64_t parts = 1; parts == 1 || (parts <= steps / 8 && all * parts <= (fill_once ? 1 : 16) * slots); ++parts) {
+      const int split_steps = (int)((steps + parts - 1) / parts);
+      if ((steps + split_steps - 1) / split_steps != parts) continue;
+      const bool kept = separate || parts > 1;
+      const double us = (double)((all * parts + slots - 1) / slots) * (split_steps * step_us + 6) + (kept ? parts * part_us : 0);
+      if (us < best_us) best_us = us, best = DxPlan{shape, (int)token_tiles, (int)hidden_tiles, (int)parts, split_steps, kept};
+    }
+  };
+  if (tokens <= 256 && w_reads <= 96 << 20) {
+    consider(kFew, Few::kL, Few::kR, 2 * kComputeUnits, 0.5, true);
+  } else {
+    consider(kMiddle, Middle::kL, Middle::kR, 2 * kComputeUnits, 0.9, false);
+    if (tokens > 96) consider(kLarge, Large::kL, Large::kR, kComputeUnits, 1.25, false);
+  }
+  return best;
 }
 
 template <class T, int MODE>
@@ -962,6 +979,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
       t.x = a.x;
       t.x_stride = a.x_stride;
       t.kept_x = c.x;
+      t.kept_stride = kept_stride(d.hidden);
       t.dx = (char*)io->dx + at * io->dx_stride * 2;
       t.dx_stride = io->dx_stride * 2;
       t.hidden = d.hidden;
@@ -983,7 +1001,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
     GradArgs g = {};
     g.g = c.e;
     g.x = c.x;
-    g.x_stride = (int64_t)d.hidden * 2;
+    g.x_stride = kept_stride(d.hidden);
     if (ordered) g.live = c.order.live + at / h->piece, g.idx = c.order.idx + at;
     g.labels = c.labels;
     g.token0 = at;
@@ -1094,7 +1112,7 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
     h->off_pos = take(n * 4);
     h->off_idx = take(n * 4);
     h->off_live = take((n / h->piece + 1) * 4);
-    h->off_x = d.gradients ? take((uint64_t)h->piece * d.hidden * 2) : 0;
+    h->off_x = d.gradients ? take((uint64_t)h->piece * kept_stride(d.hidden)) : 0;
     const uint64_t wide = (uint64_t)p.tiles * kTile;
     h->off_stats = take(std::max(std::min<uint64_t>(h->piece, 256) * (wide / (Few::kL / Few::kWavesL)), (uint64_t)h->piece * (wide / (Middle::kL / Middle::kWavesL))) * sizeof(float2));
     h->off_logits = d.gradients ? take(std::min<uint64_t>(n, kWideTokens) * wide * 4) : 0;
