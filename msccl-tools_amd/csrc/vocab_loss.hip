@@ -309,6 +309,11 @@ template <class V, class F> __device__ __forceinline__ V block_reduce(V v, F f, 
   return v;
 }
 
+// x with its rows on cache lines, a workgroup per row.
+__global__ void __launch_bounds__(256) align_kernel(const char* x, int64_t x_stride, char* out, int64_t out_stride, int bytes) {
+  for (int at = threadIdx.x * 16; at < bytes; at += 256 * 16) *(u32x4*)(out + blockIdx.x * out_stride + at) = *(const u32x4*)(x + blockIdx.x * x_stride + at);
+}
+
 struct TokenArgs {
   const float2* stats;
   int part;          // vocabulary of one entry
@@ -709,7 +714,7 @@ struct mscclx_vocab_loss {
   Pieces pieces;          // without pointers
   int64_t vocab = 0;
   int64_t piece = 0;      // tokens per piece
-  uint64_t off_z = 0, off_loss = 0, off_factor = 0, off_back = 0, off_stats = 0, off_e = 0, off_sums = 0, off_parts = 0, off_logits = 0, off_x = 0, off_pos = 0, off_idx = 0, off_live = 0, bytes = 0;
+  uint64_t off_z = 0, off_loss = 0, off_factor = 0, off_back = 0, off_stats = 0, off_e = 0, off_sums = 0, off_parts = 0, off_logits = 0, off_x = 0, off_aligned = 0, off_pos = 0, off_idx = 0, off_live = 0, bytes = 0;
 };
 
 namespace {
@@ -771,7 +776,7 @@ struct Call {
   float *z_label, *row_loss, *factor, *back, *sums, *parts, *logits;
   float2* stats;
   void* e;
-  char* x;
+  char *x, *aligned;
   OrderArgs order;
 };
 
@@ -835,13 +840,15 @@ int check_call(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool 
   c->parts = (float*)(ws + h->off_parts);
   c->logits = (float*)(ws + h->off_logits);
   c->x = ws + h->off_x;
+  c->aligned = ws + h->off_aligned;
   c->order = OrderArgs{h->piece, (int*)(ws + h->off_pos), (int*)(ws + h->off_idx), (int*)(ws + h->off_live)};
   c->sums = h->off_sums ? (float*)(ws + h->off_sums) : nullptr;
   return MSCCLX_OK;
 }
 
-// Rows of the kept x begin on cache lines.
-int64_t kept_stride(int hidden) { return ((int64_t)hidden * 2 + 127) / 128 * 128; }
+constexpr int kLine = 128;
+// Rows of the kept and of the aligned x begin on cache lines.
+int64_t kept_stride(int hidden) { return ((int64_t)hidden * 2 + kLine - 1) / kLine * kLine; }
 
 int tiles(int64_t n, int of = kTile) { return (int)((n + of - 1) / of); }
 
@@ -855,6 +862,13 @@ enum { kLarge, kMiddle, kThin, kFew };
 int logits_shape(const Pieces& p, int64_t tokens) {
   if (tokens <= 256 && (int64_t)tiles(tokens, Few::kR) * p.tiles * (kTile / Few::kL) <= 4 * kComputeUnits) return kFew;
   return tokens <= 128 || (int64_t)tiles(tokens, Middle::kR) * p.tiles * (kTile / Middle::kL) <= 2 * kComputeUnits ? kMiddle : kLarge;
+}
+// A row of x that begins within a cache line has each step's 128 bytes in two; x is copied first where that is short
+// against the product (forward and run in us, with the copy / without: 4096 x 32768 x 4104 900 / 983 and 3070 / 3180, 1500 x
+// 40000 x 2008 241 / 250 and 753 / 770, 1021 x 32003 x 1288 90 / 90 and 312 / 321; but 8192 x 8000 x 904 148 / 145, 1200 x
+// 12000 x 4000 105 / 102).  W's rows, which the same holds for, are read once: a copy of them would cost more.
+bool align_pays(const Pieces& p, int64_t tokens, int hidden) {
+  return p.tiles >= 64 && (int64_t)tiles(tokens) * p.tiles * tiles(hidden, kStepK) >= 40 * kComputeUnits;
 }
 // dw writes more than it reads where tokens are few; workgroups then hide each other's loads and stores (16 x 131072 x
 // 4096: 222 Thin / 285 Large, 200 x 20000 x 3000 47 / 55, 300 x 20000 x 1024 25 / 28 Middle; 500 x 32768 x 2048 80 / 82
@@ -961,6 +975,12 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
     a.lse = io->lse;
     if (now > 0) {
       const int shape = logits_shape(p, now);
+      if (shape == kLarge && ((uintptr_t)a.x | a.x_stride) % kLine && align_pays(p, now, d.hidden)) {
+        hipLaunchKernelGGL(align_kernel, dim3(now), dim3(256), 0, stream, a.x, a.x_stride, c.aligned, kept_stride(d.hidden), d.hidden * 2);
+        if ((rc = launched("align_kernel"))) return rc;
+        a.x = c.aligned;
+        a.x_stride = kept_stride(d.hidden);
+      }
       if (wide) a.e = c.logits;
       if ((rc = wide ? launch_logits<T, kLogits>(shape, p, a, stream) : !forward ? launch_logits<T, kGradient>(shape, p, a, stream) : backward ? launch_logits<T, kKeep>(shape, p, a, stream) : launch_logits<T, kStats>(shape, p, a, stream)))
         return rc;
@@ -976,8 +996,8 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
       t.e = c.e;
       t.logits = c.logits;
       t.pos = a.pos;
-      t.x = a.x;
-      t.x_stride = a.x_stride;
+      t.x = (const char*)io->x + at * io->x_stride * 2;
+      t.x_stride = io->x_stride * 2;
       t.kept_x = c.x;
       t.kept_stride = kept_stride(d.hidden);
       t.dx = (char*)io->dx + at * io->dx_stride * 2;
@@ -1113,6 +1133,7 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
     h->off_idx = take(n * 4);
     h->off_live = take((n / h->piece + 1) * 4);
     h->off_x = d.gradients ? take((uint64_t)h->piece * kept_stride(d.hidden)) : 0;
+    h->off_aligned = align_pays(p, h->piece, d.hidden) ? take((uint64_t)h->piece * kept_stride(d.hidden)) : 0;
     const uint64_t wide = (uint64_t)p.tiles * kTile;
     h->off_stats = take(std::max(std::min<uint64_t>(h->piece, 256) * (wide / (Few::kL / Few::kWavesL)), (uint64_t)h->piece * (wide / (Middle::kL / Middle::kWavesL))) * sizeof(float2));
     h->off_logits = d.gradients ? take(std::min<uint64_t>(n, kWideTokens) * wide * 4) : 0;

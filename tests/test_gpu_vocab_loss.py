@@ -107,6 +107,24 @@ def test_strides_labels_of_32_bits_and_what_lies_beside(dtype):
         assert bool(torch.isnan(b).all())
 
 
+@pytest.mark.parametrize("tokens, piece_tokens", [(1100, 1280), (2100, 1280)])
+def test_rows_that_begin_within_a_cache_line(tokens, piece_tokens):
+    """The same bits wherever the rows of x begin; what lies between them and behind them is not used."""
+    hidden, rows = 2000, [8200, 8300]
+    x, weights, labels, upstream = make(tokens, hidden, rows, torch.bfloat16)
+    op = operator(tokens, hidden, rows, "bfloat16", reduction="none", piece_bytes=piece_tokens * 16640 * 2)
+    want = None
+    for stride, offset in ((2048, 0), (2000, 0), (2048, 8), (2040, 32)):
+        buffer = torch.full((tokens * stride + 64,), float("nan"), dtype=x.dtype, device="cuda")
+        placed = buffer[offset:offset + tokens * stride].view(tokens, stride)[:, :hidden].copy_(x)
+        got = op.run(placed, weights, labels, upstream)
+        got = [*got[:3], *got[3], *op.forward(placed, weights, labels), op.backward(placed, weights, labels, got[1], upstream)[0]]
+        want = want or got
+        assert all(bool(torch.isfinite(t).all()) for t in got) and all(torch.equal(a, b) for a, b in zip(got, want))
+    z = x.float() @ torch.cat(weights).float().t()
+    assert float((torch.logsumexp(z, 1) - want[1]).abs().max()) < 1e-3
+
+
 def test_matrices_side_by_side_in_one_buffer():
     """x and dx, and each rank's weights and dw, as columns of one buffer; the ranks' weights twice the same memory.  A dw for two ranks is refused."""
     from msccl.executor import MscclxError
