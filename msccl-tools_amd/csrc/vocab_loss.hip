@@ -132,6 +132,7 @@ struct LogitsArgs {
   int64_t x_stride;  // bytes
   int64_t w_stride;
   int hidden, tokens, token_tiles;
+  int apart;         // so many tiles of the vocabulary begin at the same k; 0: all
   int64_t token0;    // of the labels, lse and factors
   Labels labels;
   Upstream upstream;
@@ -168,10 +169,7 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
   const int n0 = tt * TR, tokens = min(TR, a.tokens - n0);
   f32x4 acc[Product::FL][Product::FR] = {};
   {
-    // With one workgroup per compute unit all would ask for the same few bytes of each row of W at a time, which lie a
-    // power of two apart; each begins at another k (the loss of 1 token x 32768 x 2048: 36.2 us in step, 32.2 so; with
-    // more workgroups it costs 3 %)
-    const int steps = (a.hidden + kStepK - 1) / kStepK, first = TR == Few::kR && gridDim.x <= kComputeUnits ? at % steps : 0;
+    const int steps = (a.hidden + kStepK - 1) / kStepK, first = a.apart ? at / a.apart % steps : 0;
     typename Product::LLanes ll;
     typename Product::RLanes rl;
     ll.place(threadIdx.x, a.w_stride, [&](int i) { return Unit(pieces, ends, at * (TL / kUnitRows) + i).rows; });
@@ -954,7 +952,14 @@ int launch_logits(int shape, const Pieces& p, LogitsArgs& a, hipStream_t stream)
   auto go = [&](auto s) {
     typedef decltype(s) S;
     a.token_tiles = tiles(a.tokens, S::kR);
-    hipLaunchKernelGGL((logits_kernel<T, MODE, S>), dim3((unsigned)(a.token_tiles * p.tiles * (kTile / S::kL))), dim3(S::kThreads), 0, stream, p, a);
+    const int grid = a.token_tiles * p.tiles * (kTile / S::kL);
+    // In step, all workgroups ask for the same 128 bytes of each row of W at a time.  Where rows lie a multiple of 4 KiB
+    // apart those are in few of memory's channels, so every eight tiles begin at another k (128 x 65536 x 4096: 146 us, in
+    // step 175; 256 x 32768 x 2048 51 / 60, 500 x 32768 x 2048 67 / 72; not with so many tokens that W's reads hide, 4096 x
+    // 32768 x 4096 850 / 841, nor with one tile of a few, 16 x 131072 x 4096 264 / 256).  With one workgroup of Few per
+    // compute unit each begins at its own (the loss of 1 token x 32768 x 2048: 32.2 us, in step 36.2).
+    a.apart = S::kR == Few::kR && grid <= kComputeUnits ? 1 : a.tokens > Few::kR && a.tokens <= 2048 && a.w_stride % 4096 == 0 ? 8 : 0;
+    hipLaunchKernelGGL((logits_kernel<T, MODE, S>), dim3((unsigned)grid), dim3(S::kThreads), 0, stream, p, a);
     return launched("logits_kernel");
   };
   if constexpr (MODE != kLogits)  // (up to kWideTokens tokens)
