@@ -53,6 +53,10 @@ struct Pieces {
   int unit0[kMaxRanks + 1];  // the rank's first unit
   int first[kMaxRanks + 1];  // the rank's first row in the whole vocabulary
   const char* w[kMaxRanks];
+  __host__ __device__ int64_t columns() const { return (int64_t)tiles * kTile; }  // of E and G
+  // Rows of a multiple of 2^16 columns would meet in one of memory's channels: they lie a cache line further apart (dx of
+  // 2048 x 65536 x 1024: 251 us, without 280; 4096 x 65536 x 2048 837 / 852; with 32768 rows no shorter).
+  __host__ __device__ int64_t stride() const { return columns() + (columns() % 65536 == 0 ? 64 : 0); }
 };
 
 // Which rank holds something: the ranks' ends, one in each lane, are compared at once.  (A loop over the ranks waits
@@ -139,7 +143,7 @@ struct LogitsArgs {
   const int* pos;    // a token's row of E or G, -1: none; null: its own
   float2* stats;     // [tokens][waves' parts of the vocabulary]
   float* z_label;
-  void* e;           // [rows][tiles * kTile]: E or G, or with kLogits the logits in 32 bits
+  void* e;           // [rows][stride]: E or G, or with kLogits the logits in 32 bits
   const float* lse;
 };
 
@@ -181,7 +185,7 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
                  }, a.hidden, first),
                  rl, RowSource<TR>([&](int i) { return a.x + (n0 + i * kUnitRows) * a.x_stride; }, a.hidden, first), acc);
   }
-  const int64_t ld = (int64_t)pieces.tiles * kTile;
+  const int64_t ld = pieces.stride();
   const int lane = threadIdx.x & 63, part = (threadIdx.x >> 6) % Shape::kWavesL;
   // the wave's part of the vocabulary: whole units, or part of one
   constexpr int kOfWave = kPart < kUnitRows ? kPart : kUnitRows, kWaveUnits = kPart / kOfWave, kUnitFragments = kOfWave / 16;
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
         });
 #pragma unroll
         for (int d = 16; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-        if (live && lane < 16) a.stats[(n0 + n) * (ld / kPart) + at * TL / kPart + part] = make_float2(m, sum);
+        if (live && lane < 16) a.stats[(n0 + n) * (pieces.columns() / kPart) + at * TL / kPart + part] = make_float2(m, sum);
       }
     }
   };
@@ -339,12 +343,12 @@ struct TokenArgs {
 template <class T, int MODE>
 __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const TokenArgs a) {
   __shared__ float shared[4];
-  const int64_t ld = (int64_t)pieces.tiles * kTile, at = a.token0 + blockIdx.x;
-  const int parts = (int)(ld / a.part);
+  const int64_t ld = pieces.stride(), columns = pieces.columns(), at = a.token0 + blockIdx.x;
+  const int parts = (int)(columns / a.part);
   const float2* stats = a.stats + (int64_t)blockIdx.x * parts;
   typedef typename Half<T>::x8 x8;
   if (MODE == kLogits && (int)blockIdx.x >= a.tokens) {
-    for (int64_t v = (blockIdx.y * 256 + threadIdx.x) * 8; v < ld; v += gridDim.y * 256 * 8) *(x8*)((T*)a.e + blockIdx.x * ld + v) = x8{};
+    for (int64_t v = (blockIdx.y * 256 + threadIdx.x) * 8; v < columns; v += gridDim.y * 256 * 8) *(x8*)((T*)a.e + blockIdx.x * ld + v) = x8{};
     return;
   }
   const int label = a.labels.get(at);
@@ -385,7 +389,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
       of_label = expm1f((__builtin_fmaf(z_label, kLog2e, -base) - log_sum) * (float)kLn2) * g * kUnit<T>;
     }
     T* e = (T*)a.e + row * ld;
-    for (int64_t v = (blockIdx.y * 256 + threadIdx.x) * 8; v < ld; v += gridDim.y * 256 * 8) {
+    for (int64_t v = (blockIdx.y * 256 + threadIdx.x) * 8; v < columns; v += gridDim.y * 256 * 8) {
       float p[8];
       if constexpr (MODE != kLogits) {
         const float top = stats[v / a.part].x;
@@ -557,7 +561,7 @@ struct PieceSource {
 static_assert(kUnitRows == kStepK, "a step of dx's product is a unit");
 
 struct GradArgs {
-  const void* g;     // [rows][tiles * kTile]
+  const void* g;     // [rows][stride]
   const char* x;     // the kept one
   const int *live, *idx;  // rows, and a row's token; null: all tokens, in order
   Labels labels;
@@ -599,7 +603,7 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dx_kernel(cons
   int tt, ht;
   tile_in_band(in_order % tiles, token_tiles, a.hidden_tiles, &tt, &ht);
   const int n0 = tt * TR, d0 = ht * TL, tokens = min(TR, all - n0), width = min(TL, a.hidden - d0);
-  const int64_t ld = (int64_t)pieces.tiles * kTile;
+  const int64_t ld = pieces.stride();
   const int step0 = part * a.split_steps, steps = min(a.split_steps, pieces.tiles * (kTile / kStepK) - step0);
   f32x4 acc[Product::FL][Product::FR] = {};
   {
@@ -687,7 +691,7 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dw_kernel(cons
   int at, ht;
   tile_of(id, pieces.tiles * (kTile / TR), a.hidden_tiles, &at, &ht);
   const int d0 = ht * TL, width = min(TL, a.hidden - d0);
-  const int64_t ld = (int64_t)pieces.tiles * kTile;
+  const int64_t ld = pieces.stride();
   f32x4 acc[Product::FL][Product::FR] = {};
   {
     typename Product::LLanes ll;
@@ -1155,9 +1159,9 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
       delete h;
       return fail(MSCCLX_ERR_INVALID_ARG, "the vocabulary is empty");
     }
-    const uint64_t row = (uint64_t)p.tiles * kTile * 2;  // bytes of E for a token
+    const uint64_t row = (uint64_t)p.stride() * 2;  // bytes of E for a token
     const uint64_t budget = d.piece_bytes ? d.piece_bytes : MSCCLX_VOCAB_LOSS_PIECE_BYTES;
-    const int64_t fit = (int64_t)(budget / row / kTile * kTile);
+    const int64_t fit = (int64_t)(budget / ((uint64_t)p.columns() * 2) / kTile * kTile);
     h->piece = std::max<int64_t>(1, std::min<int64_t>(d.max_tokens, std::max<int64_t>(kTile, std::min<int64_t>(fit, 1 << 20))));
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
@@ -1177,7 +1181,7 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
     h->off_aligned = align_pays(p, h->piece, d.hidden) ? take((uint64_t)h->piece * kept_stride(d.hidden)) : 0;
     const uint64_t wide = (uint64_t)p.tiles * kTile;
     h->off_stats = take(std::max(std::min<uint64_t>(h->piece, 256) * (wide / (Few::kL / Few::kWavesL)), (uint64_t)h->piece * (wide / (Middle::kL / Middle::kWavesL))) * sizeof(float2));
-    h->off_logits = d.gradients ? take(std::min<uint64_t>(n, kWideTokens) * wide * 4) : 0;
+    h->off_logits = d.gradients ? take(std::min<uint64_t>(n, kWideTokens) * p.stride() * 4) : 0;
     h->off_e = d.gradients ? take(std::max<uint64_t>(h->piece, std::min<uint64_t>(n, kWideTokens) + kWideTokens) * row) : 0;
     h->off_sums = d.gradients && d.max_tokens > h->piece ? take((uint64_t)p.tiles * kTile * d.hidden * 4) : 0;
     uint64_t parts = 0;  // dx's parts at the token count that needs most of them

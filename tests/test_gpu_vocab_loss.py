@@ -71,9 +71,9 @@ def test_several_pieces_of_tokens(tokens, reduction, dtype):
     check_all(op, *make(tokens, 128, rows, DTYPES[dtype], seed=5), reduction)
 
 
-@pytest.mark.parametrize("tokens, hidden, rows", [(2100, 3976, [500, 530]), (600, 1000, [9000, 8000]), (400, 72, [20000, 30000]), (2, 576, [9000, 7001])])
+@pytest.mark.parametrize("tokens, hidden, rows", [(2100, 3976, [500, 530]), (600, 1000, [9000, 8000]), (400, 72, [20000, 30000]), (140, 64, [65536]), (20, 64, [65536]), (2, 576, [9000, 7001])])
 def test_sizes_where_dx_is_cut(tokens, hidden, rows):
-    """More than one round of tiles, large and middle tiles in many parts, and many parts of few values."""
+    """More than one round of tiles, large and middle tiles in many parts, many parts of few values, and rows of G that lie further apart than they are long."""
     op = operator(tokens, hidden, rows, "bfloat16", reduction="none")
     x, weights, labels, upstream = make(tokens, hidden, rows, torch.bfloat16)
     check_all(op, x, weights, labels, upstream, "none")
