@@ -885,11 +885,11 @@ int tiles(int64_t n, int of = kTile) { return (int)((n + of - 1) / of); }
 
 enum { kLarge, kMiddle, kThin, kFew };
 // Which shape a product takes.  Figures: us of the kernel with the shape / with the next best, by tokens x vocabulary x
-// hidden in bf16, W from memory.  Logits: Few up to four rounds of its workgroups (128 x 8192 x 1024: 10.4 / 17.9
-// Middle; 1 x 32768 x 4096: 80 / 101; 40 x 65536 x 4096: 168 / 182) but not where W would be read again from memory for
-// every 32 tokens (128 x 65536 x 4096: 245 / 187 Middle); Middle for as long as its tiles are one round (256 x 32768 x
-// 2048: 60 / 73 Large, 300 x 20000 x 1024 23 / 31), Large from there on (171 x 34664 x 1640: 67 / 80 Middle, 1200 x 12000 x
-// 4000 129 / 158, 500 x 32768 x 2048 74 / 97).
+// hidden in bf16, W from memory, all tiles in step.  Logits: Few up to four rounds of its workgroups (128 x 8192 x
+// 1024: 10.4 / 17.9 Middle; 1 x 32768 x 4096: 80 / 101; 40 x 65536 x 4096: 168 / 182) but not where W would be read
+// again from memory for every 32 tokens (128 x 65536 x 4096: 245 / 187 Middle); Middle for as long as its tiles are one
+// round (256 x 32768 x 2048: 60 / 73 Large, 300 x 20000 x 1024 23 / 31), Large from there on (171 x 34664 x 1640: 67 /
+// 80 Middle, 1200 x 12000 x 4000 129 / 158, 500 x 32768 x 2048 74 / 97).
 int logits_shape(const Pieces& p, int64_t tokens) {
   if (tokens <= 256 && (int64_t)tiles(tokens, Few::kR) * p.tiles * (kTile / Few::kL) <= 4 * kComputeUnits) return kFew;
   return tokens <= 128 || (int64_t)tiles(tokens, Middle::kR) * p.tiles * (kTile / Middle::kL) <= 2 * kComputeUnits ? kMiddle : kLarge;
