@@ -113,9 +113,9 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 template <class T> constexpr float kUnit = std::is_same_v<T, _Float16> ? 32768.0f : 1.0f;
 
 // How a workgroup's tile is cut.  Large: one workgroup of eight waves per compute unit.  Middle: two of four waves, for
-// products whose large tiles would not fill the chip.  Thin: four of four waves, each one step at a time, for products
-// that write more than they read.  Few: at most 32 tokens, with four steps of copies under way, because then memory is
-// all that counts.
+// products whose large tiles would not fill the chip.  Small: three, for those whose middle ones would not.  Thin: four
+// of four waves, each one step at a time, for products that write more than they read.  Few: at most 32 tokens, with
+// four steps of copies under way, because then memory is all that counts.
 template <int L, int R, int WL, int WR, int STAGES, int WAVES> struct Shape {  // WAVES: per SIMD, at least
   static constexpr int kL = L, kR = R, kWavesL = WL, kWavesR = WR, kThreads = WL * WR * 64, kWaves = WAVES;
   template <class T, bool LCOL, bool RCOL> using Product = TileProduct<T, L, R, WL, WR, STAGES, LCOL, RCOL>;
@@ -125,6 +125,7 @@ typedef Shape<256, 256, 2, 4, 2, 2> Large;
 // of them.  At 8192 tokens of 4096 and 32768 rows dx takes 1547 us, with 2 x 4 waves 1577.
 typedef Shape<256, 256, 4, 2, 2, 2> LargeDx;
 typedef Shape<128, 128, 2, 2, 2, 2> Middle;
+typedef Shape<128, 64, 2, 2, 2, 3> Small;
 typedef Shape<128, 128, 2, 2, 1, 4> Thin;
 typedef Shape<128, 32, 4, 1, 4, 2> Few;
 
@@ -883,16 +884,23 @@ int64_t kept_stride(int hidden) { return ((int64_t)hidden * 2 + kLine - 1) / kLi
 
 int tiles(int64_t n, int of = kTile) { return (int)((n + of - 1) / of); }
 
-enum { kLarge, kMiddle, kThin, kFew };
+enum { kLarge, kMiddle, kSmall, kThin, kFew };
 // Which shape a product takes.  Figures: us of the kernel with the shape / with the next best, by tokens x vocabulary x
-// hidden in bf16, W from memory, all tiles in step.  Logits: Few up to four rounds of its workgroups (128 x 8192 x
-// 1024: 10.4 / 17.9 Middle; 1 x 32768 x 4096: 80 / 101; 40 x 65536 x 4096: 168 / 182) but not where W would be read
-// again from memory for every 32 tokens (128 x 65536 x 4096: 245 / 187 Middle); Middle for as long as its tiles are one
-// round (256 x 32768 x 2048: 60 / 73 Large, 300 x 20000 x 1024 23 / 31), Large from there on (171 x 34664 x 1640: 67 /
-// 80 Middle, 1200 x 12000 x 4000 129 / 158, 500 x 32768 x 2048 74 / 97).
+// hidden in bf16, W from memory, all tiles in step.  Logits: Few in one round of its workgroups (128 x 8192 x 1024:
+// 10.4 / 13.8 Small, 300 x 3000 x 4096 22 / 39, 512 x 4096 x 2048 21.5 / 23.6; 192 x 12000 x 1000, with 564, 25 / 18),
+// two where W is read no more than twice (1 x 32768 x 4096: 80 / 101 Middle, 40 x 65536 x 4096 168 / 182; 128 x 65536 x
+// 4096 245 / 187); Small while there are no more middle tiles than compute units (1113 x 2880 x 896: 15.7 / 18.2
+// Middle, 600 x 3000 x 1000 17.2 / 20.6, 192 x 12000 x 1000 18.3 / 20.4; 353 x 18813 x 592, with 441, 26 / 21); Middle
+// for as long as its tiles are one round (256 x 32768 x 2048: 60 / 73 Large, 300 x 20000 x 1024 23 / 31), Large from
+// there on (171 x 34664 x 1640: 67 / 80 Middle, 1200 x 12000 x 4000 129 / 158, 500 x 32768 x 2048 74 / 97).
+int64_t most_of_few(const Pieces& p) {
+  const int columns = p.tiles * (kTile / Few::kL);
+  return Few::kR * std::max(2 * kComputeUnits / columns, std::min(2, 4 * kComputeUnits / columns));
+}
 int logits_shape(const Pieces& p, int64_t tokens) {
-  if (tokens <= 256 && (int64_t)tiles(tokens, Few::kR) * p.tiles * (kTile / Few::kL) <= 4 * kComputeUnits) return kFew;
-  return tokens <= 128 || (int64_t)tiles(tokens, Middle::kR) * p.tiles * (kTile / Middle::kL) <= 2 * kComputeUnits ? kMiddle : kLarge;
+  if (tokens <= most_of_few(p)) return kFew;
+  const int64_t middle = (int64_t)tiles(tokens, Middle::kR) * p.tiles * (kTile / Middle::kL);
+  return middle <= kComputeUnits ? kSmall : tokens <= 128 || middle <= 2 * kComputeUnits ? kMiddle : kLarge;
 }
 // A row of x that begins within a cache line has each step's 128 bytes in two; x is copied first where that is short
 // against the product (forward and run in us, with the copy / without: 4096 x 32768 x 4104 900 / 983 and 3070 / 3180, 1500 x
@@ -968,7 +976,7 @@ int launch_logits(int shape, const Pieces& p, LogitsArgs& a, hipStream_t stream)
   };
   if constexpr (MODE != kLogits)  // (up to kWideTokens tokens)
     if (shape == kLarge) return go(Large());
-  return shape == kMiddle ? go(Middle()) : go(Few());
+  return shape == kMiddle ? go(Middle()) : shape == kSmall ? go(Small()) : go(Few());
 }
 
 template <class T>
@@ -1024,7 +1032,8 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
         return rc;
       TokenArgs t = {};
       t.stats = c.stats;
-      t.part = shape == kLarge ? Large::kL / Large::kWavesL : shape == kMiddle ? Middle::kL / Middle::kWavesL : Few::kL / Few::kWavesL;
+      t.part = shape == kLarge ? Large::kL / Large::kWavesL : shape == kFew ? Few::kL / Few::kWavesL : Middle::kL / Middle::kWavesL;
+      static_assert(Small::kL / Small::kWavesL == Middle::kL / Middle::kWavesL, "their entries are of as much vocabulary");
       t.token0 = at;
       t.labels = c.labels;
       t.upstream = upstream;
@@ -1180,7 +1189,7 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
     h->off_x = d.gradients ? take((uint64_t)h->piece * kept_stride(d.hidden)) : 0;
     h->off_aligned = align_pays(p, h->piece, d.hidden) ? take((uint64_t)h->piece * kept_stride(d.hidden)) : 0;
     const uint64_t wide = (uint64_t)p.tiles * kTile;
-    h->off_stats = take(std::max(std::min<uint64_t>(h->piece, 256) * (wide / (Few::kL / Few::kWavesL)), (uint64_t)h->piece * (wide / (Middle::kL / Middle::kWavesL))) * sizeof(float2));
+    h->off_stats = take(std::max(std::min<uint64_t>(h->piece, most_of_few(p)) * (wide / (Few::kL / Few::kWavesL)), (uint64_t)h->piece * (wide / (Middle::kL / Middle::kWavesL))) * sizeof(float2));
     h->off_logits = d.gradients ? take(std::min<uint64_t>(n, kWideTokens) * p.stride() * 4) : 0;
     h->off_e = d.gradients ? take(std::max<uint64_t>(h->piece, std::min<uint64_t>(n, kWideTokens) + kWideTokens) * row) : 0;
     h->off_sums = d.gradients && d.max_tokens > h->piece ? take((uint64_t)p.tiles * kTile * d.hidden * 4) : 0;

@@ -79,6 +79,14 @@ def test_sizes_where_dx_is_cut(tokens, hidden, rows):
     check_all(op, x, weights, labels, upstream, "none")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens, hidden, rows", [(300, 136, [9000, 6001]), (300, 72, [10000]), (100, 72, [3000] * 8), (100, 72, [5000] * 8), (520, 264, [9001, 8000])])
+def test_sizes_of_every_shape_of_logits(tokens, hidden, rows, dtype):
+    """Middle and small tiles with 16-bit probabilities and with logits in 32 bits, and large ones."""
+    op = operator(tokens, hidden, rows, dtype, reduction="sum")
+    check_all(op, *make(tokens, hidden, rows, DTYPES[dtype]), "sum")
+
+
 def test_fewer_tokens_than_set_up_for():
     op = operator(900, 64, [300], "bfloat16", reduction="mean", piece_bytes=1)
     for tokens in (900, 1, 256, 257, 0):
