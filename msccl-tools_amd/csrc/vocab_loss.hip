@@ -422,7 +422,8 @@ struct SumsArgs {
   int mean;
   const float* rows;      // null: no loss
   float* loss;
-  const float* upstream;  // null: no gradients
+  int gradients;          // what they are multiplied by is wanted
+  const float* upstream;  // may be null where there is one for each of no tokens
   float* factor;          // null: one number for all tokens
   float unit;
   float* back;
@@ -457,7 +458,7 @@ __device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shar
     sum = block_reduce(sum, add, shared);
     if (threadIdx.x == 0) *a.loss = (float)(sum / count);
   }
-  if (!a.upstream) return;
+  if (!a.gradients) return;
   if (a.factor) {
     top = block_reduce(top, [](float a, float b) { return fmaxf(a, b); }, (float*)shared);
     for (int64_t n = threadIdx.x; n < a.tokens; n += blockDim.x) {
@@ -994,8 +995,8 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
   // has parts). Up to kWideTokens tokens, rows of zeros cost less than the launch that finds out which they are
   const bool ordered = backward && n > kWideTokens;
   const bool early = backward && (per_token || !forward || ordered);
-  SumsArgs first = {n, c.labels, mean, nullptr, nullptr, io->grad_loss, per_token ? c.factor : nullptr, kUnit<T>, c.back};
-  SumsArgs totals = {n, c.labels, mean, forward && !per_token ? c.row_loss : nullptr, io->loss, backward && !early ? io->grad_loss : nullptr, nullptr, kUnit<T>, c.back};
+  SumsArgs first = {n, c.labels, mean, nullptr, nullptr, 1, io->grad_loss, per_token ? c.factor : nullptr, kUnit<T>, c.back};
+  SumsArgs totals = {n, c.labels, mean, forward && !per_token ? c.row_loss : nullptr, io->loss, backward && !early, io->grad_loss, nullptr, kUnit<T>, c.back};
   auto sums = [&](const SumsArgs& what, const OrderArgs& order) {
     hipLaunchKernelGGL(sums_kernel, dim3(1), dim3(kSumsThreads), 0, stream, what, order);
     return launched("sums_kernel");
