@@ -451,12 +451,11 @@ __device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shar
     }
   }
   auto add = [](double a, double b) { return a + b; };
-  if (!a.mean) count = 1.0;
-  else if (kept >= 0) count = fmax((double)kept, 1.0);
-  else count = fmax(block_reduce(count, add, shared), 1.0);
+  auto counted = [&] { return kept >= 0 ? (double)kept : block_reduce(count, add, shared); };
+  const double divisor = a.mean ? fmax(counted(), 1.0) : 1.0;
   if (a.rows) {
     sum = block_reduce(sum, add, shared);
-    if (threadIdx.x == 0) *a.loss = (float)(sum / count);
+    if (threadIdx.x == 0) *a.loss = (float)(sum / divisor);
   }
   if (!a.gradients) return;
   if (a.factor) {
@@ -468,8 +467,9 @@ __device__ __forceinline__ void sums_over_tokens(const SumsArgs& a, double* shar
     }
   } else {
     top = fabsf(*a.upstream);
+    if (!(top < INFINITY) && counted() == 0.0) top = 0.f;  // zeros stay zeros
   }
-  if (threadIdx.x == 0) *a.back = (float)((double)top / count / a.unit);
+  if (threadIdx.x == 0) *a.back = (float)((double)top / divisor / a.unit);
 }
 
 constexpr int kSumsThreads = 1024, kSumsWaves = kSumsThreads / 64;
@@ -641,8 +641,8 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) dx_kernel(cons
 // dx from the parts of the vocabulary: four values at a time
 template <class T> __device__ __forceinline__ void store_sum(const GradArgs& a, int64_t i, f32x4 sum, float back) {
   const int64_t row = i / a.hidden, token = a.live ? a.idx[row] : row;
-  if (!a.live && a.labels.get(a.token0 + token) == -1) sum = f32x4{0.f, 0.f, 0.f, 0.f};  // (zero times what W holds may be no zero)
-  *(typename Half<T>::x4*)(a.dx + token * a.dx_stride + i % a.hidden * 2) = narrow<T>(sum, back);
+  const bool ignored = !a.live && a.labels.get(a.token0 + token) == -1;  // (zero times what W holds, or times `back`, may be no zero)
+  *(typename Half<T>::x4*)(a.dx + token * a.dx_stride + i % a.hidden * 2) = ignored ? typename Half<T>::x4{} : narrow<T>(sum, back);
 }
 template <class T> __device__ __forceinline__ void add_parts(const GradArgs& a, int adder) {
   const int64_t size = (int64_t)(a.live ? *a.live : a.tokens) * a.hidden, part = (int64_t)a.rows * a.hidden;

@@ -30,3 +30,20 @@ def test_no_tokens_whatever_the_workspace_holds(reduction, dtype):
             assert not bool(torch.cat(out[-1]).count_nonzero()) and out[-2].shape == x.shape
             if len(out) == 4 and reduction != "none":
                 assert float(out[0]) == 0.0
+
+
+@pytest.mark.parametrize("value", ["inf", "-inf", "nan"])
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+@pytest.mark.parametrize("tokens, rows", [(20, [100, 30]), (100, [257]), (100, [64] * 9), (300, [300, 77])])
+def test_one_non_finite_upstream_and_ignored_tokens(tokens, rows, reduction, value):
+    """The number belongs to the tokens that count: an ignored token's dx is 0, and without any other token every gradient is."""
+    x, weights, labels, _ = make(tokens, 72, rows, torch.bfloat16, ignored=0.4)
+    labels[0], labels[1], labels[-1] = IGNORE, 3, IGNORE
+    gone = labels == IGNORE
+    up = torch.tensor(float(value), device="cuda")
+    op = operator(tokens, 72, rows, "bfloat16", reduction=reduction)
+    for dx, dw in both_ways(op, x, weights, labels, up):
+        assert not bool(dx[gone].count_nonzero()) and not bool(torch.isfinite(dx[~gone]).any()) and not bool(torch.isfinite(dw).any())
+    for n in (tokens, 0):
+        for dx, dw in both_ways(op, x[:n], weights, torch.full_like(labels[:n], IGNORE), up):
+            assert not bool(dx.count_nonzero()) and not bool(dw.count_nonzero())
