@@ -137,9 +137,10 @@ class VocabLoss:
         return torch.empty(shape, dtype=dtype, device=self.device)
 
     def _gradients(self, io, n, grad_loss, dx, dweights):
+        """dx, dweights, and what else has to live until the kernels are enqueued."""
         if not self.gradients:
             raise RuntimeError("setup() was called with gradients=False")
-        if grad_loss is None:   # (given back to the allocator at the end of the call, in the order of this stream)
+        if grad_loss is None:
             grad_loss = torch.ones(self._shape(n), dtype=torch.float32, device=self.device)
         io.grad_loss = self._vector("grad_loss", grad_loss, self._shape(n))
         if dx is None:
@@ -154,7 +155,7 @@ class VocabLoss:
         else:
             dweights = list(dweights)
             io.dweight_stride = self._matrices("dweights", dweights, self._dweights)
-        return dx, dweights
+        return dx, dweights, grad_loss
 
     def forward(self, x, weights, labels):
         """(loss, lse): loss is one float32 number, or one per token with reduction="none"; lse one per token."""
@@ -171,9 +172,9 @@ class VocabLoss:
         n = self._tokens(x)
         self._vector("lse", lse, (n,))
         io = self._inputs(n, x, weights, labels, lse)
-        out = self._gradients(io, n, grad_loss, dx, dweights)
+        dx, dweights, _alive = self._gradients(io, n, grad_loss, dx, dweights)
         self._call(self.lib.mscclx_vocab_loss_backward, io)
-        return out
+        return dx, dweights
 
     def run(self, x, weights, labels, grad_loss=None, dx=None, dweights=None):
         """(loss, lse, dx, [dw of each rank]) in one call."""
@@ -181,6 +182,6 @@ class VocabLoss:
         loss, lse = self._new(self._shape(n)), self._new(n)
         io = self._inputs(n, x, weights, labels, lse)
         io.loss = loss.data_ptr()
-        dx, dweights = self._gradients(io, n, grad_loss, dx, dweights)
+        dx, dweights, _alive = self._gradients(io, n, grad_loss, dx, dweights)
         self._call(self.lib.mscclx_vocab_loss_run, io)
         return loss, lse, dx, dweights

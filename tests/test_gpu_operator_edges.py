@@ -47,3 +47,24 @@ def test_one_non_finite_upstream_and_ignored_tokens(tokens, rows, reduction, val
     for n in (tokens, 0):
         for dx, dw in both_ways(op, x[:n], weights, torch.full_like(labels[:n], IGNORE), up):
             assert not bool(dx.count_nonzero()) and not bool(dw.count_nonzero())
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_the_default_upstream_stays_until_the_kernels_are_enqueued(reduction, monkeypatch):
+    """What another thread allocates between the checks and the kernels is other memory."""
+    tokens = 20
+    op = operator(tokens, 64, [100, 30], "bfloat16", reduction=reduction)
+    x, weights, labels, _ = make(tokens, 64, [100, 30], torch.bfloat16)
+    want = op.run(x, weights, labels)
+    call, seen = op._call, []
+
+    def in_between(entry, io):
+        others = [torch.full((tokens,), float("nan"), device="cuda") for _ in range(16)]
+        seen.append(io.grad_loss in [o.data_ptr() for o in others])
+        call(entry, io)
+
+    monkeypatch.setattr(op, "_call", in_between)
+    _, lse, dx, dw = op.run(x, weights, labels)
+    again, _ = op.backward(x, weights, labels, lse)
+    assert seen == [False, False]
+    assert torch.equal(dx, want[2]) and all(torch.equal(a, b) for a, b in zip(dw, want[3])) and bool(torch.isfinite(again).all())
