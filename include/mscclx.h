@@ -236,6 +236,8 @@ int mscclx_plan_time(mscclx_plan* plan, void* stream, int32_t iters, float* ms_o
  * ranks' pieces one under the other.  With z[n][v] = sum over d of x[n][d] w[v][d]:
  *   lse[n] = log sum over v of exp z[n][v],  loss[n] = lse[n] - z[n][label[n]]
  *   dx[n] = sum over v of G[n][v] w[v],  dw[v] = sum over n of G[n][v] x[n],  G[n][v] = g[n] (exp(z[n][v] - lse[n]) - [v = label[n]])
+ * A token with a logit of +inf has lse +inf, as loss lse - z[label], and as G NaN at that row and -g [v = label] at the others.
+ * Logits beyond 2.3e38 in magnitude count as infinite (exponents are held in units of log 2).
  * The logits are not kept (but of up to 128 tokens): tokens go through in pieces whose probabilities, 16 bits each, fit `piece_bytes`.
  * A token whose label is `ignore_index` has loss 0 and adds nothing to either gradient, whatever its x holds; one whose label lies outside the
  * vocabulary otherwise has loss and gradients NaN (and every dw is NaN then).  MEAN divides by the number of tokens that are not

@@ -291,6 +291,15 @@ __global__ void __launch_bounds__(Shape::kThreads, Shape::kWaves) logits_kernel(
           }
           return o;
         });
+        // inf - inf: a part with a logit of +inf has sum 1 at this maximum, and its other logits' E are 0, unless one is NaN
+        if (__any(m == INFINITY)) {
+          bool nan = false;
+          each([&](int row, int rows, int, f32x4 z) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nan |= (WHOLE || row + i < rows) && z[i] != z[i];
+          });
+          if (m == INFINITY) sum = nan ? NAN : 0.25f;
+        }
 #pragma unroll
         for (int d = 16; d < 64; d *= 2) sum += __shfl_xor(sum, d);
         if (live && lane < 16) a.stats[(n0 + n) * (pieces.columns() / kPart) + at * TL / kPart + part] = make_float2(m, sum);
@@ -364,7 +373,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
     base = m == -INFINITY ? 0.f : m;
     for (int h = threadIdx.x; h < parts; h += 256) {
       const float2 s = stats[h];
-      sum += s.y * exp2_of(s.x - base);
+      sum += s.y * (s.x == base ? 1.f : exp2_of(s.x - base));  // (also where both are +inf)
     }
     sum = block_reduce(sum, [](float a, float b) { return a + b; }, shared);
     log_sum = log2f(sum);
@@ -394,7 +403,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
       float p[8];
       if constexpr (MODE != kLogits) {
         const float top = stats[v / a.part].x;
-        const float f = top == -INFINITY ? 0.f : exp2_of(top - lse2) * g;
+        const float f = top == -INFINITY ? 0.f : top == lse2 ? g : exp2_of(top - lse2) * g;  // (both may be +inf)
         const x8 kept = *(const x8*)(e + v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = (float)kept[i] * f;

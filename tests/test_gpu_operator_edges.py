@@ -68,3 +68,49 @@ def test_the_default_upstream_stays_until_the_kernels_are_enqueued(reduction, mo
     again, _ = op.backward(x, weights, labels, lse)
     assert seen == [False, False]
     assert torch.equal(dx, want[2]) and all(torch.equal(a, b) for a, b in zip(dw, want[3])) and bool(torch.isfinite(again).all())
+
+
+@pytest.mark.parametrize("how, dtype", [("overflow", "bfloat16"), ("infinite x", "bfloat16"), ("infinite x", "float16")])
+@pytest.mark.parametrize("tokens, rows", [(20, [200, 100]), (40, [200, 100]), (100, [64] * 9), (300, [200, 100]), (1100, [1000, 900])])
+def test_a_logit_of_infinity(tokens, rows, how, dtype):
+    """lse is +inf, the loss lse - z[label], the other rows' probabilities 0: no other token notices, and of dw only what the formula makes NaN is."""
+    hidden, top, bad, own = 64, 107, 4, 6   # the row whose logit is infinite, the token, and a token whose label is that row
+    x, weights, labels, upstream = make(tokens, hidden, rows, DTYPES[dtype], ignored=0.1)
+    upstream = upstream.abs() + 0.25
+    upstream[bad] = 0.25
+    w = torch.cat(weights)
+    x[:, 0] = 0
+    w[:, 0] = 0 if how == "overflow" else -1
+    w[top, 0] = 1e30 if how == "overflow" else 1
+    x[bad, 0] = 1e30 if how == "overflow" else float("inf")
+    labels[bad], labels[own] = 3, top
+    weights = [t.contiguous() for t in w.split(rows)]
+    others = torch.arange(tokens, device="cuda") != bad
+    forms = loss_forms(x[others], weights, labels[others], "none", IGNORE, upstream[others])
+    op = operator(tokens, hidden, rows, dtype, reduction="none")
+    loss, lse = op.forward(x, weights, labels)
+    assert float(lse[bad]) == float("inf") and float(loss[bad]) == float("inf")
+    check("lse", lse[others], forms["lse"])
+    check("loss", loss[others], forms["loss"])
+    u = torch.finfo(x.dtype).eps / 2
+    # the token adds G = g (0 - [v = label]) times its x to dw, and NaN at the infinite row; what its infinite x makes of column 0 is no number
+    value, bound = (t.clone() for t in forms["dw"])
+    first = 0 if how == "overflow" else 1
+    add = -0.25 * x[bad].cpu().double()
+    value[3] += add
+    bound[3] += add.abs() * (2.2 * u + 8 * F32)
+    value[top] = float("nan")
+    for dx, dw in both_ways(op, x, weights, labels, upstream):
+        check("dx", dx[others], forms["dx"])
+        assert bool(torch.isnan(dx[bad]).all())
+        check("dw", dw[:, first:], (value[:, first:], bound[:, first:]))
+        assert not bool(torch.isfinite(dw[:, :first]).any())
+    labels[bad] = top      # inf - inf
+    loss, lse = op.forward(x, weights, labels)
+    assert float(lse[bad]) == float("inf") and bool(torch.isnan(loss[bad]))
+    if how == "infinite x":  # and a logit that is no number beside it, near and far
+        for row in (top - 1, 20):
+            w[row, 0] = 0
+            lse = op.forward(x, list(w.split(rows)), labels)[1]
+            assert bool(torch.isnan(lse[bad])) and int(torch.isnan(lse).sum()) == 1
+            w[row, 0] = -1
