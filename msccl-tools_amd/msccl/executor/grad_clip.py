@@ -11,7 +11,7 @@ import torch
 
 from . import binding
 from .binding import DTYPE_CODES
-from .runner import dtype_name
+from .runner import dtype_name, new_workspace, refuse_capture
 
 NORM_CODES = {"l2": 0, "max": 1}
 
@@ -40,7 +40,9 @@ class GradientClip:
 
     def setup(self, sizes, dtype, out_dtype=None, norm="l2", counted=None):
         """sizes: elements of each tensor.  dtype, out_dtype (default: dtype): one type, or one per tensor.
-        counted: one truth value per tensor (default: all); the others are scaled but are not part of the norm."""
+        counted: one truth value per tensor (default: all); the others are scaled but are not part of the norm.
+        Waits for the current stream; refused while that is captured."""
+        refuse_capture(self.device)
         n = len(sizes)
         codes = []
         for what, given in (("dtype", dtype), ("out_dtype", dtype if out_dtype is None else out_dtype)):
@@ -67,7 +69,7 @@ class GradientClip:
         self._keepalive = None
         if not torch.cuda.is_available():
             raise RuntimeError("gradient clipping needs a GPU; there is no CPU path")
-        self._workspace = torch.zeros(self.workspace_bytes, dtype=torch.uint8, device=self.device)
+        self._workspace = new_workspace(self.workspace_bytes, self.device, clear=True)   # (.norm is 0 until the first launch)
         self.device = self._workspace.device   # with its index
         self._home = torch.cuda.current_stream(self.device).cuda_stream
         results = self._workspace[:8].view(torch.float32)

@@ -32,6 +32,22 @@ def dtype_name(dtype):
     raise ValueError(f"unsupported dtype {dtype!r}")
 
 
+def refuse_capture(device):
+    if torch.cuda.is_available():
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("setup() is called before a stream is captured, not meanwhile")
+
+
+def new_workspace(nbytes, device, clear=False):
+    """Memory that any stream may use as soon as this returns: nothing that its last owner enqueued on the current stream,
+    and no clearing, is still to come."""
+    with torch.cuda.device(device):
+        workspace = (torch.zeros if clear else torch.empty)(nbytes, dtype=torch.uint8, device=device)
+        torch.cuda.current_stream().synchronize()
+    return workspace
+
+
 class Executor:
     """plan = Executor(xml_or_tables); plan.setup(chunk_bytes, dtype); plan.run(inputs, outputs)."""
 

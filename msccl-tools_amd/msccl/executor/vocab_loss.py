@@ -11,7 +11,7 @@ import torch
 
 from . import binding
 from .binding import DTYPE_CODES, VocabLossDesc, VocabLossIO
-from .runner import dtype_name
+from .runner import dtype_name, new_workspace, refuse_capture
 
 REDUCTION_CODES = {"none": 0, "sum": 1, "mean": 2}
 
@@ -44,7 +44,8 @@ class VocabLoss:
         """Fix the most tokens of a call, the width and the ranks' rows, and allocate the workspace.
 
         piece_bytes: room for the probabilities of the tokens that are worked on at a time (0: 2 GiB, at least 256 tokens).
-        gradients=False: forward() only."""
+        gradients=False: forward() only.  Waits for the current stream; refused while that is captured."""
+        refuse_capture(self.device)
         name = dtype_name(dtype)
         if reduction not in REDUCTION_CODES:
             raise ValueError(f"unknown reduction {reduction!r}")
@@ -62,7 +63,7 @@ class VocabLoss:
         self._shapes = [torch.Size((r, self.hidden)) for r in rows]
         if not torch.cuda.is_available():
             raise RuntimeError("the vocabulary loss needs a GPU; there is no CPU path")
-        self._workspace = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=self.device)
+        self._workspace = new_workspace(self.workspace_bytes, self.device)
         self.device = self._workspace.device   # with its index
         self._home = torch.cuda.current_stream(self.device).cuda_stream
         # What the library reads of a call, filled in anew by each: a handle serves one thread at a time

@@ -114,3 +114,47 @@ def test_a_logit_of_infinity(tokens, rows, how, dtype):
             lse = op.forward(x, list(w.split(rows)), labels)[1]
             assert bool(torch.isnan(lse[bad])) and int(torch.isnan(lse).sum()) == 1
             w[row, 0] = -1
+
+
+def test_set_up_on_a_busy_stream_and_used_on_another():
+    """A workspace is the other stream's as soon as setup() returns: nothing that the first one still does reaches it."""
+    from msccl.executor import GradientClip
+    g = torch.full((1000,), 2.0, device="cuda")
+    x, weights, labels, upstream = make(20, 64, [100, 30], torch.bfloat16)
+    op = operator(20, 64, [100, 30], "bfloat16", reduction="none")
+    want = op.run(x, weights, labels, upstream)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    clip = GradientClip()
+    torch.cuda._sleep(300_000_000)
+    clip.setup([1000], "float32")
+    with torch.cuda.stream(side):
+        clip.bind([g], [g])
+        clip.launch()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        clip.launch()
+    torch.cuda.synchronize()
+    assert float(clip.norm) == pytest.approx(2 * 1000 ** 0.5, rel=1e-6)
+    torch.cuda._sleep(300_000_000)
+    op.setup(20, 64, [100, 30], "bfloat16", reduction="none")
+    assert torch.cuda.current_stream().query()
+    with torch.cuda.stream(side):
+        got = op.run(x, weights, labels, upstream)
+    torch.cuda.synchronize()
+    assert torch.equal(got[2], want[2])
+
+
+def test_no_set_up_while_a_stream_is_captured():
+    from msccl.executor import GradientClip, VocabLoss
+    x = torch.zeros(8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1.0)
+        with pytest.raises(RuntimeError, match="captured"):
+            VocabLoss().setup(8, 64, [40], "bfloat16")
+        with pytest.raises(RuntimeError, match="captured"):
+            GradientClip().setup([8], "float32")
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((x == 1.0).all())
