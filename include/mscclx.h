@@ -317,7 +317,7 @@ int mscclx_grad_clip_destroy(mscclx_grad_clip* clip);
 int mscclx_grad_clip_bind(mscclx_grad_clip* clip, const void* const* in, void* const* out, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Enqueues one kernel (the norm only: max_norm < 0) or two on `stream`; can be captured in a HIP graph.  The results are the two floats at
  * the start of the workspace: norm, coefficient.  Launches of one binding must follow each other on one stream. */
-int mscclx_grad_clip_launch(const mscclx_grad_clip* clip, float scale, float max_norm, void* stream);
+int mscclx_grad_clip_launch(const mscclx_grad_clip* clip, double scale, double max_norm, void* stream);
 
 #ifdef __cplusplus
 }

@@ -91,11 +91,11 @@ template <> struct Norm<true> {
 
 // The result from the partial results' sum; `threadIdx.x == 0` writes it.  Returns the factor.
 template <bool MAX>
-__device__ __forceinline__ float finish(typename Norm<MAX>::value sum, float scale, float max_norm, Header* header, bool writes) {
-  const double norm = Norm<MAX>::result(sum) * fabs((double)scale);
+__device__ __forceinline__ float finish(typename Norm<MAX>::value sum, double scale, double max_norm, Header* header, bool writes) {
+  const double norm = Norm<MAX>::result(sum) * fabs(scale);
   double c = 1.0;
-  if (max_norm >= 0.f) {
-    c = (double)max_norm / (norm + 1e-6);
+  if (max_norm >= 0.0) {
+    c = max_norm / (norm + 1e-6);
     if (c >= 1.0) c = 1.0;  // (a NaN stays)
   }
   if (writes && threadIdx.x == 0) {
@@ -106,7 +106,7 @@ __device__ __forceinline__ float finish(typename Norm<MAX>::value sum, float sca
 }
 
 template <bool MAX>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const Chunk* chunks, int nchunks, typename Norm<MAX>::value* partial, int alone, float scale, Header* header) {
+__global__ void __launch_bounds__(kThreads) norm_kernel(const Chunk* chunks, int nchunks, typename Norm<MAX>::value* partial, int alone, double scale, Header* header) {
   typedef Norm<MAX> N;
   typedef typename N::value V;
   __shared__ V shared[kThreads / 64];
@@ -159,11 +159,11 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const Chunk* chunks, int
   if (!last) return;
   sum = 0;
   for (int i = threadIdx.x; i < (int)gridDim.x; i += kThreads) sum = N::join(sum, __hip_atomic_load(&partial[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-  finish<MAX>(over_workgroup(sum, join, shared), scale, -1.f, header, true);
+  finish<MAX>(over_workgroup(sum, join, shared), scale, -1.0, header, true);
 }
 
 template <bool MAX>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const Chunk* chunks, int nchunks, const typename Norm<MAX>::value* partial, float scale, float max_norm,
+__global__ void __launch_bounds__(kThreads) scale_kernel(const Chunk* chunks, int nchunks, const typename Norm<MAX>::value* partial, double scale, double max_norm,
                                                          Header* header) {
   typedef Norm<MAX> N;
   typedef typename N::value V;
@@ -335,12 +335,12 @@ int mscclx_grad_clip_bind(mscclx_grad_clip* h, const void* const* in, void* cons
   });
 }
 
-int mscclx_grad_clip_launch(const mscclx_grad_clip* h, float scale, float max_norm, void* stream) {
+int mscclx_grad_clip_launch(const mscclx_grad_clip* h, double scale, double max_norm, void* stream) {
   return guarded([&] {
     if (!h || !h->workspace) return fail(MSCCLX_ERR_STATE, "bind tensors before launching");
     if (!std::isfinite(scale)) return fail(MSCCLX_ERR_INVALID_ARG, "scale must be finite");
     if (std::isnan(max_norm)) return fail(MSCCLX_ERR_INVALID_ARG, "max_norm must be a number");
-    const bool clip = max_norm >= 0.f;
+    const bool clip = max_norm >= 0.0;
     if (clip && !h->outputs) return fail(MSCCLX_ERR_STATE, "the tensors were bound without outputs");
     char* ws = h->workspace;
     const int nchunks = (int)h->chunks, grid = std::max(1, std::min(nchunks, kMaxGrid));

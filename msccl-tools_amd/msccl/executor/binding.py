@@ -137,7 +137,7 @@ def load_library(path=None):
     lib.mscclx_grad_clip_create.argtypes = [i32, ptr(u64), ptr(i32), ptr(i32), ptr(ctypes.c_uint8), i32, ptr(vp), ptr(u64)]
     lib.mscclx_grad_clip_destroy.argtypes = [vp]
     lib.mscclx_grad_clip_bind.argtypes = [vp, ptr(vp), ptr(vp), vp, u64, vp]
-    lib.mscclx_grad_clip_launch.argtypes = [vp, ctypes.c_float, ctypes.c_float, vp]
+    lib.mscclx_grad_clip_launch.argtypes = [vp, ctypes.c_double, ctypes.c_double, vp]
     for name in ("mscclx_plan_create", "mscclx_plan_destroy", "mscclx_plan_simulate", "mscclx_plan_min_fifo_depth",
                  "mscclx_plan_configure", "mscclx_plan_bind", "mscclx_plan_launch", "mscclx_plan_wait", "mscclx_plan_poll",
                  "mscclx_plan_abort", "mscclx_plan_time") + tuple(s for s in EXPORTED_SYMBOLS if "vocab_loss" in s or "grad_clip" in s):

@@ -158,3 +158,19 @@ def test_no_set_up_while_a_stream_is_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert bool((x == 1.0).all())
+
+
+def test_scale_and_max_norm_in_64_bits():
+    """With one gradient of 2 the norm is exact, so that coefficient and norm are the 64-bit formula's, rounded once."""
+    from msccl.executor import GradientClip
+    clip = GradientClip()
+    clip.setup([3], "float32")
+    g, out = torch.tensor([2.0, 0.0, 0.0], device="cuda"), torch.empty(3, device="cuda")
+    clip.bind([g], [out])
+    for max_norm, scale in ((0.01, 1.0), (0.01, 0.1), (1 + 0.99 * 2.0 ** -24, 1.0), (1e-3, 1 / 3), (0.3, 0.7), (0.07, 1e-3), (1.0, 1 - 0.99 * 2.0 ** -25), (1e-50, 1.0), (1e39, 1.0)):
+        clip.launch(max_norm=max_norm, scale=scale)
+        torch.cuda.synchronize()
+        norm = 2.0 * scale
+        coefficient = min(1.0, max_norm / (norm + 1e-6))
+        assert clip.norm.item() == np.float32(norm) and clip.coefficient.item() == np.float32(coefficient), (max_norm, scale)
+        assert abs(out[0].item() - 2.0 * scale * coefficient) <= 2.0 * scale * coefficient * 2 * 1.01 * 2.0 ** -24 + 2.0 ** -149
