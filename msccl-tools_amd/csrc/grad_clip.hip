@@ -89,9 +89,10 @@ template <> struct Norm<true> {
   static __device__ __forceinline__ double result(unsigned a) { return (double)__uint_as_float(a); }
 };
 
-// The result from the partial results' sum; `threadIdx.x == 0` writes it.  Returns the factor.
+// The result from the partial results' sum; `threadIdx.x == 0` writes it.  Returns the factor, in 64 bits: against gradients
+// of 1e36 it is below what 32 bits hold, and the output is nevertheless an ordinary number.
 template <bool MAX>
-__device__ __forceinline__ float finish(typename Norm<MAX>::value sum, double scale, double max_norm, Header* header, bool writes) {
+__device__ __forceinline__ double finish(typename Norm<MAX>::value sum, double scale, double max_norm, Header* header, bool writes) {
   const double norm = Norm<MAX>::result(sum) * fabs(scale);
   double c = 1.0;
   if (max_norm >= 0.0) {
@@ -102,7 +103,7 @@ __device__ __forceinline__ float finish(typename Norm<MAX>::value sum, double sc
     header->norm = (float)norm;
     header->coefficient = (float)c;
   }
-  return (float)(c * scale);
+  return c * scale;
 }
 
 template <bool MAX>
@@ -170,10 +171,10 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const Chunk* chunks, in
   __shared__ V shared[kThreads / 64];
   V sum = 0;
   for (int i = threadIdx.x; i < (int)gridDim.x; i += kThreads) sum = N::join(sum, partial[i]);
-  const float factor = finish<MAX>(over_workgroup(sum, [](V a, V b) { return N::join(a, b); }, shared), scale, max_norm, header, blockIdx.x == 0);
+  const double factor = finish<MAX>(over_workgroup(sum, [](V a, V b) { return N::join(a, b); }, shared), scale, max_norm, header, blockIdx.x == 0);
   for (int b = blockIdx.x; b < nchunks; b += gridDim.x) {
     const Chunk t = chunks[b];
-    if (factor == 1.f && t.in == t.out) continue;  // nothing changes (in place, types are the same)
+    if (factor == 1.0 && t.in == t.out) continue;  // nothing changes (in place, types are the same)
     by_type(t.in_type, [&](auto* in_type) {
       by_type(t.out_type, [&](auto* out_type) {
         typedef std::remove_pointer_t<decltype(in_type)> T;
@@ -189,10 +190,10 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const Chunk* chunks, in
           U o[W];
           load(p + i, v);
 #pragma unroll
-          for (int k = 0; k < W; ++k) o[k] = (U)(widen(v[k]) * factor);
+          for (int k = 0; k < W; ++k) o[k] = (U)(float)(widen(v[k]) * factor);
           store(q + i, o);
         }
-        for (; i < n && i + W > n; ++i) q[i] = (U)(widen(p[i]) * factor);
+        for (; i < n && i + W > n; ++i) q[i] = (U)(float)(widen(p[i]) * factor);
       });
     });
   }

@@ -174,3 +174,19 @@ def test_scale_and_max_norm_in_64_bits():
         coefficient = min(1.0, max_norm / (norm + 1e-6))
         assert clip.norm.item() == np.float32(norm) and clip.coefficient.item() == np.float32(coefficient), (max_norm, scale)
         assert abs(out[0].item() - 2.0 * scale * coefficient) <= 2.0 * scale * coefficient * 2 * 1.01 * 2.0 ** -24 + 2.0 ** -149
+
+
+@pytest.mark.parametrize("dtype, size, max_norm", [("float32", 1e36, 1e-6), ("float32", 1e30, 1e-10), ("bfloat16", 1e36, 1e-6), ("float32", 1e-2, 0.01), ("float16", 1e-2, 1e-3)])
+def test_a_factor_of_any_size(dtype, size, max_norm):
+    """Outputs are one rounding from the formula, also where the coefficient is below what 32 bits hold."""
+    from msccl.executor import GradientClip
+    gen = torch.Generator().manual_seed(7)
+    g = (torch.randn(5000, generator=gen) * size).to(DTYPES.get(dtype, torch.float32)).cuda()
+    out = torch.empty(5000, device="cuda")
+    clip = GradientClip()
+    clip.setup([5000], dtype, out_dtype="float32")
+    for scale in (1.0, 0.3):
+        clip.run([g], [out], max_norm=max_norm, scale=scale)
+        wide = g.cpu().double()
+        want = wide * (scale * (max_norm / (wide.square().sum().sqrt() * scale + 1e-6)))
+        check("output", out, (want, want.abs() * 1.01 * 2.0 ** -24 + 2.0 ** -149))
