@@ -12,7 +12,7 @@ LIB = os.path.join(HERE, "libmscclx.so")
 KERNEL_GROUPS = 5
 OPERATORS = ["vocab_loss", "grad_clip"]
 SOURCES = ["plan.cpp", "exec.hip", "exec_kernels.hip"] + [o + ".hip" for o in OPERATORS]
-HEADERS = ["plan.h", "exec_device.h", "tile_product.h", os.path.join(ROOT, "include", "mscclx.h")]
+HEADERS = ["plan.h", "exec_device.h", "tile_product.h", "step_walk.h", os.path.join(ROOT, "include", "mscclx.h")]
 
 
 def hipcc():

@@ -21,6 +21,8 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "step_walk.h"
+
 namespace mscclx {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -107,21 +109,13 @@ struct Lanes {
 // Where an operand's copies read: `base(i)`, the resource of the rows of unit i (row) or of all (col), for step after
 // step `next()`; then `further` is what they add to it, and `left` the values of k from the step's first on.  Behind
 // the last step nothing is left.
-template <int TILE> struct RowSource {  // k contiguous
+template <int TILE> struct RowSource : StepWalk<kStepK, 2 * kStepK> {  // k contiguous
   static constexpr int kUnits = (TILE + kUnitRows - 1) / kUnitRows;
   i32x4 bases[kUnits];
-  int further, left, turn, steps;
   // at(i): the address of unit i's first row.  first: the step to begin with; those in front of it come last
-  template <class F> __device__ __forceinline__ RowSource(F at, int k, int first = 0) : steps((k + kStepK - 1) / kStepK) {
+  template <class F> __device__ __forceinline__ RowSource(F at, int k, int first = 0) : StepWalk(k, first) {
 #pragma unroll
     for (int i = 0; i < kUnits; ++i) bases[i] = resource_at(at(i));
-    further = (first - 1) * 2 * kStepK;
-    left = k - (first - 1) * kStepK;
-    turn = first ? steps - first : -1;  // steps up to the first one again
-  }
-  __device__ __forceinline__ void next() {
-    further += 2 * kStepK, left -= kStepK;
-    if (turn-- == 0) further -= steps * 2 * kStepK, left += steps * kStepK;
   }
   __device__ __forceinline__ i32x4 base(int i) const { return bases[i]; }
 };

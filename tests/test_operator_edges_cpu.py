@@ -1,0 +1,41 @@
+"""The operators at the edges of what their documentation allows, without a GPU."""
+import os
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "msccl-tools_amd", "csrc")
+
+WALK = r"""
+#include <cstdio>
+#include <vector>
+#include "step_walk.h"
+int main() {
+  for (int k = 1; k <= 700; k += k < 140 ? 1 : 8)
+    for (int first = 0, steps = (k + 63) / 64; first < steps; ++first) {
+      mscclx::StepWalk<64, 128> walk(k, first);
+      std::vector<int> seen(steps);
+      for (int s = 0; s < steps; ++s) {
+        walk.next();
+        const int step = (first + s) % steps, there = k - step * 64 < 64 ? k - step * 64 : 64;
+        // at the step's bytes, and all of its values are there, none of the next row's
+        if (walk.further != step * 128 || (walk.left < 64 ? walk.left : 64) != there || walk.left > k - step * 64) return printf("k %d first %d: turn %d\n", k, first, s), 1;
+        ++seen[step];
+      }
+      for (int n : seen) if (n != 1) return printf("k %d first %d: a step came %d times\n", k, first, n), 1;
+      for (int s = 0; s < 8; ++s) {
+        walk.next();
+        if (walk.left > 0) return printf("k %d first %d: %d values left behind the last step\n", k, first, walk.left), 1;
+      }
+    }
+}
+"""
+
+
+def test_the_steps_of_a_row_come_once_each(tmp_path):
+    source, exe = tmp_path / "walk.cpp", str(tmp_path / "walk")
+    source.write_text(WALK)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I", CSRC, str(source), "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
