@@ -1161,7 +1161,7 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
     int units = 0;
     for (int r = 0; r < d.ranks; ++r) {
       const int64_t rows = d.rank_rows[r];
-      if (rows < 0 || (int64_t)units * kUnitRows + rows > MSCCLX_VOCAB_LOSS_MAX_STRIDE - kTile) {  // (rows of G are addressed with 32-bit offsets, 64 at a time)
+      if (rows < 0 || rows > MSCCLX_VOCAB_LOSS_MAX_STRIDE || (int64_t)units * kUnitRows + rows > MSCCLX_VOCAB_LOSS_MAX_STRIDE - kTile) {  // (rows of G are addressed with 32-bit offsets, 64 at a time)
         delete h;
         return fail(MSCCLX_ERR_INVALID_ARG, "the ranks' rows must not be negative and, each rank's rounded up to 64, add up to less than 2^22");
       }

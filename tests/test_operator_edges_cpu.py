@@ -4,6 +4,8 @@ import subprocess
 
 import pytest
 
+from test_operators_cpu import INVALID, create_loss
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "msccl-tools_amd", "csrc")
 
@@ -39,3 +41,9 @@ def test_the_steps_of_a_row_come_once_each(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I", CSRC, str(source), "-o", exe], check=True)
     r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("rows", [(64, (1 << 63) - 1), ((1 << 63) - 1, 64), (1, 1 << 62), (64, (1 << 63) - 64)])
+def test_rows_whose_sum_passes_64_bits_are_refused(mscclx_lib, rows):
+    rc, handle, _, _ = create_loss(mscclx_lib, rows=rows)
+    assert rc == INVALID and not handle.value
