@@ -96,6 +96,14 @@ class VocabLossIO(ctypes.Structure):  # weights, dweights: addresses of arrays o
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 
+def whole(what, value, bits, signed=True):
+    """`value` as an integer that a C argument of so many bits holds (ctypes cuts off what is more)."""
+    value, least = int(value), -(1 << (bits - 1)) if signed else 0
+    if not least <= value < least + (1 << bits):
+        raise ValueError(f"{what}: {value} is not in the range of a {bits}-bit {'' if signed else 'unsigned '}integer")
+    return value
+
+
 _lib = None
 
 

@@ -10,7 +10,7 @@ import ctypes
 import torch
 
 from . import binding
-from .binding import DTYPE_CODES
+from .binding import DTYPE_CODES, whole
 from .runner import dtype_name, new_workspace, refuse_capture
 
 NORM_CODES = {"l2": 0, "max": 1}
@@ -57,6 +57,7 @@ class GradientClip:
         sizes = [int(s) for s in sizes]
         if any(s < 0 for s in sizes):
             raise ValueError("sizes must not be negative")
+        sizes = [whole("sizes", s, 64, signed=False) for s in sizes]
         array = lambda kind, values: (kind * max(1, n))(*values)  # noqa: E731
         handle, nbytes = ctypes.c_void_p(), ctypes.c_uint64()
         binding._check(self.lib, self.lib.mscclx_grad_clip_create(

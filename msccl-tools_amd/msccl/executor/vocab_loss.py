@@ -10,7 +10,7 @@ import ctypes
 import torch
 
 from . import binding
-from .binding import DTYPE_CODES, VocabLossDesc, VocabLossIO
+from .binding import DTYPE_CODES, VocabLossDesc, VocabLossIO, whole
 from .runner import dtype_name, new_workspace, refuse_capture
 
 REDUCTION_CODES = {"none": 0, "sum": 1, "mean": 2}
@@ -49,9 +49,9 @@ class VocabLoss:
         name = dtype_name(dtype)
         if reduction not in REDUCTION_CODES:
             raise ValueError(f"unknown reduction {reduction!r}")
-        rows = [int(r) for r in rank_rows]
-        desc = VocabLossDesc(len(rows), int(hidden), (ctypes.c_int64 * max(1, len(rows)))(*rows), int(tokens), DTYPE_CODES[name],
-                             REDUCTION_CODES[reduction], int(ignore_index), int(piece_bytes), int(bool(gradients)), 0)
+        rows = [whole("rank_rows", r, 64) for r in rank_rows]
+        desc = VocabLossDesc(len(rows), whole("hidden", hidden, 32), (ctypes.c_int64 * max(1, len(rows)))(*rows), whole("tokens", tokens, 64), DTYPE_CODES[name],
+                             REDUCTION_CODES[reduction], whole("ignore_index", ignore_index, 64), whole("piece_bytes", piece_bytes, 64, signed=False), int(bool(gradients)), 0)
         handle, nbytes, piece = ctypes.c_void_p(), ctypes.c_uint64(), ctypes.c_int64()
         binding._check(self.lib, self.lib.mscclx_vocab_loss_create(ctypes.byref(desc), ctypes.byref(handle), ctypes.byref(nbytes), ctypes.byref(piece)))
         self.close()

@@ -47,3 +47,14 @@ def test_the_steps_of_a_row_come_once_each(tmp_path):
 def test_rows_whose_sum_passes_64_bits_are_refused(mscclx_lib, rows):
     rc, handle, _, _ = create_loss(mscclx_lib, rows=rows)
     assert rc == INVALID and not handle.value
+
+
+@pytest.mark.parametrize("changed", [dict(tokens=(1 << 64) + 5), dict(hidden=(1 << 32) + 64), dict(rank_rows=[(1 << 64) + 100]), dict(piece_bytes=-1), dict(piece_bytes=(1 << 64) + 1),
+                                     dict(ignore_index=1 << 63), dict(ignore_index=-(1 << 63) - 1)])
+def test_numbers_that_no_argument_of_the_library_holds_are_refused(mscclx_lib, changed):
+    """ctypes would cut them off: 2^64 + 5 tokens would be 5."""
+    from msccl.executor import GradientClip, VocabLoss
+    with pytest.raises(ValueError, match="range"):
+        VocabLoss().setup(**{**dict(tokens=8, hidden=64, rank_rows=[100], dtype="bfloat16"), **changed})
+    with pytest.raises(ValueError, match="range"):
+        GradientClip().setup([3, (1 << 64) + 3], "float32")
