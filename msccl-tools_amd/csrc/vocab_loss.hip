@@ -925,6 +925,9 @@ bool align_pays(const Pieces& p, int64_t tokens, int hidden) {
 // Middle; 1024 x 4096 x 512: 29 / 20 Middle).
 int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 384 ? kThin : (int64_t)p.tiles * tiles(hidden) < kComputeUnits ? kMiddle : kLarge; }
 
+// Logits in 32 bits and G twice where that decides about a rank's dw: with few tokens, or few for each rank.
+bool is_wide(int64_t tokens, int ranks) { return tokens <= 32 || (tokens <= kWideTokens && tokens < 16 * ranks); }
+int64_t most_wide(int64_t tokens, int ranks) { return std::min<int64_t>(tokens, std::max(32, std::min(kWideTokens, 16 * ranks - 1))); }
 // Where G's second rows begin, so that no step of dw's product and no tile of dx's has more of them than need be; rows
 // behind the first ones are zeros.
 int second_row(int64_t tokens) { return tokens <= 16 ? 16 : tokens <= 32 ? 32 : (int)((tokens + kStepK - 1) / kStepK * kStepK); }
@@ -997,8 +1000,7 @@ int enqueue(const mscclx_vocab_loss* h, const mscclx_vocab_loss_io* io, bool for
   const int mean = d.reduction == MSCCLX_LOSS_MEAN, per_token = d.reduction == MSCCLX_LOSS_NONE;
   const Upstream upstream = {io->grad_loss, per_token ? c.factor : nullptr};
   int rc;
-  // Twice where that decides about a rank's dw: with few tokens, or few for each rank
-  const bool wide = backward && (n <= 32 || (n <= kWideTokens && n < 16 * d.ranks));
+  const bool wide = backward && is_wide(n, d.ranks);
   // The sums over tokens: for the gradients in front of everything, unless that is one number and nothing in front of
   // the products asks for it; for the loss as one number behind the last piece's tokens (beside its gradients, where dx
   // has parts). Up to kWideTokens tokens, rows of zeros cost less than the launch that finds out which they are
@@ -1200,15 +1202,16 @@ int mscclx_vocab_loss_create(const mscclx_vocab_loss_desc* desc, mscclx_vocab_lo
     h->off_aligned = align_pays(p, h->piece, d.hidden) ? take((uint64_t)h->piece * kept_stride(d.hidden)) : 0;
     const uint64_t wide = (uint64_t)p.tiles * kTile;
     h->off_stats = take(std::max(std::min<uint64_t>(h->piece, most_of_few(p)) * (wide / (Few::kL / Few::kWavesL)), (uint64_t)h->piece * (wide / (Middle::kL / Middle::kWavesL))) * sizeof(float2));
-    h->off_logits = d.gradients ? take(std::min<uint64_t>(n, kWideTokens) * p.stride() * 4) : 0;
-    h->off_e = d.gradients ? take(std::max<uint64_t>(h->piece, std::min<uint64_t>(n, kWideTokens) + kWideTokens) * row) : 0;
+    const uint64_t wide_rows = most_wide(d.max_tokens, d.ranks);
+    h->off_logits = d.gradients ? take(wide_rows * p.stride() * 4) : 0;
+    h->off_e = d.gradients ? take(std::max<uint64_t>(h->piece, second_row(wide_rows) + wide_rows) * row) : 0;
     h->off_sums = d.gradients && d.max_tokens > h->piece ? take((uint64_t)p.tiles * kTile * d.hidden * 4) : 0;
     uint64_t parts = 0;  // dx's parts at the token count that needs most of them
     auto need = [&](int64_t rows, bool separate) {
       const DxPlan plan = dx_plan(p, rows, d.hidden, separate);
       if (plan.separate) parts = std::max(parts, (uint64_t)plan.parts * rows * d.hidden * 4);
     };
-    for (int64_t t = 1; d.gradients && t <= std::min<int64_t>(h->piece, kWideTokens); ++t) need(t, true), need(second_row(t) + t, true);
+    for (int64_t t = 1; d.gradients && t <= std::min<int64_t>(h->piece, kWideTokens); ++t) need(is_wide(t, d.ranks) ? second_row(t) + t : t, true);
     for (int64_t t = 32; d.gradients && t - 31 <= h->piece; t += 32) need(std::min(t, h->piece), false);  // (the plan is the same from t - 31 on)
     h->off_parts = take(parts);
     h->bytes = at;

@@ -58,3 +58,15 @@ def test_numbers_that_no_argument_of_the_library_holds_are_refused(mscclx_lib, c
         VocabLoss().setup(**{**dict(tokens=8, hidden=64, rank_rows=[100], dtype="bfloat16"), **changed})
     with pytest.raises(ValueError, match="range"):
         GradientClip().setup([3, (1 << 64) + 3], "float32")
+
+
+def test_workspace_has_no_32_bit_logits_that_no_call_keeps(mscclx_lib):
+    """One rank keeps those of at most 32 tokens, eight ranks of 127; what else a token costs is its 16-bit probabilities and their statistics."""
+    def size(ranks, tokens, rows=131072):
+        rc, handle, nbytes, _ = create_loss(mscclx_lib, rows=(rows // ranks,) * ranks, hidden=8, tokens=tokens)
+        assert rc == 0
+        mscclx_lib.mscclx_vocab_loss_destroy(handle)
+        return nbytes
+    per_token = 131072 * 2 + 131072 // 32 * 8
+    assert size(1, 128) - size(1, 32) <= 96 * per_token * 1.05
+    assert size(8, 127) - size(1, 127) >= 95 * 131072 * 4    # their logits, at least
