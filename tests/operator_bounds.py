@@ -54,6 +54,32 @@ def loss_forms(x, weights, labels, reduction, ignore_index, upstream):
             "dx": (dx, off(dx, dx_size, G_off @ w.abs(), v)), "dw": (dw, off(dw, dw_size, G_off.t() @ x.abs(), n))}
 
 
+def wide_forms(x, weights, labels, ignore_index, upstream):
+    """dx and dw as loss_forms, but with G held in two 16-bit numbers: what the second leaves is half a step of half a step."""
+    forms = loss_forms(x, weights, labels, "none", ignore_index, upstream)
+    dtype = x.dtype
+    u = torch.finfo(dtype).eps / 2
+    x, w, labels = x.cpu().double(), torch.cat([t.cpu() for t in weights]).double(), labels.cpu().long()
+    lse, lse_off = forms["lse"]
+    n = x.shape[0]
+    z = x @ w.t()
+    y = torch.zeros_like(z)
+    kept = labels != ignore_index
+    y[torch.arange(n), labels.where(kept, torch.zeros_like(labels))] = 1.0
+    g = upstream.cpu().double() * kept
+    p = torch.exp(z - lse[:, None])
+    G = g[:, None] * (p - y)
+    z_off = (x.shape[1] + 4) * F32 * (x.abs() @ w.abs().t()).amax(1)
+    relative = 2 * (z_off + lse_off)[:, None] + F32 * (8 + (z - lse[:, None]).abs())
+    least = 2.0 ** -25 / 2.0 ** 15 if dtype == torch.float16 else 2.0 ** -126
+    G_off = g.abs()[:, None] * (p * 1.5 * relative + (p - y).abs() * (1.1 * u * u + 16 * 2.0 ** -24)) + 2.2 * least * g.abs().max() * kept[:, None]
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    off = lambda value, size, rounded, terms: rounded * 1.01 + (terms + 8) * F32 * size + u * 1.01 * value.abs() + tiny  # noqa: E731
+    dx, dw = G @ w, G.t() @ x
+    return {"G": G, "dx": (dx, off(dx, G.abs() @ w.abs(), G_off @ w.abs(), 2 * w.shape[0])),
+            "dw": (dw, off(dw, G.abs().t() @ x.abs(), G_off.t() @ x.abs(), 2 * n))}
+
+
 def check(what, got, form):
     """`got` within the bound of form = (value, bound), elementwise; NaN only where the value is NaN."""
     value, bound = form

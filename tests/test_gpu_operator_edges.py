@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from operator_bounds import F32, check, loss_forms
+from operator_bounds import check, loss_forms, wide_forms
 from test_gpu_vocab_loss import DTYPES, IGNORE, check_all, make, operator
 
 pytestmark = pytest.mark.gpu
@@ -190,3 +190,18 @@ def test_a_factor_of_any_size(dtype, size, max_norm):
         wide = g.cpu().double()
         want = wide * (scale * (max_norm / (wide.square().sum().sqrt() * scale + 1e-6)))
         check("output", out, (want, want.abs() * 1.01 * 2.0 ** -24 + 2.0 ** -149))
+
+
+WIDE = [(1, 64, [500, 300]), (2, 72, [130]), (16, 72, [257, 0, 255]), (17, 64, [300]), (32, 64, [129, 90]), (33, 64, [40] * 8), (100, 136, [40] * 8)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens, hidden, rows", WIDE)
+def test_gradients_of_few_tokens_lose_nothing_to_16_bits(tokens, hidden, rows, dtype):
+    x, weights, labels, upstream = make(tokens, hidden, rows, DTYPES[dtype], seed=11)
+    labels[0] = 5
+    forms = wide_forms(x, weights, labels, IGNORE, upstream)
+    op = operator(tokens, hidden, rows, dtype, reduction="none")
+    for dx, dw in both_ways(op, x, weights, labels, upstream):
+        check("dx", dx, forms["dx"])
+        check("dw", dw, forms["dw"])

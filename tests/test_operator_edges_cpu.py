@@ -3,7 +3,10 @@ import os
 import subprocess
 
 import pytest
+import torch
 
+from operator_bounds import check, wide_forms
+from test_gpu_operator_edges import WIDE
 from test_operators_cpu import INVALID, create_loss
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -70,3 +73,26 @@ def test_workspace_has_no_32_bit_logits_that_no_call_keeps(mscclx_lib):
     per_token = 131072 * 2 + 131072 // 32 * 8
     assert size(1, 128) - size(1, 32) <= 96 * per_token * 1.05
     assert size(8, 127) - size(1, 127) >= 95 * 131072 * 4    # their logits, at least
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens, hidden, rows", WIDE)
+def test_the_bound_for_few_tokens_tells_two_numbers_from_one(tokens, hidden, rows, dtype):
+    """The bound that the kernel's gradients of few tokens are held to: G in two 16-bit numbers meets it, G rounded once does not."""
+    gen = torch.Generator().manual_seed(11)
+    weights = [(torch.randn(r, hidden, generator=gen) * 1.5 / hidden ** 0.5).to(dtype) for r in rows]
+    x = torch.randn(tokens, hidden, generator=gen).to(dtype)
+    labels = torch.randint(sum(rows), (tokens,), generator=gen)
+    upstream = torch.rand(tokens, generator=gen) + 0.5
+    forms = wide_forms(x, weights, labels, -100, upstream)
+    unit = (2.0 ** 15 if dtype == torch.float16 else 1.0) / upstream.max().double()
+    G = forms["G"] * unit
+    once = G.to(dtype).double()
+    both = once + (G - once).to(dtype).double()
+    w = torch.cat(weights).double()
+    gradients = lambda G: {"dx": (G @ w / unit).to(dtype), "dw": (G.t() @ x.double() / unit).to(dtype)}  # noqa: E731
+    for what, got in gradients(both).items():
+        check(what, got, forms[what])
+    with pytest.raises(AssertionError, match="beyond their bound"):
+        for what, got in gradients(once).items():
+            check(what, got, forms[what])
