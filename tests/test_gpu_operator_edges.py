@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from operator_bounds import check, loss_forms, wide_forms
+from operator_bounds import F32, check, loss_forms, wide_forms
 from test_gpu_vocab_loss import DTYPES, IGNORE, check_all, make, operator
 
 pytestmark = pytest.mark.gpu
@@ -205,3 +205,118 @@ def test_gradients_of_few_tokens_lose_nothing_to_16_bits(tokens, hidden, rows, d
     for dx, dw in both_ways(op, x, weights, labels, upstream):
         check("dx", dx, forms["dx"])
         check("dw", dw, forms["dw"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens, rows", [(30, [100, 30]), (150, [300, 77])])
+def test_upstreams_of_very_different_sizes(tokens, rows, dtype):
+    """fp16 holds G to 2^-41 of the largest upstream (the bound's `least`), bf16 relative to itself."""
+    x, weights, labels, upstream = make(tokens, 72, rows, DTYPES[dtype])
+    upstream = torch.where(upstream < 0, -1.0, 1.0) * 2.0 ** -(torch.arange(tokens, device="cuda") % 25).float()
+    check_all(operator(tokens, 72, rows, dtype, reduction="none"), x, weights, labels, upstream * 1024, "none")
+
+
+def reference_rows(x, weights, labels, upstream, rows):
+    """lse of all tokens and dw of some rows of the vocabulary, on the device in 64 bits, block by block; with bounds as in loss_forms."""
+    u = torch.finfo(x.dtype).eps / 2
+    x = x.double()
+    n, d = x.shape
+    top, total, dot = torch.full((n,), -1e300, dtype=torch.float64, device="cuda"), torch.zeros(n, dtype=torch.float64, device="cuda"), torch.zeros(n, dtype=torch.float64, device="cuda")
+    longest = torch.zeros((), dtype=torch.float64, device="cuda")
+    for w in weights:
+        for part in w.split(1 << 17):
+            part = part.double()
+            longest = torch.maximum(longest, part.square().sum(1).max().sqrt())
+            z = x @ part.t()
+            m = torch.maximum(top, z.amax(1))
+            e = torch.exp(z - m[:, None])
+            shrink = torch.exp(top - m)
+            total, dot, top = total * shrink + e.sum(1), dot * shrink + (e * z).sum(1), m
+    lse = top + total.log()
+    z_off = (d + 4) * F32 * x.square().sum(1).sqrt() * longest       # |x| |w| is at least the sum of |x[d] w[d]|
+    lse_off = z_off + F32 * (lse.abs() + 4 * (top - dot / total) + 64)
+    w = torch.cat(weights)[rows].double()
+    kept = labels != IGNORE
+    g = (upstream.double() * kept)[:, None]
+    z = x @ w.t()
+    p, y = torch.exp(z - lse[:, None]), (labels[:, None] == rows[None, :]).double()
+    relative = 2 * (z_off + lse_off)[:, None] + F32 * (8 + (z - lse[:, None]).abs())
+    G = g * (p - y)
+    G_off = g.abs() * (p * (1.1 * u + 1.5 * relative) + (p - y).abs() * 1.1 * u) + 2.2 * 2.0 ** -126
+    dw = G.t() @ x
+    off = (G_off.t() @ x.abs()) * 1.01 + (n + 8) * F32 * (G.abs().t() @ x.abs()) + u * 1.01 * dw.abs() + 2.0 ** -133
+    return (lse.cpu(), lse_off.cpu()), (dw.cpu(), off.cpu())
+
+
+def large_case(tokens, hidden, rows, seed):
+    """Inputs made on the device, few of the tokens ignored."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    weights = [(torch.randn(r, hidden, generator=gen, device="cuda") * 1.5 / hidden ** 0.5).bfloat16() for r in rows]
+    x = torch.randn(tokens, hidden, generator=gen, device="cuda").bfloat16()
+    labels = torch.randint(sum(rows), (tokens,), generator=gen, device="cuda")
+    labels[::50], labels[1], labels[-1] = IGNORE, 0, sum(rows) - 1
+    return x, weights, labels, torch.rand(tokens, generator=gen, device="cuda") + 0.5
+
+
+def test_probabilities_beyond_32_bit_offsets():
+    """A piece of 2300 tokens against 2^20 rows: G has more than 2^31 elements, its last rows lie behind 2^32 bytes."""
+    rows, tokens = [600_000, (1 << 20) - 600_000], 2300
+    x, weights, labels, upstream = large_case(tokens, 64, rows, 3)
+    op = operator(tokens, 64, rows, "bfloat16", reduction="none", piece_bytes=6 << 30)
+    assert op.piece_tokens == tokens and int((labels != IGNORE).sum()) << 20 > 1 << 31
+    picked = torch.tensor([0, 1, 599_999, 600_000, 1 << 19, (1 << 20) - 2, (1 << 20) - 1], device="cuda")
+    lse_form, dw_form = reference_rows(x, weights, labels, upstream, picked)
+    some = torch.tensor([0, 1, 1023, 2047, 2048, 2049, tokens - 2, tokens - 1], device="cuda")
+    forms = loss_forms(x[some], weights, labels[some], "none", IGNORE, upstream[some])
+    loss, lse = op.forward(x, weights, labels)
+    check("lse", lse, lse_form)
+    check("loss", loss[some], forms["loss"])
+    for dx, dw in both_ways(op, x, weights, labels, upstream):
+        check("dx", dx[some], forms["dx"])
+        check("dw", dw[picked], dw_form)
+
+
+def test_sums_of_pieces_beyond_32_bit_offsets():
+    """dw over two pieces of tokens, kept in 32 bits meanwhile: 2^20 rows of 1032 are more than 2^32 bytes."""
+    rows, tokens = [1 << 19, 1 << 19], 300
+    x, weights, labels, upstream = large_case(tokens, 1032, rows, 4)
+    op = operator(tokens, 1032, rows, "bfloat16", reduction="none", piece_bytes=1)
+    assert op.piece_tokens == 256
+    picked = torch.tensor([0, 1, (1 << 19) - 1, 1 << 19, 1_000_000, (1 << 20) - 64, (1 << 20) - 2, (1 << 20) - 1], device="cuda")
+    lse_form, dw_form = reference_rows(x, weights, labels, upstream, picked)
+    for dx, dw in both_ways(op, x, weights, labels, upstream):
+        check("dw", dw[picked], dw_form)
+        assert bool(torch.isfinite(dx).all())
+    check("lse", op.forward(x, weights, labels)[1], lse_form)
+
+
+def test_matrices_beyond_32_bit_offsets():
+    """Rows 2^22 elements apart: the last ones of x, dx and of the first rank's W and dw lie behind 2^32 bytes; what lies between is left alone."""
+    tokens, hidden, rows, stride = 560, 64, [560, 3], 1 << 22
+
+    def apart(t):
+        buffer = torch.empty((len(t) - 1) * stride + 2 * hidden, dtype=t.dtype, device="cuda")
+        spread = buffer.as_strided((len(t), 2 * hidden), (stride, 1))
+        spread.fill_(float("nan"))
+        spread[:, :hidden] = t
+        return spread
+
+    x, weights, labels, upstream = make(tokens, hidden, rows, torch.bfloat16)
+    forms = loss_forms(x, weights, labels, "none", IGNORE, upstream)
+    op = operator(tokens, hidden, rows, "bfloat16", reduction="none")
+    dx, dw = apart(torch.zeros_like(x)), [apart(torch.zeros_like(w)) for w in weights]
+    px, pw = apart(x), [apart(w) for w in weights]
+    for way in ("run", "backward"):
+        args = px[:, :hidden], [w[:, :hidden] for w in pw], labels
+        outs = dict(dx=dx[:, :hidden], dweights=[t[:, :hidden] for t in dw])
+        if way == "run":
+            loss, lse, _, _ = op.run(*args, upstream, **outs)
+            check("loss", loss, forms["loss"])
+            check("lse", lse, forms["lse"])
+        else:
+            op.backward(*args, lse, upstream, **outs)
+        check("dx", dx[:, :hidden], forms["dx"])
+        check("dw", torch.cat([t[:, :hidden] for t in dw]), forms["dw"])
+        for t in (dx, *dw):
+            assert bool(torch.isnan(t[:, hidden:]).all())
+            t[:, :hidden] = 0
