@@ -58,9 +58,10 @@ template <> struct Half<_Float16> {
 };
 
 // 16 bytes per lane from `resource` at `offset` (per lane) + `further` to LDS at m0 + 16 * lane.  Nothing else in these
-// kernels uses m0.
+// kernels uses m0.  A vector instruction may have written `resource` just before (resource_at): a load wants five wait
+// states behind it, which the compiler does not see to in here.
 __device__ __forceinline__ void copy_to_lds(unsigned lds, unsigned offset, i32x4 resource, int further) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(resource), "s"(further) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(resource), "s"(further) : "memory");
 }
 __device__ __forceinline__ i32x4 resource_at(const char* p) {
   const uint64_t a = (uint64_t)p;

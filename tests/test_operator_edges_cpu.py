@@ -1,6 +1,7 @@
 """The operators at the edges of what their documentation allows, without a GPU."""
 import os
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -96,3 +97,29 @@ def test_the_bound_for_few_tokens_tells_two_numbers_from_one(tokens, hidden, row
     with pytest.raises(AssertionError, match="beyond their bound"):
         for what, got in gradients(once).items():
             check(what, got, forms[what])
+
+
+COPY = r"""
+#include "tile_product.h"
+__global__ void copy(const char* const* from, const int* which) {
+  __shared__ __attribute__((aligned(1024))) char smem[1024];
+  const int lane = threadIdx.x;
+  typedef __attribute__((address_space(3))) char* lds_char;
+  mscclx::copy_to_lds((unsigned)(uintptr_t)(lds_char)smem, lane * 16, mscclx::resource_at(from[which[lane]]), 0);
+}
+"""
+
+
+def test_copies_to_lds_wait_for_a_resource_that_a_vector_instruction_wrote(tmp_path):
+    """Five wait states between the write of a scalar register and the load that takes its address from it, in the compiled code."""
+    sys.path.insert(0, CSRC)
+    import build
+    source, listing = tmp_path / "copy.hip", tmp_path / "copy.s"
+    source.write_text(COPY)
+    subprocess.run([build.hipcc(), "-O3", "-std=c++17", "-I", CSRC, "--offload-arch=gfx950", "--cuda-device-only", "-S", str(source), "-o", str(listing)], check=True)
+    lines = [line.split(";")[0].split() for line in listing.read_text().splitlines()]
+    lines = [line for line in lines if line and not line[0].startswith(".") and not line[0].endswith(":")]
+    load = next(i for i, line in enumerate(lines) if line[0] == "buffer_load_dwordx4")
+    write = max(i for i in range(load) if lines[i][0] == "v_readfirstlane_b32")
+    states = sum(int(line[1], 0) + 1 if line[0] == "s_nop" else 1 for line in lines[write + 1:load])
+    assert states >= 5, lines[write:load + 1]
