@@ -242,7 +242,9 @@ int mscclx_plan_time(mscclx_plan* plan, void* stream, int32_t iters, float* ms_o
  * A token whose label is `ignore_index` has loss 0 and adds nothing to either gradient, whatever its x holds; one whose label lies outside the
  * vocabulary otherwise has loss and gradients NaN (and every dw is NaN then).  MEAN divides by the number of tokens that are not
  * ignored, or by 1 if all are.  A non-finite grad_loss makes its token's dx, and every dw, non-finite; no other token's dx (one number for all: those of the
- * tokens that are not ignored).
+ * tokens that are not ignored).  With up to 32 tokens (128, if they are fewer
+ * than 16 for each rank) G is held as two 16-bit numbers; with more it is rounded to 16 bits twice, which in MSCCLX_F16 is off by up to 2^-40 of the largest |g| of the
+ * call each time.
  * What a call writes (loss, lse, dx, dweights, the workspace) may not overlap any other of its buffers (ALIASED); two
  * inputs may, and matrices whose rows are equally far apart may lie side by side in one buffer.
  * Every call only enqueues kernels on `stream`: it can be captured in a HIP graph and replayed.  Calls that share a
@@ -301,7 +303,7 @@ int mscclx_vocab_loss_run(const mscclx_vocab_loss* loss, const mscclx_vocab_loss
  *   norm = |scale| sqrt(sum g^2) (L2) or |scale| max |g| (MAX), over the elements of all counted tensors
  *   coefficient = min(1, max_norm / (norm + 1e-6)),  out = g scale coefficient
  * Sums are held in 64 bits and added in one order: the same bits at every call.  A NaN among the gradients makes norm,
- * coefficient and every output NaN; an infinity makes the coefficient 0 (and NaN of itself).  Without tensors the norm is 0. */
+ * coefficient and every output NaN; an infinity makes the coefficient 0 (and NaN of itself), and NaN if max_norm is infinite too.  Without tensors the norm is 0. */
 typedef enum { MSCCLX_NORM_L2 = 0, MSCCLX_NORM_MAX = 1 } mscclx_norm;
 typedef struct mscclx_grad_clip mscclx_grad_clip;
 

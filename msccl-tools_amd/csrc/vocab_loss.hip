@@ -22,7 +22,9 @@
 // once, dw was up to 1.9 times as far off as with G in 32 bits.)  With more tokens E and G are both rounded, each
 // relative to its own size (bf16 2^-8, fp16 2^-11 at the most), with 2^15 as unit in fp16, so that probabilities down
 // to 2^-29 are normal numbers; |g| is divided by its largest value for the same reason and multiplied back in 32 bits
-// behind the products.
+// behind the products.  In fp16 a token's G is therefore off by up to 2^-40 of the largest |g| in each of the two roundings,
+// whatever its own g: over 32000 rows at most 2^-24 of it times the largest |w| in the token's dx, which with both up to 1 is one
+// step of the smallest numbers that dx holds.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -347,7 +349,10 @@ struct TokenArgs {
 
 // A workgroup per token: its parts' (m, sum) -> lse and loss, and with gradients its row of x, and of G: kKeep from E,
 // in place; kLogits from the logits; kGradient: G is there and so is the lse.  Where tokens are few, several workgroups
-// share one: each works out the lse for itself (a thirtieth of what it then moves) and takes gridDim.y'ths of the row.
+// share one: each works out the lse for itself and takes gridDim.y'ths of the row, 4096 columns.  The token's statistics,
+// 8 bytes for `part` rows, are then read twice by each of them, from cache: with 32 workgroups twice what they move.  With
+// half and a quarter as many the kernel is longer all the same (1 token x 131072: 12.7 us, 13.5 and 15.7; 100 tokens 16.4,
+// 16.5 and 17.2; 1 x 32768 7.0, 8.1 and 10.2).
 // The label's own G = (p - 1) g comes from its logit in 32 bits: from a rounded p close to 1 next to nothing would be
 // left of it.
 template <class T, int MODE>
@@ -373,7 +378,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
     base = m == -INFINITY ? 0.f : m;
     for (int h = threadIdx.x; h < parts; h += 256) {
       const float2 s = stats[h];
-      sum += s.y * (s.x == base ? 1.f : exp2_of(s.x - base));  // (also where both are +inf)
+      sum += s.y * exp2_of(s.x == base ? 0.f : s.x - base);  // (also where both are +inf)
     }
     sum = block_reduce(sum, [](float a, float b) { return a + b; }, shared);
     log_sum = log2f(sum);
@@ -403,7 +408,7 @@ __global__ void __launch_bounds__(256) token_kernel(const Pieces pieces, const T
       float p[8];
       if constexpr (MODE != kLogits) {
         const float top = stats[v / a.part].x;
-        const float f = top == -INFINITY ? 0.f : top == lse2 ? g : exp2_of(top - lse2) * g;  // (both may be +inf)
+        const float f = top == -INFINITY ? 0.f : exp2_of(top == lse2 ? 0.f : top - lse2) * g;  // (both may be +inf)
         const x8 kept = *(const x8*)(e + v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = (float)kept[i] * f;
@@ -913,9 +918,10 @@ int logits_shape(const Pieces& p, int64_t tokens) {
   return middle <= kComputeUnits ? kSmall : tokens <= 128 || middle <= 2 * kComputeUnits ? kMiddle : kLarge;
 }
 // A row of x that begins within a cache line has each step's 128 bytes in two; x is copied first where that is short
-// against the product (forward and run in us, with the copy / without: 4096 x 32768 x 4104 900 / 983 and 3070 / 3180, 1500 x
-// 40000 x 2008 241 / 250 and 753 / 770, 1021 x 32003 x 1288 90 / 90 and 312 / 321; but 8192 x 8000 x 904 148 / 145, 1200 x
-// 12000 x 4000 105 / 102).  W's rows, which the same holds for, are read once: a copy of them would cost more.
+// against the product (forward and run in us, with the copy / without: 4096 x 32768 x 4104 908 / 982 and 3110 / 3210, 1500 x
+// 40000 x 2008 249 / 263 and 762 / 779; near the border 1021 x 32003 x 1288 101 / 102 and 322 / 326, 1021 x 24000 x 1800 114 /
+// 115 and 339 / 349, 1300 x 20000 x 2008 121 / 120 and 387 / 387, 1400 x 17000 x 2600 154 / 153 and 459 / 462; but 8192 x 8000
+// x 904 148 / 145, 1200 x 12000 x 4000 105 / 102).  W's rows, which the same holds for, are read once: a copy of them would cost more.
 bool align_pays(const Pieces& p, int64_t tokens, int hidden) {
   return p.tiles >= 64 && (int64_t)tiles(tokens) * p.tiles * tiles(hidden, kStepK) >= 40 * kComputeUnits;
 }
@@ -980,7 +986,7 @@ int launch_logits(int shape, const Pieces& p, LogitsArgs& a, hipStream_t stream)
     const int grid = a.token_tiles * p.tiles * (kTile / S::kL);
     // In step, all workgroups ask for the same 128 bytes of each row of W at a time.  Where rows lie a multiple of 4 KiB
     // apart those are in few of memory's channels, so every eight tiles begin at another k (128 x 65536 x 4096: 146 us, in
-    // step 175; 256 x 32768 x 2048 51 / 60, 500 x 32768 x 2048 67 / 72; not with so many tokens that W's reads hide, 4096 x
+    // step 175; 256 x 32768 x 2048 51 / 59, 500 x 32768 x 2048 68 / 79; not with so many tokens that W's reads hide, 4096 x
     // 32768 x 4096 850 / 841, nor with one tile of a few, 16 x 131072 x 4096 264 / 256).  With one workgroup of Few per
     // compute unit each begins at its own (the loss of 1 token x 32768 x 2048: 32.2 us, in step 36.2).
     a.apart = S::kR == Few::kR && grid <= kComputeUnits ? 1 : a.tokens > Few::kR && a.tokens <= 2048 && a.w_stride % 4096 == 0 ? 8 : 0;

@@ -23,7 +23,10 @@ class VocabLoss:
     and no gradient, a label outside the vocabulary makes loss and gradients NaN.
 
     Calls only enqueue kernels on the current stream and can be captured in a HIP graph, which needs the handle as it was at its capture.  A handle has one
-    workspace: its calls follow each other on one stream, or are ordered by events, and come from one thread at a time."""
+    workspace: its calls follow each other on one stream, or are ordered by events, and come from one thread at a time.
+
+    Autograd does not see the calls: what they return is detached, also from an x or weights that require gradients, and dweights
+    are overwritten, not added to.  All ranks' pieces are in this process's memory."""
 
     def __init__(self, device="cuda:0"):
         self.device = torch.device(device)
