@@ -321,3 +321,95 @@ def test_matrices_beyond_32_bit_offsets():
         for t in (dx, *dw):
             assert bool(torch.isnan(t[:, hidden:]).all())
             t[:, :hidden] = 0
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("tokens, rows, piece_bytes", [(0, [100, 30], 0), (1, [5000] * 3, 0), (20, [100, 30], 0), (100, [257], 0), (100, [64] * 9, 0), (300, [9000, 6001], 0), (600, [300, 200], 1)])
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")  # (forward of no tokens)
+def test_graphs_of_forward_backward_and_run(tokens, rows, piece_bytes, reduction):
+    """Each path captured once and replayed on other inputs, with eager calls between the replays: the same bits."""
+    op = operator(tokens, 72, rows, "bfloat16", reduction=reduction, piece_bytes=piece_bytes)
+    cases = [make(tokens, 72, rows, torch.bfloat16, seed=s) for s in range(3)]
+    up = lambda u: u if reduction == "none" else torch.tensor(0.7, device="cuda")  # noqa: E731
+    flat = lambda out: [t for part in out for t in (part if isinstance(part, list) else [part])]  # noqa: E731
+    x, weights, labels, upstream = [t.clone() if torch.is_tensor(t) else [w.clone() for w in t] for t in cases[0]]
+    given, lse = up(upstream), op.forward(x, weights, labels)[1]
+    calls = {"forward": lambda: op.forward(x, weights, labels), "backward": lambda: op.backward(x, weights, labels, lse, given), "run": lambda: op.run(x, weights, labels, given)}
+    graphs = {}
+    torch.cuda.synchronize()
+    for name, call in calls.items():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs[name] = (graph, flat(call()))
+    for nx, nw, nl, nu in cases * 2:
+        x.copy_(nx), labels.copy_(nl), upstream.copy_(nu)
+        for a, b in zip(weights, nw):
+            a.copy_(b)
+        lse.copy_(op.forward(x, weights, labels)[1])
+        for name, (graph, got) in graphs.items():
+            want = flat(calls[name]())
+            for t in got:
+                t.fill_(3.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+
+
+@pytest.mark.parametrize("norm", ["l2", "max"])
+def test_graphs_of_the_norm_alone_and_of_clipping(norm):
+    from msccl.executor import GradientClip
+    sizes = [5, 700_000, 3, 2_000_003]
+    clip = GradientClip()
+    clip.setup(sizes, "float16", out_dtype="float32", norm=norm)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    grads = [torch.zeros(n, dtype=torch.half, device="cuda") for n in sizes]
+    outs = [torch.empty(n, device="cuda") for n in sizes]
+    clip.bind(grads, outs)
+    torch.cuda.synchronize()
+    alone, both = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(alone):
+        clip.launch(scale=0.5)
+    with torch.cuda.graph(both):
+        clip.launch(max_norm=0.25, scale=0.5)
+    for _ in range(4):
+        for g in grads:
+            g.copy_(torch.randn(g.numel(), generator=gen, device="cuda"))
+        wide = torch.cat(grads).double()
+        want = 0.5 * float(wide.square().sum().sqrt() if norm == "l2" else wide.abs().max())
+        for go in (alone.replay, both.replay, lambda: clip.launch(scale=0.5), alone.replay, both.replay):
+            clip._workspace[:8].fill_(255)
+            go()
+            torch.cuda.synchronize()
+            assert clip.norm.item() == pytest.approx(want, rel=2.0 ** -23)
+            assert clip.coefficient.item() == pytest.approx(1.0 if go != both.replay else 0.25 / (want + 1e-6), rel=2.0 ** -23)
+
+
+def test_two_threads_with_handles_of_their_own():
+    """On the same stream, and on two: every call's results are its own."""
+    from concurrent.futures import ThreadPoolExecutor
+    from msccl.executor import GradientClip
+    cases = [(150, [300, 77], 1), (20, [100, 30], 2)]
+    inputs = [make(n, 72, rows, torch.bfloat16, seed=s) for n, rows, s in cases]
+    ops = [operator(n, 72, rows, "bfloat16", reduction="none") for n, rows, _ in cases]
+    clips = [GradientClip() for _ in cases]
+    want = []
+    for op, clip, data in zip(ops, clips, inputs):
+        _, _, dx, dw = op.run(*data)
+        clip.setup([t.numel() for t in dw], "bfloat16")
+        want.append((dx, dw, clip.run(dw)))
+    torch.cuda.synchronize()
+
+    def work(i, stream):
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                _, _, dx, dw = ops[i].run(*inputs[i])
+                size = clips[i].run(dw)
+                stream.synchronize()
+                if not (torch.equal(dx, want[i][0]) and all(torch.equal(a, b) for a, b in zip(dw, want[i][1])) and torch.equal(size, want[i][2])):
+                    return False
+        return True
+
+    for streams in ([torch.cuda.current_stream()] * 2, [torch.cuda.Stream(), torch.cuda.Stream()]):
+        with ThreadPoolExecutor(2) as pool:
+            assert list(pool.map(work, range(2), streams)) == [True, True]
+        torch.cuda.synchronize()
