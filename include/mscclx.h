@@ -241,10 +241,10 @@ int mscclx_plan_time(mscclx_plan* plan, void* stream, int32_t iters, float* ms_o
  * The logits are not kept (but of up to 128 tokens): tokens go through in pieces whose probabilities, 16 bits each, fit `piece_bytes`.
  * A token whose label is `ignore_index` has loss 0 and adds nothing to either gradient, whatever its x holds; one whose label lies outside the
  * vocabulary otherwise has loss and gradients NaN (and every dw is NaN then).  MEAN divides by the number of tokens that are not
- * ignored, or by 1 if all are.  A non-finite grad_loss makes its token's dx, and every dw, non-finite; no other token's dx (one number for all: those of the
- * tokens that are not ignored).  With up to 32 tokens (128, if they are fewer
- * than 16 for each rank) G is held as two 16-bit numbers; with more it is rounded to 16 bits twice, which in MSCCLX_F16 is off by up to 2^-40 of the largest |g| of the
- * call each time.
+ * ignored, or by 1 if all are.  A non-finite grad_loss makes its token's dx, and every dw, non-finite; no other token's dx
+ * (one number for all: the dx of the tokens that are not ignored).
+ * With up to 32 tokens (128, if they are fewer than 16 for each rank) G is held as two 16-bit numbers; with more it is
+ * rounded to 16 bits twice, which in MSCCLX_F16 is off by up to 2^-40 of the call's largest |g| each time.
  * What a call writes (loss, lse, dx, dweights, the workspace) may not overlap any other of its buffers (ALIASED); two
  * inputs may, and matrices whose rows are equally far apart may lie side by side in one buffer.
  * Every call only enqueues kernels on `stream`: it can be captured in a HIP graph and replayed.  Calls that share a

@@ -928,7 +928,7 @@ bool align_pays(const Pieces& p, int64_t tokens, int hidden) {
 // dw writes more than it reads where tokens are few; workgroups then hide each other's loads and stores (16 x 131072 x
 // 4096: 222 Thin / 285 Large, 200 x 20000 x 3000 47 / 55, 300 x 20000 x 1024 25 / 28 Middle; 500 x 32768 x 2048 80 / 82
 // Large, 1021 x 32003 x 1288 100 / 93).  More tokens: Large once its tiles fill the chip (1021 x 32003 x 1288: 93 / 110
-// Middle; 1024 x 4096 x 512: 29 / 20 Middle).
+// Middle; 1024 x 4096 x 512: 29 / 20 Middle).  How many of the tokens are ignored is known on the device only.
 int dw_shape(const Pieces& p, int64_t tokens, int hidden) { return tokens <= 384 ? kThin : (int64_t)p.tiles * tiles(hidden) < kComputeUnits ? kMiddle : kLarge; }
 
 // Logits in 32 bits and G twice where that decides about a rank's dw: with few tokens, or few for each rank.
